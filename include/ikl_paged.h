@@ -216,6 +216,99 @@ typedef struct ikl_rope_append_args {
  * query rows are rotated regardless. */
 int ikl_rope_append_kv(const ikl_rope_append_args *args, void *stream);
 
+/* Arguments of ikl_qk_norm_rope_append_kv: those of ikl_rope_append_kv
+ * (cache, slots, rows, tables of cos / sin) and the norms' weights and eps. */
+typedef struct ikl_qk_norm_rope_args {
+  ikl_rope_append_args rope;
+  const void *q_weight;      /* [head_dim] or [num_heads, head_dim], tensor dtype */
+  const void *k_weight;      /* [head_dim] or [num_kv_heads, head_dim] */
+  int64_t q_weight_stride_h; /* 0: one row for all heads */
+  int64_t k_weight_stride_h;
+  float eps;
+} ikl_qk_norm_rope_args;
+
+/* RMSNorm of each query and key head, rotary embedding and KV append in one
+ * launch: y = x * rsqrt(mean(x^2) + eps) * weight over a head's row, then
+ * query_out = rope(y of query), cache.k[slot] = rope(y of key), cache.v[slot]
+ * = value, rope as in ikl_rope_append_kv. fp32 throughout, rounded once at the
+ * end; into an FP8 cache the fp32 rows are quantised as ikl_append_kv does.
+ * Slots outside the cache are skipped; query rows are written regardless. Rows
+ * of a multiple of 32 bytes up to 2048. Neighbour of ikl_rope_append_kv for
+ * models that normalise their heads; the reference's model does not. */
+int ikl_qk_norm_rope_append_kv(const ikl_qk_norm_rope_args *args, void *stream);
+
+/* Arguments of ikl_copy_blocks: pages of up to four tensors [layers, blocks,
+ * page], each page a dense run of bytes (cache.k, cache.v and an FP8 cache's
+ * scales). */
+#define IKL_COPY_MAX_TENSORS 4
+typedef struct ikl_copy_blocks_args {
+  void *base[IKL_COPY_MAX_TENSORS];
+  int64_t page_bytes[IKL_COPY_MAX_TENSORS];
+  int64_t stride_layer[IKL_COPY_MAX_TENSORS]; /* BYTES, unlike the other structs */
+  int64_t stride_block[IKL_COPY_MAX_TENSORS]; /* bytes */
+  int32_t num_tensors;
+  int64_t num_layers;
+  int64_t num_blocks;
+  const void *src;           /* [num_pairs] block ids */
+  const void *dst;           /* [num_pairs] */
+  int64_t num_pairs;
+  int32_t index_type;        /* enum ikl_index_type */
+  /* 1: src / dst are host memory, read during the call. Ids outside the
+   * cache, a dst named twice and a block that is both read and written are
+   * refused. 0: device memory, not looked at on the host: pairs with an id
+   * outside the cache are skipped, and the caller keeps the written blocks
+   * apart from each other and from the read ones. */
+  int32_t pairs_on_host;
+} ikl_copy_blocks_args;
+
+/* tensor[l, dst[i]] = tensor[l, src[i]] for every pair, layer and tensor: the
+ * page copies of a forked request or of a compaction, whatever the layout
+ * inside a page. No counterpart in the reference, whose pages have one owner. */
+int ikl_copy_blocks(const ikl_copy_blocks_args *args, void *stream);
+
+/* Arguments of ikl_sample_tokens. Per-row settings are used where their
+ * pointer is not NULL, else the one value for all rows. */
+#define IKL_SAMPLE_MAX_VOCAB (1 << 22)
+typedef struct ikl_sample_args {
+  const void *logits;        /* [rows, vocab], contiguous rows */
+  int64_t logits_stride;
+  int64_t rows;
+  int64_t vocab;             /* 1 .. IKL_SAMPLE_MAX_VOCAB */
+  int32_t dtype;             /* enum ikl_dtype: F16, BF16, F32 */
+  int32_t top_k_type;        /* enum ikl_index_type of top_k_rows */
+  const void *uniform;       /* [rows] fp32 in [0, 1) */
+  const void *temperature_rows; /* [rows] fp32 or NULL */
+  const void *top_k_rows;    /* [rows] or NULL */
+  const void *top_p_rows;    /* [rows] fp32 or NULL */
+  const void *min_p_rows;    /* [rows] fp32 or NULL */
+  float temperature;         /* 0 (or less): the likeliest token */
+  float top_p;               /* 1: off */
+  float min_p;               /* 0: off */
+  int64_t top_k;             /* 0: off */
+  void *tokens;              /* [rows] int64 */
+  void *policy_logprobs;     /* [rows] fp32 or NULL: under all tokens, at the temperature */
+  void *sampling_logprobs;   /* [rows] fp32 or NULL: among the tokens kept */
+  void *workspace;           /* 16-byte aligned, ikl_sample_workspace_size bytes; NULL if 0 */
+  int64_t workspace_bytes;
+} ikl_sample_args;
+
+/* Draws one token per row. Tokens in the order of falling logit, equal ones by
+ * index; weight e^((x - max) / temperature). Kept are the first top_k; of
+ * those, the tokens whose mass before them is at most top_p times the mass of
+ * the first top_k; of those, the ones whose weight is at least min_p (the
+ * likeliest weighs 1). The token is the first whose cumulative mass exceeds
+ * uniform times the kept mass. Temperature 0 takes the first token and states
+ * log probabilities at temperature 1. NaN logits count as -inf; a row with
+ * nothing above -inf gets token -1 and log probabilities -inf; logits of +inf
+ * share all mass. Settings outside their range act as the nearest one inside.
+ * The result does not depend on how a row is split over workgroups. Replaces
+ * hf_benchmark.py:578-606. */
+int ikl_sample_tokens(const ikl_sample_args *args, void *stream);
+
+/* Bytes of workspace ikl_sample_tokens needs with these sizes; negative on
+ * invalid ones. Two calls that may overlap need a workspace each. */
+int64_t ikl_sample_workspace_size(const ikl_sample_args *args);
+
 /* Arguments of ikl_paged_prefill_attention.
  * Replaces paged_prefill_attention_sdpa (attention.py:230-321, called by the
  * batched prefill at hf_benchmark.py:491-498): the gather of the whole
@@ -313,7 +406,7 @@ int ikl_hbm_read_probe(const void *buffer, int64_t bytes, void *sink, int64_t si
  * here). A caller compares it with IKL_ABI_VERSION of the header it was
  * built against and refuses to run on a mismatch. No counterpart in the
  * reference, whose operators are Python functions. */
-#define IKL_ABI_VERSION 3
+#define IKL_ABI_VERSION 4
 int32_t ikl_abi_version(void);
 
 /* Findings of ikl_check_metadata, a bit each. */

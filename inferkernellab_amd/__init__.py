@@ -11,6 +11,7 @@ from .cache import BlockAllocator, CacheLayout, PagedKVCache
 from .ops import (
     append_kv_hip,
     append_kv_triton,
+    copy_blocks_hip,
     hip_append_available,
     hip_available,
     paged_decode_attention_hip,
@@ -28,11 +29,14 @@ from .ops import (
     PreparedDecodeStep,
     PreparedPagedAttention,
     PreparedPagedPrefill,
+    PreparedQKNormRopeAppend,
+    qk_norm_rope_append_kv_hip,
     rope_append_kv_hip,
     triton_append_available,
     triton_available,
 )
 from .runtime import InferenceRuntime, RuntimeStats
+from .sampling import PreparedSampler, sample_tokens_hip
 from .scheduler import InferenceRequest, ScheduleBatch, TokenBudgetScheduler
 
 __all__ = [
@@ -61,6 +65,11 @@ __all__ = [
     "paged_prefill_path",
     "PreparedPagedPrefill",
     "rope_append_kv_hip",
+    "copy_blocks_hip",
+    "qk_norm_rope_append_kv_hip",
+    "PreparedQKNormRopeAppend",
+    "sample_tokens_hip",
+    "PreparedSampler",
     "paged_decode_autotune_config",
     "paged_decode_grouped_autotune_config",
     "paged_decode_grouped_dot_autotune_config",

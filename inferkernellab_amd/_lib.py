@@ -27,7 +27,7 @@ IKL_PREFILL_AUTO, IKL_PREFILL_ROWS = -1, 8  # plans of ikl_paged_prefill_plan
 IKL_CHECK_LENGTH_POSITIVE, IKL_CHECK_LENGTH_CAPACITY, IKL_CHECK_BLOCK_ID, IKL_CHECK_LENGTH_MAX = 1, 2, 4, 8
 # IKL_ABI_VERSION of the header these mirrors follow; load() refuses a
 # library that reports another
-IKL_ABI_VERSION = 3
+IKL_ABI_VERSION = 4
 
 EXPORTED_SYMBOLS = (
     "ikl_last_error",
@@ -55,6 +55,10 @@ EXPORTED_SYMBOLS = (
     "ikl_paged_decode_step_workspace_size",
     "ikl_paged_attention_noalloc",
     "ikl_hbm_read_probe",
+    "ikl_qk_norm_rope_append_kv",
+    "ikl_copy_blocks",
+    "ikl_sample_tokens",
+    "ikl_sample_workspace_size",
 )
 
 _c_i64 = ctypes.c_int64
@@ -185,6 +189,71 @@ class RopeAppendArgs(ctypes.Structure):
         ("v_scale", _c_ptr),
         ("scale_stride_block", _c_i64),
         ("scale_stride_head", _c_i64),
+    ]
+
+
+class QKNormRopeArgs(ctypes.Structure):
+    """Mirror of ikl_qk_norm_rope_args."""
+
+    _fields_ = [
+        ("rope", RopeAppendArgs),
+        ("q_weight", _c_ptr),
+        ("k_weight", _c_ptr),
+        ("q_weight_stride_h", _c_i64),
+        ("k_weight_stride_h", _c_i64),
+        ("eps", ctypes.c_float),
+    ]
+
+
+COPY_MAX_TENSORS = 4  # IKL_COPY_MAX_TENSORS
+
+
+class CopyBlocksArgs(ctypes.Structure):
+    """Mirror of ikl_copy_blocks_args."""
+
+    _fields_ = [
+        ("base", _c_ptr * COPY_MAX_TENSORS),
+        ("page_bytes", _c_i64 * COPY_MAX_TENSORS),
+        ("stride_layer", _c_i64 * COPY_MAX_TENSORS),
+        ("stride_block", _c_i64 * COPY_MAX_TENSORS),
+        ("num_tensors", _c_i32),
+        ("num_layers", _c_i64),
+        ("num_blocks", _c_i64),
+        ("src", _c_ptr),
+        ("dst", _c_ptr),
+        ("num_pairs", _c_i64),
+        ("index_type", _c_i32),
+        ("pairs_on_host", _c_i32),
+    ]
+
+
+SAMPLE_MAX_VOCAB = 1 << 22  # IKL_SAMPLE_MAX_VOCAB
+
+
+class SampleArgs(ctypes.Structure):
+    """Mirror of ikl_sample_args."""
+
+    _fields_ = [
+        ("logits", _c_ptr),
+        ("logits_stride", _c_i64),
+        ("rows", _c_i64),
+        ("vocab", _c_i64),
+        ("dtype", _c_i32),
+        ("top_k_type", _c_i32),
+        ("uniform", _c_ptr),
+        ("temperature_rows", _c_ptr),
+        ("top_k_rows", _c_ptr),
+        ("top_p_rows", _c_ptr),
+        ("min_p_rows", _c_ptr),
+        ("temperature", ctypes.c_float),
+        ("top_p", ctypes.c_float),
+        ("min_p", ctypes.c_float),
+        ("top_k", _c_i64),
+        ("tokens", _c_ptr),
+        ("policy_logprobs", _c_ptr),
+        ("sampling_logprobs", _c_ptr),
+        ("workspace", _c_ptr),
+        ("workspace_bytes", _c_i64),
     ]
 
 
@@ -349,6 +418,14 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ikl_paged_decode_step_workspace_size.restype = _c_i64
     lib.ikl_paged_decode_step_workspace_size.argtypes = [ctypes.POINTER(PagedAttentionArgs),
                                                          ctypes.POINTER(AppendArgs)]
+    lib.ikl_qk_norm_rope_append_kv.restype = ctypes.c_int
+    lib.ikl_qk_norm_rope_append_kv.argtypes = [ctypes.POINTER(QKNormRopeArgs), _c_ptr]
+    lib.ikl_copy_blocks.restype = ctypes.c_int
+    lib.ikl_copy_blocks.argtypes = [ctypes.POINTER(CopyBlocksArgs), _c_ptr]
+    lib.ikl_sample_tokens.restype = ctypes.c_int
+    lib.ikl_sample_tokens.argtypes = [ctypes.POINTER(SampleArgs), _c_ptr]
+    lib.ikl_sample_workspace_size.restype = _c_i64
+    lib.ikl_sample_workspace_size.argtypes = [ctypes.POINTER(SampleArgs)]
     lib.ikl_hbm_read_probe.restype = ctypes.c_int
     lib.ikl_hbm_read_probe.argtypes = [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr]
     lib.ikl_paged_attention_launch_config.restype = ctypes.c_int

@@ -25,13 +25,16 @@ SOURCES = (
     "abi.hip",
     "append_kv.hip",
     "check_metadata.hip",
+    "copy_blocks.hip",
     "layer_ops.hip",
+    "norm_rope.hip",
     "paged_decode.hip",
     "paged_decode_mfma.hip",
     "paged_prefill.hip",
     "paged_prefill_f32.hip",
     "paged_prefill_split.hip",
     "rope_append.hip",
+    "sample.hip",
     "read_probe.hip",
 )
 

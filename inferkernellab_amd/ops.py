@@ -24,6 +24,7 @@ without the built library or a GPU it raises ``RuntimeError``.
 
 from __future__ import annotations
 
+import array
 import contextlib
 import ctypes
 
@@ -594,6 +595,22 @@ def rope_append_kv_hip(query: torch.Tensor | None, key: torch.Tensor, value: tor
     the cache are skipped.
     """
     lib = _require_backend()
+    query, query_out, key, value, cos, sin, slots = _rope_operands(query, key, value, cos, sin, cache, slots, layer,
+                                                                   query_out)
+    if key.shape[0] == 0:
+        return query_out
+    a = _lib.RopeAppendArgs()
+    _fill_rope_args(a, query, query_out, key, value, cos, sin, cache, slots, layer)
+    with torch.cuda.device(key.device):
+        stream = torch.cuda.current_stream(key.device).cuda_stream
+        status = lib.ikl_rope_append_kv(ctypes.byref(a), ctypes.c_void_p(stream))
+    _lib.check(status, "rope_append_kv")
+    return query_out
+
+
+def _rope_operands(query, key, value, cos, sin, cache, slots, layer, query_out):
+    """The checks of the rotary appends, and their tensors with rows the
+    kernels can read: (query, query_out, key, value, cos, sin, slots)."""
     layout = cache.layout
     if key.shape != value.shape or key.ndim != 3 or tuple(key.shape[1:]) != (layout.num_kv_heads, layout.head_dim):
         raise ValueError("key/value must have shape [T, Hkv, D] matching the cache layout")
@@ -620,10 +637,11 @@ def rope_append_kv_hip(query: torch.Tensor | None, key: torch.Tensor, value: tor
             query_out = query
         elif query_out.shape != query.shape or query_out.dtype != query.dtype or not _aligned_rows(query_out):
             raise ValueError("query_out must match query and have 16-byte aligned rows")
-    slots = slots.reshape(-1).contiguous()
-    if t == 0:
-        return query_out
-    a = _lib.RopeAppendArgs()
+    return query, query_out, key, value, cos, sin, slots.reshape(-1).contiguous()
+
+
+def _fill_rope_args(a, query, query_out, key, value, cos, sin, cache, slots, layer) -> None:
+    layout = cache.layout
     if query is not None:
         a.query, a.q_stride_t, a.q_stride_h = query.data_ptr(), query.stride(0), query.stride(1)
         a.query_out, a.q_out_stride_t, a.q_out_stride_h = query_out.data_ptr(), query_out.stride(0), query_out.stride(1)
@@ -638,18 +656,184 @@ def rope_append_kv_hip(query: torch.Tensor | None, key: torch.Tensor, value: tor
     a.k_cache, a.v_cache = kc.data_ptr(), vc.data_ptr()
     a.k_stride_block, a.k_stride_token, a.k_stride_head = kc.stride(0), kc.stride(1), kc.stride(2)
     a.v_stride_block, a.v_stride_token, a.v_stride_head = vc.stride(0), vc.stride(1), vc.stride(2)
-    a.num_tokens, a.num_blocks, a.block_size = t, layout.num_blocks, layout.block_size
+    a.num_tokens, a.num_blocks, a.block_size = key.shape[0], layout.num_blocks, layout.block_size
     a.num_kv_heads, a.head_dim, a.dtype = layout.num_kv_heads, layout.head_dim, _DTYPES[cache.act_dtype]
     if cache.fp8:
         ks, vs = cache.k_scale[layer], cache.v_scale[layer]
         a.cache_dtype = _lib.IKL_FP8_E4M3
         a.k_scale, a.v_scale = ks.data_ptr(), vs.data_ptr()
         a.scale_stride_block, a.scale_stride_head = ks.stride(0), ks.stride(1)
-    with torch.cuda.device(key.device):
-        stream = torch.cuda.current_stream(key.device).cuda_stream
-        status = lib.ikl_rope_append_kv(ctypes.byref(a), ctypes.c_void_p(stream))
-    _lib.check(status, "rope_append_kv")
+
+
+def _head_weight(weight, name: str, heads: int, like: torch.Tensor, head_dim: int) -> torch.Tensor:
+    """A head norm's weight, [D] for all heads or [heads, D], in rows the kernel can read."""
+    if tuple(weight.shape) not in ((head_dim,), (heads, head_dim)):
+        raise ValueError(f"{name} must have shape [head_dim] or [heads, head_dim]")
+    if weight.dtype != like.dtype or weight.device != like.device:
+        raise ValueError(f"{name} must have the dtype and device of the rows it scales")
+    return _readable(weight)
+
+
+def _readable(t: torch.Tensor | None) -> torch.Tensor | None:
+    """`t`, or a copy of it where its rows are not contiguous from 16-byte addresses."""
+    if t is None or (t.ndim and t.stride(-1) == 1 and _aligned_rows(t)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _qk_norm_rope_args(query, key, value, q_weight, k_weight, cos, sin, cache, slots, layer, eps, query_out):
+    """(argument struct, tensors it points into, query_out) of a normalised rotary append."""
+    if not eps >= 0.0:
+        raise ValueError("eps must be non-negative")
+    query, key, value, cos, sin = (_readable(x) for x in (query, key, value, cos, sin))
+    if query is not None and query_out is not None and (query_out.device != query.device
+                                                        or query_out.stride(-1) != 1):
+        raise ValueError("query_out must match query and have 16-byte aligned rows")
+    query, query_out, key, value, cos, sin, slots = _rope_operands(query, key, value, cos, sin, cache, slots, layer,
+                                                                   query_out)
+    layout = cache.layout
+    k_weight = _head_weight(k_weight, "k_weight", layout.num_kv_heads, key, layout.head_dim)
+    args = _lib.QKNormRopeArgs()
+    _fill_rope_args(args.rope, query, query_out, key, value, cos, sin, cache, slots, layer)
+    args.k_weight, args.k_weight_stride_h = k_weight.data_ptr(), k_weight.stride(0) if k_weight.ndim == 2 else 0
+    if query is not None:
+        q_weight = _head_weight(q_weight, "q_weight", query.shape[1], query, layout.head_dim)
+        args.q_weight, args.q_weight_stride_h = q_weight.data_ptr(), q_weight.stride(0) if q_weight.ndim == 2 else 0
+    args.eps = eps
+    return args, (query, query_out, key, value, q_weight, k_weight, cos, sin, slots, cache.k, cache.v), query_out
+
+
+def qk_norm_rope_append_kv_hip(query: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor,
+                               q_weight: torch.Tensor | None, k_weight: torch.Tensor, cos: torch.Tensor,
+                               sin: torch.Tensor, cache, slots: torch.Tensor, layer: int = 0, *, eps: float = 1e-6,
+                               query_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """RMSNorm of each query and key head, rotary embedding and KV append in
+    one launch, for models that normalise their heads before attention.
+
+    Arguments as :func:`rope_append_kv_hip`, and the norms' ``q_weight`` /
+    ``k_weight``, ``[head_dim]`` for all heads or one row per head, with their
+    ``eps``. ``rope(x * rsqrt(mean(x^2) + eps) * weight)`` is computed in fp32
+    and rounded once: to the tensors' dtype, or quantised into an FP8 cache.
+    Returns the normalised, rotated query (into ``query_out``, default:
+    ``query`` in place; a query whose rows have to be copied for the kernel is
+    returned as a new tensor). Rows of up to 2048 bytes, in whole 32 bytes.
+    """
+    lib = _require_backend()
+    args, keep, query_out = _qk_norm_rope_args(query, key, value, q_weight, k_weight, cos, sin, cache, slots, layer,
+                                               eps, query_out)
+    with _on_device(cache.device):
+        stream = torch.cuda.current_stream(cache.device).cuda_stream
+        status = lib.ikl_qk_norm_rope_append_kv(ctypes.byref(args), ctypes.c_void_p(stream))
+    del keep
+    _lib.check(status, "qk_norm_rope_append_kv")
     return query_out
+
+
+class PreparedQKNormRopeAppend:
+    """:func:`qk_norm_rope_append_kv_hip` checked once on fixed buffers; each
+    call only enqueues the kernel on the current stream. Tensors have to be
+    readable as they are: 16-byte aligned rows, contiguous slots."""
+
+    def __init__(self, query, key, value, q_weight, k_weight, cos, sin, cache, slots, layer: int = 0, *,
+                 eps: float = 1e-6, query_out=None):
+        self._lib = _require_backend()
+        given = (query, key, value, q_weight, k_weight, cos, sin, slots)
+        self._args, self._keep, self.query_out = _qk_norm_rope_args(*given[:7], cache, slots, layer, eps, query_out)
+        query_, _, key_, value_, q_weight_, k_weight_, cos_, sin_, slots_ = self._keep[:9]
+        bound = (query_, key_, value_, q_weight_, k_weight_, cos_, sin_, slots_)
+        if any(x is not None and x.data_ptr() != y.data_ptr() for x, y in zip(given, bound)):
+            raise ValueError("tensors of a prepared launch must have 16-byte aligned rows and contiguous slots")
+        self.device = cache.device
+
+    def __call__(self) -> torch.Tensor | None:
+        with _on_device(self.device):
+            stream = torch.cuda.current_stream(self.device).cuda_stream
+            status = self._lib.ikl_qk_norm_rope_append_kv(ctypes.byref(self._args), ctypes.c_void_p(stream))
+        _lib.check(status, "qk_norm_rope_append_kv")
+        return self.query_out
+
+
+# ------------------------------------------------------------ page copies
+def _dense_page(pages: torch.Tensor) -> bool:
+    """Whether a page ([layers, blocks, ...] indexed twice) is a dense run."""
+    run = 1
+    for size, stride in sorted(zip(pages.shape[2:], pages.stride()[2:]), key=lambda d: d[1]):
+        if size == 1:
+            continue
+        if stride != run:
+            return False
+        run *= size
+    return True
+
+
+def _copy_args(cache):
+    layout = cache.layout
+    args = _lib.CopyBlocksArgs()
+    tensors = (cache.k, cache.v) + ((cache.k_scale, cache.v_scale) if cache.fp8 else ())
+    for i, t in enumerate(tensors):
+        if not _dense_page(t):
+            raise ValueError("cache pages must be dense")
+        size = t.element_size()
+        args.base[i] = t.data_ptr()
+        args.page_bytes[i] = t[0, 0].numel() * size
+        args.stride_layer[i], args.stride_block[i] = t.stride(0) * size, t.stride(1) * size
+    args.num_tensors = len(tensors)
+    args.num_layers, args.num_blocks = layout.num_layers, layout.num_blocks
+    return args
+
+
+def copy_blocks_hip(cache, src, dst, *, validate_inputs: bool = True) -> None:
+    """Copy the pages ``src[i]`` of the cache to ``dst[i]``, all layers of K and
+    V (and an FP8 cache's scales), in one launch on the current stream.
+
+    ``src`` / ``dst``: lists of block ids on the host, or int32 / int64 GPU
+    tensors. Ids outside the cache, a page written twice and one that is both
+    read and written raise ``ValueError``; for tensors that check reads them
+    back, and ``validate_inputs=False`` leaves it out: pairs with an id outside
+    the cache are then skipped, and keeping the written pages apart is the
+    caller's part. Lists travel with the launch (a captured one keeps them);
+    tensors are read when it runs.
+    """
+    lib = _require_backend()
+    if cache.device.type != "cuda":
+        raise ValueError("the cache must be on a GPU (torch 'cuda' device)")
+    on_device = isinstance(src, torch.Tensor)
+    if on_device != isinstance(dst, torch.Tensor):
+        raise ValueError("src and dst must both be lists or both be tensors")
+    args = _copy_args(cache)
+    if on_device:
+        if src.ndim != 1 or src.shape != dst.shape:
+            raise ValueError("src and dst must have one entry per copied block")
+        if src.dtype not in _INDEX_TYPES or src.dtype != dst.dtype:
+            raise ValueError("src and dst must both use int32 or int64")
+        if src.device != cache.device or dst.device != cache.device:
+            raise ValueError("src and dst must be on the cache device")
+        if validate_inputs:
+            _check_pairs(src.tolist(), dst.tolist(), cache.layout.num_blocks)
+        src, dst = src.contiguous(), dst.contiguous()
+        args.src, args.dst, args.num_pairs = src.data_ptr(), dst.data_ptr(), src.numel()
+        args.index_type = _INDEX_TYPES[src.dtype]
+    else:
+        if len(src) != len(dst):
+            raise ValueError("src and dst must have one entry per copied block")
+        src, dst = array.array("q", src), array.array("q", dst)
+        args.src, args.dst, args.num_pairs = src.buffer_info()[0], dst.buffer_info()[0], len(src)
+        args.index_type, args.pairs_on_host = _lib.IKL_I64, 1
+    if args.num_pairs == 0:
+        return
+    with _on_device(cache.device):
+        stream = torch.cuda.current_stream(cache.device).cuda_stream
+        status = lib.ikl_copy_blocks(ctypes.byref(args), ctypes.c_void_p(stream))
+    _lib.check(status, "copy_blocks")
+
+
+def _check_pairs(src: list[int], dst: list[int], num_blocks: int) -> None:
+    if any(not 0 <= b < num_blocks for b in src) or any(not 0 <= b < num_blocks for b in dst):
+        raise ValueError("copy blocks: invalid block id")
+    if len(set(dst)) != len(dst):
+        raise ValueError("copy blocks: a block is written twice")
+    if not set(dst).isdisjoint(src):
+        raise ValueError("copy blocks: a block is both read and written")
 
 
 def _append_args(key, value, cache, slots, layer):
