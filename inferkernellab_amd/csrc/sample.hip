@@ -22,37 +22,46 @@
 namespace ikl {
 namespace {
 
+// One workgroup per row and three passes over it: the largest logit; the
+// histogram of the weights, in shared memory; the tokens of the bins where the
+// cuts fall.
 template <typename Tag>
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_row_kernel(const SampleParams p) {
   __shared__ RowShared sh;
   const int64_t b = blockIdx.x;
   const RowReader<Tag> row(p.logits + b * p.stride, p.vocab);
   const RowSettings set = row_settings(p, b);
-  // the largest logit
-  uint32_t top = 0;
+  uint32_t top = 0, least = 0xffffffffu;
   for (int v = threadIdx.x; v < row.vectors; v += SAMPLE_THREADS)
-    row.each(v, [&](int, float x) { top = max(top, order_key(x)); });
-  top = block_max(top, sh);
+    row.each(v, [&](int, float x) { extremes(x, top, least); });
+  block_extremes(top, least, sh);
   if (top <= KEY_NEG_INF) {
     if (threadIdx.x == 0) store_nothing(p, b);
     return;
   }
   const Weigher weigh(top, set.temperature, p.fraction_bits);
-  // all mass, the mass that min-p leaves, and how many tokens weigh anything
-  uint64_t total = 0, likely = 0, count = 0;
-  const double least = weigh.scaled(set.min_p);
+  const Binner bin_of(weigh, least);
+  Totals sums;
+  clear_histogram(sh);
+  __syncthreads();
   for (int v = threadIdx.x; v < row.vectors; v += SAMPLE_THREADS)
-    row.each(v, [&](int, float x) {
-      double exact;
-      const uint64_t w = weigh(x, exact);
-      total += w;
-      likely += exact >= least ? w : 0;
-      count += w != 0;
+    row.each(v, [&](int, float x) { add_token(x, set, weigh, bin_of, sums, sh); });
+  const uint64_t total = block_sum(sums.total, sh);
+  const uint64_t likely = set.min_p > 0.f ? block_sum(sums.likely, sh) : total;
+  const uint64_t count = set.top_k > 0 ? block_sum(sums.count, sh) : 0;
+  const Cuts cuts = find_cuts(set, total, likely, count, sh);
+  if (threadIdx.x == 0) sh.listed = 0;
+  __syncthreads();
+  for (int v = threadIdx.x; v < row.vectors; v += SAMPLE_THREADS)
+    row.each(v, [&](int i, float x) {
+      if (!cuts.has(bin_of(x)) || weigh(x) == 0) return;
+      const uint32_t at = atomicAdd(&sh.listed, 1u);
+      if (at < LIST) sh.list[at] = token_word(order_key(x), i);
     });
-  total = block_sum(total, sh);
-  likely = block_sum(likely, sh);
-  count = block_sum(count, sh);
-  sample_by_radix<Tag>(p, b, row, set, weigh, total, likely, count, sh);
+  __syncthreads();
+  const uint32_t n = sh.listed;
+  if (n <= LIST) sample_from_list(p, b, set, weigh, bin_of, total, likely, count, (int)n, sh);
+  else sample_by_radix<Tag>(p, b, row, set, weigh, total, likely, count, sh);
 }
 
 template <typename Tag>

@@ -1,6 +1,6 @@
 // Parts of the sampling kernels: reading a row of logits, its order, integer
-// weights, workgroup sums and scans, and the selection by radix passes that is
-// right for every row.
+// weights, workgroup sums and scans, the selection by a histogram of the
+// weights, and the one by radix passes that every row can take.
 #pragma once
 
 #include <type_traits>
@@ -11,7 +11,8 @@ namespace ikl {
 
 constexpr int SAMPLE_THREADS = 1024;
 constexpr int SAMPLE_WAVES = SAMPLE_THREADS / 64;
-constexpr int RADIX_BINS = 2048;
+constexpr int BINS = 2048;  // of a histogram
+constexpr int LIST = 2048;  // tokens of the bins where the cuts fall
 
 struct SampleParams {
   const char *logits;
@@ -180,11 +181,13 @@ __device__ inline uint64_t scaled_floor(float r, uint64_t m) {
 
 // ------------------------------------------------------- workgroup reductions
 struct RowShared {
-  uint64_t mass[RADIX_BINS];
-  uint32_t count[RADIX_BINS];
+  uint64_t mass[BINS];
+  uint32_t count[BINS];
+  uint64_t list[LIST];
   uint64_t part[SAMPLE_WAVES];
   uint64_t part2[SAMPLE_WAVES];
   uint64_t found[4];
+  uint32_t listed;
 };
 
 __device__ inline uint64_t shfl_xor64(uint64_t v, int mask) {
@@ -195,13 +198,21 @@ __device__ inline uint64_t shfl_up64(uint64_t v, int by) {
 }
 
 // Every thread of the workgroup calls these and receives the result.
-__device__ inline uint32_t block_max(uint32_t v, RowShared &sh) {
-  for (int d = 32; d; d >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d, 64));
+__device__ inline void block_extremes(uint32_t &top, uint32_t &least, RowShared &sh) {
+  for (int d = 32; d; d >>= 1) {
+    top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+    least = min(least, (uint32_t)__shfl_xor((int)least, d, 64));
+  }
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh.part[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0) {
+    sh.part[threadIdx.x >> 6] = top;
+    sh.part2[threadIdx.x >> 6] = least;
+  }
   __syncthreads();
-  for (int i = 0; i < SAMPLE_WAVES; ++i) v = max(v, (uint32_t)sh.part[i]);
-  return v;
+  for (int i = 0; i < SAMPLE_WAVES; ++i) {
+    top = max(top, (uint32_t)sh.part[i]);
+    least = min(least, (uint32_t)sh.part2[i]);
+  }
 }
 __device__ inline uint64_t block_sum(uint64_t v, RowShared &sh) {
   for (int d = 32; d; d >>= 1) v += shfl_xor64(v, d);
@@ -232,6 +243,13 @@ __device__ inline uint64_t block_before(uint64_t v, uint64_t *part, uint64_t &al
   return before + run - v;
 }
 
+// The largest key, and the smallest of those that may have a weight.
+__device__ inline void extremes(float x, uint32_t &top, uint32_t &least) {
+  const uint32_t key = order_key(x);
+  top = max(top, key);
+  least = min(least, key > KEY_NEG_INF ? key : 0xffffffffu);
+}
+
 // ----------------------------------------------------------- radix selection
 struct Selected {
   uint32_t key;     // of the group of equal logits
@@ -251,7 +269,7 @@ __device__ inline Selected radix_select(const RowReader<Tag> &row, const Weigher
     const int bits = level == 2 ? 10 : 11;
     const uint32_t mask = (1u << bits) - 1u;
     __syncthreads();
-    for (int i = threadIdx.x; i < RADIX_BINS; i += SAMPLE_THREADS) {
+    for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) {
       sh.mass[i] = 0;
       sh.count[i] = 0;
     }
@@ -276,7 +294,7 @@ __device__ inline Selected radix_select(const RowReader<Tag> &row, const Weigher
         atomicAdd(&sh.count[bin], 1u);
       });
     __syncthreads();
-    constexpr int PER = RADIX_BINS / SAMPLE_THREADS;
+    constexpr int PER = BINS / SAMPLE_THREADS;
     const int first = threadIdx.x * PER;
     uint64_t mass = 0, count = 0, all;
     for (int i = 0; i < PER; ++i) {
@@ -339,7 +357,216 @@ __device__ inline void store_token(const SampleParams &p, int64_t b, const Weigh
   if (p.sampling) p.sampling[b] = weigh.log_share(x, kept);
 }
 
-// The whole draw by radix selections: `total` the row's mass, `likely` what
+// ------------------------------------------------------ selection by a histogram
+// One histogram of the weights over their logarithm tells in which bins the
+// cuts and the draw fall; only the tokens of those bins are put in order.
+//
+// Bins are even steps of log2(w) from 0 to the row's smallest weight, at most
+// to where weights round to 0: the bin number falls with the logit, in any row.
+struct Binner {
+  double m, rate;
+  float top;
+  __device__ inline Binner(const Weigher &weigh, uint32_t least_key) : m(weigh.m), rate(0.0), top(weigh.top) {
+    const double range = fmin(((double)key_float(least_key) - weigh.m) * -weigh.rate, (double)(weigh.bits + 2));
+    if (range > 0.0) rate = weigh.rate * (-(double)BINS / range);
+  }
+  __device__ inline int operator()(float x) const {
+    const int b = x == top ? 0 : (int)fmin(((double)x - m) * rate, (double)(BINS - 1));
+    return b < 0 ? 0 : b;
+  }
+};
+
+// A thread's share of the row's mass, of what min-p leaves of it, and of the
+// tokens with a weight (the last two where the settings need them).
+struct Totals {
+  uint64_t total = 0, likely = 0, count = 0;
+};
+
+__device__ inline void clear_histogram(RowShared &sh) {
+  for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) {
+    sh.mass[i] = 0;
+    sh.count[i] = 0;
+  }
+}
+
+__device__ inline void add_token(float x, const RowSettings &set, const Weigher &weigh, const Binner &bin_of,
+                                 Totals &sums, RowShared &sh) {
+  double exact;
+  const uint64_t w = weigh(x, exact);
+  if (w == 0) return;
+  sums.total += w;
+  sums.likely += exact >= weigh.scaled(set.min_p) ? w : 0;
+  ++sums.count;
+  const int bin = bin_of(x);
+  atomicAdd((unsigned long long *)&sh.mass[bin], (unsigned long long)w);
+  if (set.top_k > 0) atomicAdd(&sh.count[bin], 1u);
+}
+
+// The bins whose tokens have to be known one by one: first and last of up to
+// three runs (where top-k, top-p and the draw may fall).
+struct Cuts {
+  int first[3], last[3];
+  __device__ inline bool has(int bin) const {
+    bool in = false;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) in |= bin >= first[i] && bin <= last[i];
+    return in;
+  }
+};
+
+// Turns the histogram in shared memory into the masses and counts before each
+// bin (counts only where top-k needs them) and finds the cuts' bins. A cut
+// that depends on an earlier one's exact place is bracketed by that one's bin.
+__device__ inline Cuts find_cuts(const RowSettings &set, uint64_t total, uint64_t likely, uint64_t count,
+                                 RowShared &sh) {
+  constexpr int PER = BINS / SAMPLE_THREADS;
+  const bool by_rank = set.top_k > 0 && (uint64_t)set.top_k < count;
+  const int first = threadIdx.x * PER;
+  uint64_t mass[PER + 1], rank[PER + 1], all, sum = 0, num = 0;
+  for (int i = 0; i < PER; ++i) {
+    mass[i + 1] = sh.mass[first + i];
+    rank[i + 1] = sh.count[first + i];
+    sum += mass[i + 1];
+    num += rank[i + 1];
+  }
+  mass[0] = block_before(sum, sh.part, all);
+  rank[0] = by_rank ? block_before(num, sh.part2, all) : 0;
+  for (int i = 0; i < PER; ++i) {
+    sh.mass[first + i] = mass[i];
+    sh.count[first + i] = (uint32_t)rank[i];
+    mass[i + 1] += mass[i];
+    rank[i + 1] += rank[i];
+  }
+  Cuts c;
+  uint64_t low = total, high = total;  // the kept mass lies between
+  for (int i = 0; i < 3; ++i) {
+    c.first[i] = 1;
+    c.last[i] = 0;
+  }
+  // the bin through which the cumulative mass exceeds `bound`, for two bounds
+  const auto bins_of = [&](uint64_t a, uint64_t b, int which) {
+    __syncthreads();
+    for (int i = 0; i < PER; ++i) {
+      if (mass[i] <= a && a < mass[i + 1]) {
+        sh.found[0] = (uint64_t)(first + i);
+        sh.found[1] = mass[i];
+      }
+      if (mass[i] <= b && b < mass[i + 1]) {
+        sh.found[2] = (uint64_t)(first + i);
+        sh.found[3] = mass[i + 1];
+      }
+    }
+    __syncthreads();
+    c.first[which] = (int)sh.found[0];
+    c.last[which] = (int)sh.found[2];
+  };
+  if (by_rank) {
+    __syncthreads();
+    for (int i = 0; i < PER; ++i)
+      if (rank[i] < (uint64_t)set.top_k && (uint64_t)set.top_k <= rank[i + 1]) {
+        sh.found[0] = (uint64_t)(first + i);
+        sh.found[1] = mass[i];
+        sh.found[3] = mass[i + 1];
+      }
+    __syncthreads();
+    c.first[0] = c.last[0] = (int)sh.found[0];
+    low = sh.found[1] + 1;
+    high = sh.found[3];
+  }
+  if (set.top_p < 1.f) {
+    bins_of(scaled_floor(set.top_p, low), scaled_floor(set.top_p, high), 1);
+    low = min(low, sh.found[1] + 1);
+    high = min(high, sh.found[3]);
+  }
+  if (set.min_p > 0.f) {
+    low = min(low, likely);
+    high = min(high, likely);
+  }
+  bins_of(scaled_floor(set.uniform, low), scaled_floor(set.uniform, high), 2);
+  return c;
+}
+
+// A listed token: its key above its index, so that falling order of the word
+// is the order of the tokens.
+__device__ inline uint64_t token_word(uint32_t key, int index) { return ((uint64_t)key << 32) | (uint32_t)~index; }
+
+// Puts the `n` words in sh.list in falling order, in place (n <= LIST; words behind them are overwritten).
+__device__ inline void sort_list(int n, RowShared &sh) {
+  int size = 64;
+  while (size < n) size <<= 1;
+  for (int i = n + threadIdx.x; i < size; i += SAMPLE_THREADS) sh.list[i] = 0;
+  for (int run = 2; run <= size; run <<= 1)
+    for (int d = run >> 1; d; d >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < size / 2; i += SAMPLE_THREADS) {
+        const int a = ((i & ~(d - 1)) << 1) | (i & (d - 1)), b = a | d;
+        const uint64_t x = sh.list[a], y = sh.list[b];
+        if ((x < y) == ((a & run) == 0)) {
+          sh.list[a] = y;
+          sh.list[b] = x;
+        }
+      }
+    }
+  __syncthreads();
+}
+
+// The draw from the `n` tokens in sh.list, all those of the cuts' bins, with
+// sh.mass and sh.count as find_cuts left them.
+__device__ inline void sample_from_list(const SampleParams &p, int64_t b, const RowSettings &set, const Weigher &weigh,
+                                        const Binner &bin_of, uint64_t total, uint64_t likely, uint64_t count, int n,
+                                        RowShared &sh) {
+  constexpr int PER = LIST / SAMPLE_THREADS;
+  sort_list(n, sh);
+  const int first = threadIdx.x * PER;
+  uint64_t before[PER], w[PER], sum = 0, all;
+  int bin[PER];
+  for (int i = 0; i < PER; ++i) {
+    const bool on = first + i < n;
+    const float x = on ? key_float((uint32_t)(sh.list[first + i] >> 32)) : 0.f;
+    w[i] = on ? weigh(x) : 0;
+    bin[i] = on ? bin_of(x) : -1;
+    before[i] = sum;
+    sum += w[i];
+  }
+  const uint64_t ahead = block_before(sum, sh.part, all);
+  // where a bin's tokens begin in the list: what stands before the bin less
+  // what stands before them here (modulo 2^64)
+  for (int i = 0; i < PER; ++i) {
+    before[i] += ahead;
+    const int at = first + i;
+    if (bin[i] < 0 || (at > 0 && bin_of(key_float((uint32_t)(sh.list[at - 1] >> 32))) == bin[i])) continue;
+    sh.mass[bin[i]] -= before[i];
+    sh.count[bin[i]] -= (uint32_t)at;
+  }
+  if (threadIdx.x == 0) sh.found[0] = sh.found[1] = 0;
+  __syncthreads();
+  const bool by_rank = set.top_k > 0 && (uint64_t)set.top_k < count;
+  for (int i = 0; i < PER; ++i) {
+    if (bin[i] < 0) continue;
+    before[i] += sh.mass[bin[i]];
+    if (by_rank && sh.count[bin[i]] + (uint32_t)(first + i) == (uint32_t)set.top_k - 1) sh.found[0] = before[i] + w[i];
+  }
+  __syncthreads();
+  uint64_t kept = by_rank ? sh.found[0] : total;
+  if (set.top_p < 1.f) {
+    const uint64_t most = scaled_floor(set.top_p, kept);
+    for (int i = 0; i < PER; ++i)
+      if (bin[i] >= 0 && before[i] <= most)
+        atomicMax((unsigned long long *)&sh.found[1], (unsigned long long)(before[i] + w[i]));
+    __syncthreads();
+    kept = min(kept, sh.found[1]);
+  }
+  if (set.min_p > 0.f) kept = min(kept, likely);
+  const uint64_t aim = scaled_floor(set.uniform, kept);
+  for (int i = 0; i < PER; ++i)
+    if (bin[i] >= 0 && before[i] <= aim && aim - before[i] < w[i]) {  // one token
+      const uint64_t word = sh.list[first + i];
+      store_token(p, b, weigh, (int)~(uint32_t)word, key_float((uint32_t)(word >> 32)), total, kept);
+    }
+}
+
+// The whole draw by radix selections, for rows whose cuts fall in bins of more
+// than LIST tokens: `total` the row's mass, `likely` what
 // min-p leaves of it, `count` the tokens with weight.
 template <typename Tag>
 __device__ inline void sample_by_radix(const SampleParams &p, int64_t b, const RowReader<Tag> &row,
