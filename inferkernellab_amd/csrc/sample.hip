@@ -25,48 +25,229 @@ namespace {
 // One workgroup per row and three passes over it: the largest logit; the
 // histogram of the weights, in shared memory; the tokens of the bins where the
 // cuts fall.
+constexpr int MAX_PARTS = 64;
+
+// The tokens of the cuts' bins among the vectors [from, to) of the row.
+template <typename Tag>
+__device__ inline void list_tokens(const RowReader<Tag> &row, int from, int to, const Binner &bin_of, const Cuts &cuts,
+                                   RowShared &sh) {
+  row.each(from, to, [&](int i, float x) {
+    if (!cuts.has(bin_of(x)) || !(x > -INFINITY)) return;
+    const uint32_t at = atomicAdd(&sh.listed, 1u);
+    if (at < LIST) sh.list[at] = token_word(order_key(clean(x)), i);
+  });
+}
+
+// One workgroup per row and three passes over it: the largest logit; the
+// histogram of the weights, in shared memory; the tokens of the bins where the
+// cuts fall.
 template <typename Tag>
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_row_kernel(const SampleParams p) {
   __shared__ RowShared sh;
   const int64_t b = blockIdx.x;
   const RowReader<Tag> row(p.logits + b * p.stride, p.vocab);
   const RowSettings set = row_settings(p, b);
-  uint32_t top = 0, least = 0xffffffffu;
-  for (int v = threadIdx.x; v < row.vectors; v += SAMPLE_THREADS)
-    row.each(v, [&](int, float x) { extremes(x, top, least); });
+  fill_roots(sh.roots);
+  clear_histogram(sh);
+  if (threadIdx.x == 0) sh.listed = 0;
+  float top = -INFINITY, least = INFINITY;
+  row.each(0, row.vectors, [&](int, float x) { extremes(x, top, least); });
   block_extremes(top, least, sh);
-  if (top <= KEY_NEG_INF) {
+  if (top == -INFINITY) {
     if (threadIdx.x == 0) store_nothing(p, b);
     return;
   }
-  const Weigher weigh(top, set.temperature, p.fraction_bits);
-  const Binner bin_of(weigh, least);
+  if (top == INFINITY) {
+    sample_infinite(p, b, row, set, sh);
+    return;
+  }
+  const Weigher weigh(top, set.temperature, p.fraction_bits, sh.roots);
+  const Binner bin_of(weigh, top, least);
   Totals sums;
-  clear_histogram(sh);
-  __syncthreads();
-  for (int v = threadIdx.x; v < row.vectors; v += SAMPLE_THREADS)
-    row.each(v, [&](int, float x) { add_token(x, set, weigh, bin_of, sums, sh); });
+  row.each(0, row.vectors, [&](int, float x) { add_token(x, set, weigh, bin_of, sums, sh); });
   const uint64_t total = block_sum(sums.total, sh);
   const uint64_t likely = set.min_p > 0.f ? block_sum(sums.likely, sh) : total;
   const uint64_t count = set.top_k > 0 ? block_sum(sums.count, sh) : 0;
   const Cuts cuts = find_cuts(set, total, likely, count, sh);
-  if (threadIdx.x == 0) sh.listed = 0;
-  __syncthreads();
-  for (int v = threadIdx.x; v < row.vectors; v += SAMPLE_THREADS)
-    row.each(v, [&](int i, float x) {
-      if (!cuts.has(bin_of(x)) || weigh(x) == 0) return;
-      const uint32_t at = atomicAdd(&sh.listed, 1u);
-      if (at < LIST) sh.list[at] = token_word(order_key(x), i);
-    });
+  list_tokens(row, 0, row.vectors, bin_of, cuts, sh);
   __syncthreads();
   const uint32_t n = sh.listed;
   if (n <= LIST) sample_from_list(p, b, set, weigh, bin_of, total, likely, count, (int)n, sh);
   else sample_by_radix<Tag>(p, b, row, set, weigh, total, likely, count, sh);
 }
 
+// A row split over the launch's workgroups, `parts` to a row: three launches
+// for the three passes. The parts' histograms and lists meet in memory, and the
+// last part of a row to finish its list draws the token. Sums of integers: the
+// order of arrival leaves no trace.
+struct SplitRow {  // of the workspace
+  uint64_t mass[BINS];
+  uint64_t list[LIST];
+  uint32_t count[BINS];
+  uint64_t total, likely, weighted;
+  uint32_t listed, arrived;
+  float top[MAX_PARTS], least[MAX_PARTS];
+};
+
+// What a row's parts hand over inside a launch is written and read by atomic
+// operations of device scope only: they take effect in memory, past the caches
+// of the 8 dies, so no cache has to be written back. (With a device-wide fence
+// in each wave instead, 32 rows of 131072 tokens took 155 us a launch.)
+template <typename T>
+__device__ inline T shared_load(const T *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ inline void shared_store(T *p, T v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Whether this workgroup is the row's last to come here. Each wave waits for its
+// own operations to be complete before the workgroup's arrival is counted.
+__device__ inline bool last_to_arrive(uint32_t *arrived, int parts, RowShared &sh) {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) sh.found[0] = atomicAdd(arrived, 1u) == (uint32_t)(parts - 1);
+  __syncthreads();
+  const bool last = sh.found[0] != 0;
+  __syncthreads();
+  return last;
+}
+
+// This workgroup's row and its vectors of it.
 template <typename Tag>
-void launch(const SampleParams &p, int64_t rows, hipStream_t s) {
-  sample_row_kernel<Tag><<<dim3((unsigned)rows), SAMPLE_THREADS, 0, s>>>(p);
+struct Part {
+  int64_t b;
+  RowReader<Tag> row;
+  int part, from, to;
+  __device__ inline Part(const SampleParams &p, int parts)
+      : b(blockIdx.x / parts), row(p.logits + b * p.stride, p.vocab), part((int)(blockIdx.x - b * parts)) {
+    const int per = (row.vectors + parts - 1) / parts;
+    from = min(part * per, row.vectors);
+    to = min(from + per, row.vectors);
+  }
+};
+
+template <typename Tag>
+__global__ __launch_bounds__(SAMPLE_THREADS) void sample_extremes_kernel(const SampleParams p, SplitRow *rows, int parts) {
+  __shared__ RowShared sh;
+  const Part<Tag> at(p, parts);
+  SplitRow &r = rows[at.b];
+  for (int i = at.part * SAMPLE_THREADS + threadIdx.x; i < BINS; i += parts * SAMPLE_THREADS) {
+    r.mass[i] = 0;
+    r.count[i] = 0;
+  }
+  float top = -INFINITY, least = INFINITY;
+  at.row.each(at.from, at.to, [&](int, float x) { extremes(x, top, least); });
+  block_extremes(top, least, sh);
+  if (threadIdx.x == 0) {
+    r.top[at.part] = top;
+    r.least[at.part] = least;
+    if (at.part == 0) {
+      r.total = r.likely = r.weighted = 0;
+      r.listed = r.arrived = 0;
+    }
+  }
+}
+
+__device__ inline void row_extremes(const SplitRow &r, int parts, float &top, float &least) {
+  const int lane = threadIdx.x & 63;  // MAX_PARTS lanes
+  top = wave_max(lane < parts ? r.top[lane] : -INFINITY);
+  least = -wave_max(lane < parts ? -r.least[lane] : -INFINITY);
+}
+
+template <typename Tag>
+__global__ __launch_bounds__(SAMPLE_THREADS) void sample_histogram_kernel(const SampleParams p, SplitRow *rows, int parts) {
+  __shared__ RowShared sh;
+  const Part<Tag> at(p, parts);
+  SplitRow &r = rows[at.b];
+  fill_roots(sh.roots);
+  clear_histogram(sh);
+  const RowSettings set = row_settings(p, at.b);
+  float top, least;
+  row_extremes(r, parts, top, least);
+  if (top == -INFINITY || top == INFINITY) return;
+  const Weigher weigh(top, set.temperature, p.fraction_bits, sh.roots);
+  const Binner bin_of(weigh, top, least);
+  Totals sums;
+  __syncthreads();
+  at.row.each(at.from, at.to, [&](int, float x) { add_token(x, set, weigh, bin_of, sums, sh); });
+  const uint64_t total = block_sum(sums.total, sh);
+  const uint64_t likely = set.min_p > 0.f ? block_sum(sums.likely, sh) : total;
+  const uint64_t count = set.top_k > 0 ? block_sum(sums.count, sh) : 0;
+  if (threadIdx.x == 0) {
+    atomicAdd((unsigned long long *)&r.total, (unsigned long long)total);
+    atomicAdd((unsigned long long *)&r.likely, (unsigned long long)likely);
+    atomicAdd((unsigned long long *)&r.weighted, (unsigned long long)count);
+  }
+  for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) {
+    if (sh.mass[i]) atomicAdd((unsigned long long *)&r.mass[i], (unsigned long long)sh.mass[i]);
+    if (sh.count[i]) atomicAdd(&r.count[i], sh.count[i]);
+  }
+}
+
+template <typename Tag>
+__global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(const SampleParams p, SplitRow *rows, int parts) {
+  __shared__ RowShared sh;
+  const Part<Tag> at(p, parts);
+  SplitRow &r = rows[at.b];
+  const RowSettings set = row_settings(p, at.b);
+  float top, least;
+  row_extremes(r, parts, top, least);
+  if (top == -INFINITY || top == INFINITY) {  // nothing to weigh
+    if (at.part != 0) return;
+    if (top == INFINITY) sample_infinite(p, at.b, at.row, set, sh);
+    else if (threadIdx.x == 0) store_nothing(p, at.b);
+    return;
+  }
+  fill_roots(sh.roots);
+  for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) {
+    sh.mass[i] = r.mass[i];
+    sh.count[i] = r.count[i];
+  }
+  if (threadIdx.x == 0) sh.listed = 0;
+  const Weigher weigh(top, set.temperature, p.fraction_bits, sh.roots);
+  const Binner bin_of(weigh, top, least);
+  const uint64_t total = r.total, likely = r.likely, count = r.weighted;
+  __syncthreads();
+  const Cuts cuts = find_cuts(set, total, likely, count, sh);
+  list_tokens(at.row, at.from, at.to, bin_of, cuts, sh);
+  __syncthreads();
+  const uint32_t mine = sh.listed;
+  if (threadIdx.x == 0) sh.found[1] = mine ? atomicAdd(&r.listed, mine) : 0;
+  __syncthreads();
+  const uint32_t start = (uint32_t)sh.found[1];  // past LIST in all, no list is read
+  for (uint32_t i = threadIdx.x; i < mine && i < LIST && start + i < LIST; i += SAMPLE_THREADS)
+    shared_store(&r.list[start + i], sh.list[i]);
+  if (!last_to_arrive(&r.arrived, parts, sh)) return;
+  const uint32_t n = shared_load(&r.listed);
+  if (n > LIST) {
+    sample_by_radix<Tag>(p, at.b, at.row, set, weigh, total, likely, count, sh);
+    return;
+  }
+  for (uint32_t i = threadIdx.x; i < n; i += SAMPLE_THREADS) sh.list[i] = shared_load(&r.list[i]);
+  __syncthreads();
+  sample_from_list(p, at.b, set, weigh, bin_of, total, likely, count, (int)n, sh);
+}
+
+// Workgroups of a row.
+int parts_of(int64_t rows, int64_t vocab, int64_t dtype) {
+  const int64_t vectors = (vocab + (dtype == IKL_F32 ? 3 : 7)) / (dtype == IKL_F32 ? 4 : 8);
+  const int64_t most = (vectors + SAMPLE_THREADS - 1) / SAMPLE_THREADS, want = (512 + rows - 1) / rows;
+  const int64_t n = most < want ? most : want;
+  return (int)(n < MAX_PARTS ? n : MAX_PARTS);
+}
+
+template <typename Tag>
+void launch(const SampleParams &p, int64_t rows, int parts, SplitRow *split, hipStream_t s) {
+  if (parts == 1) {
+    sample_row_kernel<Tag><<<dim3((unsigned)rows), SAMPLE_THREADS, 0, s>>>(p);
+    return;
+  }
+  const dim3 grid((unsigned)(rows * parts));
+  sample_extremes_kernel<Tag><<<grid, SAMPLE_THREADS, 0, s>>>(p, split, parts);
+  sample_histogram_kernel<Tag><<<grid, SAMPLE_THREADS, 0, s>>>(p, split, parts);
+  sample_pick_kernel<Tag><<<grid, SAMPLE_THREADS, 0, s>>>(p, split, parts);
 }
 
 }  // namespace
@@ -111,11 +292,16 @@ extern "C" int ikl_sample_tokens(const ikl_sample_args *a, void *stream) {
   p.sampling = (float *)a->sampling_logprobs;
   p.vocab = (int32_t)a->vocab;
   p.fraction_bits = fraction_bits(a->vocab);
+  const int parts = parts_of(a->rows, a->vocab, a->dtype);
+  if (parts > 1 && (!a->workspace || (uintptr_t)a->workspace % 16 ||
+                    a->workspace_bytes < a->rows * (int64_t)sizeof(SplitRow)))
+    return fail(IKL_EWORKSPACE, "sample: workspace missing, misaligned or too small");
+  SplitRow *split = (SplitRow *)a->workspace;
   hipStream_t s = (hipStream_t)stream;
   switch (a->dtype) {
-    case IKL_F16: launch<f16_tag>(p, a->rows, s); break;
-    case IKL_BF16: launch<bf16_tag>(p, a->rows, s); break;
-    default: launch<f32_tag>(p, a->rows, s); break;
+    case IKL_F16: launch<f16_tag>(p, a->rows, parts, split, s); break;
+    case IKL_BF16: launch<bf16_tag>(p, a->rows, parts, split, s); break;
+    default: launch<f32_tag>(p, a->rows, parts, split, s); break;
   }
   return check_launch("sample launch");
 }
@@ -123,5 +309,6 @@ extern "C" int ikl_sample_tokens(const ikl_sample_args *a, void *stream) {
 extern "C" int64_t ikl_sample_workspace_size(const ikl_sample_args *a) {
   if (!a || a->rows < 0 || a->vocab <= 0 || a->vocab > IKL_SAMPLE_MAX_VOCAB)
     return fail(IKL_EINVAL, "sample: invalid sizes");
-  return 0;
+  if (a->rows == 0 || parts_of(a->rows, a->vocab, a->dtype) == 1) return 0;
+  return a->rows * (int64_t)sizeof(SplitRow);
 }

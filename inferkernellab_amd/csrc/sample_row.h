@@ -70,8 +70,11 @@ __device__ inline float key_float(uint32_t k) {
   return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
 }
 
-// A row in 16-byte vectors from the aligned address at or below its start;
-// vectors that the row fills only in part are read by elements.
+// NaN as -inf, and one zero.
+__device__ inline float clean(float x) { return x != x ? -INFINITY : x + 0.f; }
+
+// A row in 16-byte vectors from the aligned address at or below its start.
+// Elements of the first and last vector that are not the row's read as -inf.
 template <typename Tag>
 struct RowReader {
   static constexpr int EB = std::is_same<Tag, f32_tag>::value ? 4 : 2;
@@ -86,30 +89,45 @@ struct RowReader {
     vectors = (n + shift + VEC - 1) / VEC;
   }
   __device__ inline static float value(const v4u32 &w, int j) {
-    float x;
-    if constexpr (EB == 4) x = __uint_as_float(w[j]);
-    else x = (j & 1) ? elem<Tag>::hi(w[j >> 1]) : elem<Tag>::lo(w[j >> 1]);
-    return clean(x);
+    if constexpr (EB == 4) return __uint_as_float(w[j]);
+    else return (j & 1) ? elem<Tag>::hi(w[j >> 1]) : elem<Tag>::lo(w[j >> 1]);
   }
-  __device__ inline static float clean(float x) { return x != x ? -INFINITY : x + 0.f; }
-  __device__ inline float one(int i) const {  // element i of the row
-    const char *at = base + (int64_t)(i + shift) * EB;
-    if constexpr (EB == 4) return clean(*reinterpret_cast<const float *>(at));
-    else return clean(elem<Tag>::lo(*reinterpret_cast<const uint16_t *>(at)));
-  }
-  __device__ inline bool whole(int v) const { return v * VEC >= shift && (v + 1) * VEC <= vocab + shift; }
-  __device__ inline v4u32 load(int v) const { return load16v_global(base + (int64_t)v * 16); }
-  // f(index, value) for each element of vector v, in order
-  template <typename F>
-  __device__ inline void each(int v, F f) const {
-    const int first = v * VEC - shift;
-    if (whole(v)) {
-      const v4u32 w = load(v);
+  __device__ inline v4u32 load(int v) const {
+    const char *at = base + (int64_t)v * 16;
+    if (v * VEC >= shift && (v + 1) * VEC <= vocab + shift) return load16v_global(at);
+    const uint32_t none = std::is_same<Tag, f32_tag>::value   ? 0xff800000u
+                          : std::is_same<Tag, f16_tag>::value ? 0xfc00u
+                                                              : 0xff80u;
+    v4u32 w = {0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) f(first + j, value(w, j));
-    } else {
-      for (int j = 0; j < VEC; ++j)
-        if (first + j >= 0 && first + j < vocab) f(first + j, one(first + j));
+    for (int j = 0; j < VEC; ++j) {
+      const int i = v * VEC + j - shift;
+      uint32_t e = none;
+      if (i >= 0 && i < vocab) {
+        if constexpr (EB == 4) e = reinterpret_cast<const uint32_t *>(at)[j];
+        else e = reinterpret_cast<const uint16_t *>(at)[j];
+      }
+      if constexpr (EB == 4) w[j] = e;
+      else w[j >> 1] |= e << (16 * (j & 1));
+    }
+    return w;
+  }
+  // f(index, value) for the elements of the vectors [from, to), each thread's in
+  // order; the next vector is on its way meanwhile
+  template <typename F>
+  __device__ inline void each(int from, int to, F f) const {
+    int v = from + threadIdx.x;
+    if (v >= to) return;
+    v4u32 w = load(v);
+    while (true) {
+      const int ahead = v + SAMPLE_THREADS;
+      v4u32 next = w;
+      if (ahead < to) next = load(ahead);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f(v * VEC + j - shift, value(w, j));
+      if (ahead >= to) return;
+      v = ahead;
+      w = next;
     }
   }
 };
@@ -124,48 +142,54 @@ __host__ __device__ inline int fraction_bits(int64_t vocab) {
 }
 
 // w(x) = 2^((x - m) log2(e) / T) as the nearest integer to w 2^bits, and
-// unrounded in units of 2^-bits. 2^f is its Taylor series about 0 up to f^12;
-// on |f| <= 1/2 the next term is 2.4e-16 of the value.
+// unrounded in units of 2^-bits. 2^(k/32 + r/32) for whole k and |r| <= 1/2 is
+// a power of two, one of 32 roots in shared memory (64 banks: no two entries
+// collide) and the Taylor series of 2^(r/32) up to r^5, whose next term is
+// 2.2e-15 of the value. m is finite; NaN and -inf weigh 0.
 struct Weigher {
-  float top;
-  double m, rate;
+  double m, rate;  // rate: 32 log2(e) / T
+  const double *roots;
   int bits;
-  __device__ inline Weigher(uint32_t top_key, float temperature, int fraction)
-      : top(key_float(top_key)), m(top), rate(1.4426950408889634 / (double)temperature), bits(fraction) {}
+  __device__ inline Weigher(float top, float temperature, int fraction, const double *table)
+      : m(top), rate(32.0 * 1.4426950408889634 / (double)temperature), roots(table), bits(fraction) {}
   __device__ inline double scaled(float w) const { return ldexp((double)w, bits); }
-  // log2 of the weight; NaN or -inf where x does not count
-  __device__ inline double log2w(float x) const { return x == top ? 0.0 : ((double)x - m) * rate; }
-  __device__ inline uint64_t of(double y, double &exact) const {
-    exact = 0.0;
-    if (!(y > -(double)(bits + 2))) return 0;
-    const double n = rint(y), f = y - n;
-    double p = 2.5678435993488196e-11;  // ln(2)^k / k!
-    p = fma(p, f, 4.44553827187081e-10);
-    p = fma(p, f, 7.054911620801121e-09);
-    p = fma(p, f, 1.0178086009239696e-07);
-    p = fma(p, f, 1.3215486790144305e-06);
-    p = fma(p, f, 1.5252733804059838e-05);
-    p = fma(p, f, 0.00015403530393381606);
-    p = fma(p, f, 0.0013333558146428441);
-    p = fma(p, f, 0.009618129107628477);
-    p = fma(p, f, 0.055504108664821576);
-    p = fma(p, f, 0.2402265069591007);
-    p = fma(p, f, 0.6931471805599453);
-    p = fma(p, f, 1.0);
-    exact = ldexp(p, (int)n + bits);
+  __device__ inline uint64_t operator()(float x, double &exact) const {
+    const double y = ((double)x - m) * rate;
+    const double z = y + 0x1.8p52;  // its low word: y to the nearest whole number
+    const int k = (int)(uint32_t)__double_as_longlong(z);
+    const double r = y - (z - 0x1.8p52);
+    double q = 3.9737099845494154e-11;  // (ln(2) / 32)^i / i!
+    q = fma(q, r, 9.172562701824643e-09);
+    q = fma(q, r, 1.6938509724371819e-06);
+    q = fma(q, r, 0.00023459619820224677);
+    q = fma(q, r, 0.02166084939249829);
+    q = fma(q, r, 1.0);
+    const int64_t v = __double_as_longlong(roots[k & 31] * q) + (int64_t)((uint64_t)(int64_t)((k >> 5) + bits) << 52);
+    const bool on = y > -32.0 * (bits + 2);
+    exact = on ? __longlong_as_double(v) : 0.0;
     // rounded to a whole number by the addition: doubles from 2^52 are 1 apart
     return (uint64_t)(__double_as_longlong(exact + 0x1p52) - __double_as_longlong(0x1p52));
   }
-  __device__ inline uint64_t operator()(float x, double &exact) const { return of(log2w(x), exact); }
   __device__ inline uint64_t operator()(float x) const {
     double exact;
-    return of(log2w(x), exact);
+    return (*this)(x, exact);
   }
   // ln of the share of token x in `mass`
   __device__ inline float log_share(float x, uint64_t mass) const {
-    return (float)(log2w(x) * 0.69314718055994531 - log(ldexp((double)mass, -bits)));
+    return (float)(((double)x - m) * rate * (0.69314718055994531 / 32.0) - log(ldexp((double)mass, -bits)));
   }
 };
+
+// The weights of a row whose largest logit is +inf: those tokens share all mass.
+struct InfiniteWeigher {
+  int bits;
+  __device__ inline uint64_t operator()(float x) const { return x == INFINITY ? (uint64_t)1 << bits : 0; }
+  __device__ inline float log_share(float, uint64_t mass) const { return (float)-log(ldexp((double)mass, -bits)); }
+};
+
+__device__ inline void fill_roots(double *table) {
+  if (threadIdx.x < 32) table[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
+}
 
 // floor(r m) for r in [0, 1): r is a whole number of at most 24 bits over a power of two.
 __device__ inline uint64_t scaled_floor(float r, uint64_t m) {
@@ -187,67 +211,82 @@ struct RowShared {
   uint64_t part[SAMPLE_WAVES];
   uint64_t part2[SAMPLE_WAVES];
   uint64_t found[4];
+  double roots[32];
   uint32_t listed;
 };
 
-__device__ inline uint64_t shfl_xor64(uint64_t v, int mask) {
-  return ((uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), mask, 64) << 32) | (uint32_t)__shfl_xor((int)v, mask, 64);
+// Lane permutations inside rows of 16 lanes without the LDS round trip.
+template <int CTRL>
+__device__ inline uint64_t dpp64(uint64_t v) {  // lanes without a source get 0
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, 0xf, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, 0xf, 0xf, true);
+  return ((uint64_t)hi << 32) | lo;
 }
-__device__ inline uint64_t shfl_up64(uint64_t v, int by) {
-  return ((uint64_t)(uint32_t)__shfl_up((int)(v >> 32), by, 64) << 32) | (uint32_t)__shfl_up((int)v, by, 64);
+__device__ inline uint64_t lane64(uint64_t v, int lane) {
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+// Sum over the lanes up to this one.
+__device__ inline uint64_t wave_scan(uint64_t v) {
+  v += dpp64<0x111>(v);  // row_shr 1, 2, 4, 8
+  v += dpp64<0x112>(v);
+  v += dpp64<0x114>(v);
+  v += dpp64<0x118>(v);
+  const uint64_t a = lane64(v, 15), b = a + lane64(v, 31), c = b + lane64(v, 47);
+  const int row = (threadIdx.x & 63) >> 4;
+  return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
+}
+__device__ inline float wave_max(float v) {
+  v = fmaxf(v, dpp_mov<DPP_QUAD_XOR1>(v));
+  v = fmaxf(v, dpp_mov<DPP_QUAD_XOR2>(v));
+  v = fmaxf(v, dpp_mov<DPP_ROW_HALF_MIRROR>(v));
+  v = fmaxf(v, dpp_mov<DPP_ROW_MIRROR>(v));
+  return max_xor32(max_xor16(v));
 }
 
 // Every thread of the workgroup calls these and receives the result.
-__device__ inline void block_extremes(uint32_t &top, uint32_t &least, RowShared &sh) {
-  for (int d = 32; d; d >>= 1) {
-    top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
-    least = min(least, (uint32_t)__shfl_xor((int)least, d, 64));
-  }
+__device__ inline void block_extremes(float &top, float &least, RowShared &sh) {
+  top = wave_max(top);
+  least = -wave_max(-least);
+  float *part = reinterpret_cast<float *>(sh.part);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) {
-    sh.part[threadIdx.x >> 6] = top;
-    sh.part2[threadIdx.x >> 6] = least;
+    part[threadIdx.x >> 6] = top;
+    part[SAMPLE_WAVES + (threadIdx.x >> 6)] = least;
   }
   __syncthreads();
+#pragma unroll
   for (int i = 0; i < SAMPLE_WAVES; ++i) {
-    top = max(top, (uint32_t)sh.part[i]);
-    least = min(least, (uint32_t)sh.part2[i]);
+    top = fmaxf(top, part[i]);
+    least = fminf(least, part[SAMPLE_WAVES + i]);
   }
-}
-__device__ inline uint64_t block_sum(uint64_t v, RowShared &sh) {
-  for (int d = 32; d; d >>= 1) v += shfl_xor64(v, d);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh.part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0;
-  for (int i = 0; i < SAMPLE_WAVES; ++i) v += sh.part[i];
-  return v;
 }
 // Sum of the values of the threads before this one; `all` the sum of all.
 __device__ inline uint64_t block_before(uint64_t v, uint64_t *part, uint64_t &all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t run = v;
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t up = shfl_up64(run, d);
-    if (lane >= d) run += up;
-  }
+  const int wave = threadIdx.x >> 6;
+  const uint64_t run = wave_scan(v);
   __syncthreads();
-  if (lane == 63) part[wave] = run;
+  if ((threadIdx.x & 63) == 63) part[wave] = run;
   __syncthreads();
   uint64_t before = 0;
   all = 0;
+#pragma unroll
   for (int i = 0; i < SAMPLE_WAVES; ++i) {
-    if (i < wave) before += part[i];
+    before += i < wave ? part[i] : 0;
     all += part[i];
   }
   return before + run - v;
 }
+__device__ inline uint64_t block_sum(uint64_t v, RowShared &sh) {
+  uint64_t all;
+  block_before(v, sh.part, all);
+  return all;
+}
 
-// The largest key, and the smallest of those that may have a weight.
-__device__ inline void extremes(float x, uint32_t &top, uint32_t &least) {
-  const uint32_t key = order_key(x);
-  top = max(top, key);
-  least = min(least, key > KEY_NEG_INF ? key : 0xffffffffu);
+// The largest logit, and the smallest above -inf.
+__device__ inline void extremes(float x, float &top, float &least) {
+  top = fmaxf(top, x);
+  least = fminf(least, x > -INFINITY ? x : INFINITY);
 }
 
 // ----------------------------------------------------------- radix selection
@@ -261,8 +300,8 @@ struct Selected {
 // cumulative count (BY_COUNT) or mass exceeds `bound`, which the row's total
 // does. Three passes over the row, each a histogram of the next bits of the
 // keys that are left. Tokens without weight do not count.
-template <bool BY_COUNT, typename Tag>
-__device__ inline Selected radix_select(const RowReader<Tag> &row, const Weigher &weigh, uint64_t bound, RowShared &sh) {
+template <bool BY_COUNT, typename Tag, typename W>
+__device__ inline Selected radix_select(const RowReader<Tag> &row, const W &weigh, uint64_t bound, RowShared &sh) {
   Selected s = {0, 0, 0};
   for (int level = 0; level < 3; ++level) {
     const int shift = level == 0 ? 21 : level == 1 ? 10 : 0;
@@ -274,8 +313,8 @@ __device__ inline Selected radix_select(const RowReader<Tag> &row, const Weigher
       sh.count[i] = 0;
     }
     __syncthreads();
-    for (int v = threadIdx.x; v < row.vectors; v += SAMPLE_THREADS)
-      row.each(v, [&](int, float x) {
+    row.each(0, row.vectors, [&](int, float raw) {
+        const float x = clean(raw);
         const uint32_t key = order_key(x);
         if (level > 0 && (key >> (shift + bits)) != s.key) return;
         const uint64_t w = weigh(x);
@@ -331,12 +370,19 @@ __device__ inline int nth_of_key(const RowReader<Tag> &row, uint32_t key, uint64
   for (int v0 = 0; v0 < row.vectors; v0 += SAMPLE_THREADS) {
     const int v = v0 + threadIdx.x;
     uint64_t mine = 0, all;
-    if (v < row.vectors) row.each(v, [&](int, float x) { mine += order_key(x) == key; });
+    v4u32 w = {0, 0, 0, 0};
+    if (v < row.vectors) {
+      w = row.load(v);
+#pragma unroll
+      for (int j = 0; j < RowReader<Tag>::VEC; ++j) mine += order_key(clean(row.value(w, j))) == key;
+    }
     uint64_t before = passed + block_before(mine, sh.part, all);
-    if (mine && nth >= before && nth - before < mine)
-      row.each(v, [&](int i, float x) {
-        if (order_key(x) == key && before++ == nth) sh.found[3] = (uint64_t)i;
-      });
+    if (mine && nth >= before && nth - before < mine) {
+#pragma unroll
+      for (int j = 0; j < RowReader<Tag>::VEC; ++j)
+        if (order_key(clean(row.value(w, j))) == key && before++ == nth)
+          sh.found[3] = (uint64_t)(v * RowReader<Tag>::VEC + j - row.shift);
+    }
     passed += all;
     if (passed > nth) break;
   }
@@ -350,7 +396,8 @@ __device__ inline void store_nothing(const SampleParams &p, int64_t b) {
   if (p.sampling) p.sampling[b] = -INFINITY;
 }
 
-__device__ inline void store_token(const SampleParams &p, int64_t b, const Weigher &weigh, int token, float x,
+template <typename W>
+__device__ inline void store_token(const SampleParams &p, int64_t b, const W &weigh, int token, float x,
                                    uint64_t total, uint64_t kept) {
   p.tokens[b] = token;
   if (p.policy) p.policy[b] = weigh.log_share(x, total);
@@ -361,19 +408,16 @@ __device__ inline void store_token(const SampleParams &p, int64_t b, const Weigh
 // One histogram of the weights over their logarithm tells in which bins the
 // cuts and the draw fall; only the tokens of those bins are put in order.
 //
-// Bins are even steps of log2(w) from 0 to the row's smallest weight, at most
-// to where weights round to 0: the bin number falls with the logit, in any row.
+// Bins are even steps of the logit from the largest down to the smallest, at
+// most to where weights round to 0: the bin number falls with the logit, in any
+// row, which is all that is asked of it.
 struct Binner {
-  double m, rate;
-  float top;
-  __device__ inline Binner(const Weigher &weigh, uint32_t least_key) : m(weigh.m), rate(0.0), top(weigh.top) {
-    const double range = fmin(((double)key_float(least_key) - weigh.m) * -weigh.rate, (double)(weigh.bits + 2));
-    if (range > 0.0) rate = weigh.rate * (-(double)BINS / range);
+  float top, rate;
+  __device__ inline Binner(const Weigher &weigh, float most, float least) : top(most) {
+    const double range = fmin((double)most - (double)least, 32.0 * (weigh.bits + 2) / weigh.rate);
+    rate = (float)((double)BINS / range);  // inf for a row of equal logits
   }
-  __device__ inline int operator()(float x) const {
-    const int b = x == top ? 0 : (int)fmin(((double)x - m) * rate, (double)(BINS - 1));
-    return b < 0 ? 0 : b;
-  }
+  __device__ inline int operator()(float x) const { return (int)fminf((top - x) * rate, (float)(BINS - 1)); }
 };
 
 // A thread's share of the row's mass, of what min-p leaves of it, and of the
@@ -490,9 +534,27 @@ __device__ inline Cuts find_cuts(const RowSettings &set, uint64_t total, uint64_
 // is the order of the tokens.
 __device__ inline uint64_t token_word(uint32_t key, int index) { return ((uint64_t)key << 32) | (uint32_t)~index; }
 
-// Puts the `n` words in sh.list in falling order, in place (n <= LIST; words behind them are overwritten).
+// Puts the `n` words in sh.list in falling order, in place (n <= LIST; words
+// behind them may be overwritten). Few words take their place by counting the
+// larger ones, several threads to a word: one pass, where a sorting network
+// has 36 steps for 256 words, a barrier each.
+constexpr int RANKED = 256;
+
 __device__ inline void sort_list(int n, RowShared &sh) {
-  int size = 64;
+  if (n <= RANKED) {
+    int lanes = 64;  // to a word
+    while (lanes * n > SAMPLE_THREADS) lanes >>= 1;
+    const int i = threadIdx.x / lanes, sub = threadIdx.x & (lanes - 1);
+    const uint64_t word = sh.list[i < n ? i : 0];
+    int rank = 0;
+    for (int j = sub; j < n; j += lanes) rank += sh.list[j] > word;
+    for (int d = 1; d < lanes; d <<= 1) rank += __shfl_xor(rank, d, 64);
+    __syncthreads();
+    if (sub == 0 && i < n) sh.list[rank] = word;
+    __syncthreads();
+    return;
+  }
+  int size = 2 * RANKED;
   while (size < n) size <<= 1;
   for (int i = n + threadIdx.x; i < size; i += SAMPLE_THREADS) sh.list[i] = 0;
   for (int run = 2; run <= size; run <<= 1)
@@ -566,11 +628,11 @@ __device__ inline void sample_from_list(const SampleParams &p, int64_t b, const 
 }
 
 // The whole draw by radix selections, for rows whose cuts fall in bins of more
-// than LIST tokens: `total` the row's mass, `likely` what
-// min-p leaves of it, `count` the tokens with weight.
-template <typename Tag>
+// than LIST tokens: `total` the row's mass, `likely` what min-p leaves of it,
+// `count` the tokens with weight.
+template <typename Tag, typename W>
 __device__ inline void sample_by_radix(const SampleParams &p, int64_t b, const RowReader<Tag> &row,
-                                       const RowSettings &set, const Weigher &weigh, uint64_t total, uint64_t likely,
+                                       const RowSettings &set, const W &weigh, uint64_t total, uint64_t likely,
                                        uint64_t count, RowShared &sh) {
   uint64_t kept = total;
   if (set.top_k > 0 && (uint64_t)set.top_k < count) {
@@ -589,6 +651,17 @@ __device__ inline void sample_by_radix(const SampleParams &p, int64_t b, const R
   const float x = key_float(s.key);
   const int token = nth_of_key(row, s.key, (aim - s.mass) / weigh(x), sh);
   if (threadIdx.x == 0) store_token(p, b, weigh, token, x, total, kept);
+}
+
+// A row whose largest logit is +inf: one group of equal tokens.
+template <typename Tag>
+__device__ inline void sample_infinite(const SampleParams &p, int64_t b, const RowReader<Tag> &row,
+                                       const RowSettings &set, RowShared &sh) {
+  const InfiniteWeigher weigh = {p.fraction_bits};
+  uint64_t count = 0;
+  row.each(0, row.vectors, [&](int, float x) { count += x == INFINITY; });
+  count = block_sum(count, sh);
+  sample_by_radix<Tag>(p, b, row, set, weigh, count << p.fraction_bits, count << p.fraction_bits, count, sh);
 }
 
 }  // namespace ikl
