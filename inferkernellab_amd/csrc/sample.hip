@@ -29,10 +29,11 @@ constexpr int MAX_PARTS = 64;
 
 // The tokens of the cuts' bins among the vectors [from, to) of the row.
 template <typename Tag>
-__device__ inline void list_tokens(const RowReader<Tag> &row, int from, int to, const Binner &bin_of, const Cuts &cuts,
-                                   RowShared &sh) {
+__device__ inline void list_tokens(const RowReader<Tag> &row, int from, int to, const Weigher &weigh,
+                                   const Binner &bin_of, RowShared &sh) {
+  const Cuts cuts = sh.cuts;
   row.each(from, to, [&](int i, float x) {
-    if (!cuts.has(bin_of(x)) || !(x > -INFINITY)) return;
+    if (!cuts.has(bin_of(x)) || !weigh.counts(x)) return;
     const uint32_t at = atomicAdd(&sh.listed, 1u);
     if (at < LIST) sh.list[at] = token_word(order_key(clean(x)), i);
   });
@@ -42,7 +43,7 @@ __device__ inline void list_tokens(const RowReader<Tag> &row, int from, int to, 
 // histogram of the weights, in shared memory; the tokens of the bins where the
 // cuts fall.
 template <typename Tag>
-__global__ __launch_bounds__(SAMPLE_THREADS) void sample_row_kernel(const SampleParams p) {
+__global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_row_kernel(const SampleParams p) {
   __shared__ RowShared sh;
   const int64_t b = blockIdx.x;
   const RowReader<Tag> row(p.logits + b * p.stride, p.vocab);
@@ -63,17 +64,20 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_row_kernel(const Sample
   }
   const Weigher weigh(top, set.temperature, p.fraction_bits, sh.roots);
   const Binner bin_of(weigh, top, least);
-  Totals sums;
-  row.each(0, row.vectors, [&](int, float x) { add_token(x, set, weigh, bin_of, sums, sh); });
-  const uint64_t total = block_sum(sums.total, sh);
-  const uint64_t likely = set.min_p > 0.f ? block_sum(sums.likely, sh) : total;
-  const uint64_t count = set.top_k > 0 ? block_sum(sums.count, sh) : 0;
-  const Cuts cuts = find_cuts(set, total, likely, count, sh);
-  list_tokens(row, 0, row.vectors, bin_of, cuts, sh);
+  const double lowest = weigh.scaled(set.min_p);
+  uint64_t likely = 0;
+  row.each(0, row.vectors, [&](int, float x) { add_token(x, set, weigh, lowest, bin_of, likely, sh); });
+  if (set.min_p > 0.f) {
+    likely = block_sum(likely, sh);
+    if (threadIdx.x == 0) sh.likely = likely;
+  }
+  __syncthreads();
+  find_cuts(set, sh);
+  list_tokens(row, 0, row.vectors, weigh, bin_of, sh);
   __syncthreads();
   const uint32_t n = sh.listed;
-  if (n <= LIST) sample_from_list(p, b, set, weigh, bin_of, total, likely, count, (int)n, sh);
-  else sample_by_radix<Tag>(p, b, row, set, weigh, total, likely, count, sh);
+  if (n <= LIST) sample_from_list(p, b, set, weigh, bin_of, (int)n, sh);
+  else sample_by_radix<Tag>(p, b, row, set, weigh, sh);
 }
 
 // A row split over the launch's workgroups, `parts` to a row: three launches
@@ -84,7 +88,7 @@ struct SplitRow {  // of the workspace
   uint64_t mass[BINS];
   uint64_t list[LIST];
   uint32_t count[BINS];
-  uint64_t total, likely, weighted;
+  uint64_t likely;
   uint32_t listed, arrived;
   float top[MAX_PARTS], least[MAX_PARTS];
 };
@@ -144,7 +148,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_extremes_kernel(const S
     r.top[at.part] = top;
     r.least[at.part] = least;
     if (at.part == 0) {
-      r.total = r.likely = r.weighted = 0;
+      r.likely = 0;
       r.listed = r.arrived = 0;
     }
   }
@@ -169,17 +173,15 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_histogram_kernel(const 
   if (top == -INFINITY || top == INFINITY) return;
   const Weigher weigh(top, set.temperature, p.fraction_bits, sh.roots);
   const Binner bin_of(weigh, top, least);
-  Totals sums;
+  const double lowest = weigh.scaled(set.min_p);
+  uint64_t likely = 0;
   __syncthreads();
-  at.row.each(at.from, at.to, [&](int, float x) { add_token(x, set, weigh, bin_of, sums, sh); });
-  const uint64_t total = block_sum(sums.total, sh);
-  const uint64_t likely = set.min_p > 0.f ? block_sum(sums.likely, sh) : total;
-  const uint64_t count = set.top_k > 0 ? block_sum(sums.count, sh) : 0;
-  if (threadIdx.x == 0) {
-    atomicAdd((unsigned long long *)&r.total, (unsigned long long)total);
-    atomicAdd((unsigned long long *)&r.likely, (unsigned long long)likely);
-    atomicAdd((unsigned long long *)&r.weighted, (unsigned long long)count);
+  at.row.each(at.from, at.to, [&](int, float x) { add_token(x, set, weigh, lowest, bin_of, likely, sh); });
+  if (set.min_p > 0.f) {
+    likely = block_sum(likely, sh);
+    if (threadIdx.x == 0) atomicAdd((unsigned long long *)&r.likely, (unsigned long long)likely);
   }
+  __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) {
     if (sh.mass[i]) atomicAdd((unsigned long long *)&r.mass[i], (unsigned long long)sh.mass[i]);
     if (sh.count[i]) atomicAdd(&r.count[i], sh.count[i]);
@@ -187,7 +189,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_histogram_kernel(const 
 }
 
 template <typename Tag>
-__global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(const SampleParams p, SplitRow *rows, int parts) {
+__global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_pick_kernel(const SampleParams p, SplitRow *rows, int parts) {
   __shared__ RowShared sh;
   const Part<Tag> at(p, parts);
   SplitRow &r = rows[at.b];
@@ -205,13 +207,15 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(const Sampl
     sh.mass[i] = r.mass[i];
     sh.count[i] = r.count[i];
   }
-  if (threadIdx.x == 0) sh.listed = 0;
+  if (threadIdx.x == 0) {
+    sh.listed = 0;
+    sh.likely = r.likely;
+  }
   const Weigher weigh(top, set.temperature, p.fraction_bits, sh.roots);
   const Binner bin_of(weigh, top, least);
-  const uint64_t total = r.total, likely = r.likely, count = r.weighted;
   __syncthreads();
-  const Cuts cuts = find_cuts(set, total, likely, count, sh);
-  list_tokens(at.row, at.from, at.to, bin_of, cuts, sh);
+  find_cuts(set, sh);
+  list_tokens(at.row, at.from, at.to, weigh, bin_of, sh);
   __syncthreads();
   const uint32_t mine = sh.listed;
   if (threadIdx.x == 0) sh.found[1] = mine ? atomicAdd(&r.listed, mine) : 0;
@@ -222,12 +226,12 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(const Sampl
   if (!last_to_arrive(&r.arrived, parts, sh)) return;
   const uint32_t n = shared_load(&r.listed);
   if (n > LIST) {
-    sample_by_radix<Tag>(p, at.b, at.row, set, weigh, total, likely, count, sh);
+    sample_by_radix<Tag>(p, at.b, at.row, set, weigh, sh);
     return;
   }
   for (uint32_t i = threadIdx.x; i < n; i += SAMPLE_THREADS) sh.list[i] = shared_load(&r.list[i]);
   __syncthreads();
-  sample_from_list(p, at.b, set, weigh, bin_of, total, likely, count, (int)n, sh);
+  sample_from_list(p, at.b, set, weigh, bin_of, (int)n, sh);
 }
 
 // Workgroups of a row.

@@ -145,34 +145,40 @@ __host__ __device__ inline int fraction_bits(int64_t vocab) {
 // unrounded in units of 2^-bits. 2^(k/32 + r/32) for whole k and |r| <= 1/2 is
 // a power of two, one of 32 roots in shared memory (64 banks: no two entries
 // collide) and the Taylor series of 2^(r/32) up to r^5, whose next term is
-// 2.2e-15 of the value. m is finite; NaN and -inf weigh 0.
+// 2.2e-15 of the value. m is finite; tokens that round to no unit, NaN and -inf
+// have no weight. The products and sums are fused where it says so and nowhere
+// else: a token weighs the same in every kernel.
 struct Weigher {
-  double m, rate;  // rate: 32 log2(e) / T
+  double m, rate, floor;  // rate: 32 log2(e) / T; floor: of x - m, just above half a unit
   const double *roots;
   int bits;
   __device__ inline Weigher(float top, float temperature, int fraction, const double *table)
-      : m(top), rate(32.0 * 1.4426950408889634 / (double)temperature), roots(table), bits(fraction) {}
+      : m(top), rate(32.0 * 1.4426950408889634 / (double)temperature), roots(table), bits(fraction) {
+    floor = -32.0 * (fraction + 1 - 1e-9) / rate;
+  }
   __device__ inline double scaled(float w) const { return ldexp((double)w, bits); }
-  __device__ inline uint64_t operator()(float x, double &exact) const {
-    const double y = ((double)x - m) * rate;
-    const double z = y + 0x1.8p52;  // its low word: y to the nearest whole number
+  __device__ inline bool counts(float x) const { return (double)x - m > floor; }
+  // of a token that counts
+  __device__ inline uint64_t of(float x, double &exact) const {
+#pragma clang fp contract(off)
+    const double d = (double)x - m;
+    const double z = fma(d, rate, 0x1.8p52);  // its low word: the nearest whole number
     const int k = (int)(uint32_t)__double_as_longlong(z);
-    const double r = y - (z - 0x1.8p52);
+    const double r = fma(d, rate, -(z - 0x1.8p52));
     double q = 3.9737099845494154e-11;  // (ln(2) / 32)^i / i!
     q = fma(q, r, 9.172562701824643e-09);
     q = fma(q, r, 1.6938509724371819e-06);
     q = fma(q, r, 0.00023459619820224677);
     q = fma(q, r, 0.02166084939249829);
     q = fma(q, r, 1.0);
-    const int64_t v = __double_as_longlong(roots[k & 31] * q) + (int64_t)((uint64_t)(int64_t)((k >> 5) + bits) << 52);
-    const bool on = y > -32.0 * (bits + 2);
-    exact = on ? __longlong_as_double(v) : 0.0;
+    const double v = roots[k & 31] * q;
+    exact = __hiloint2double(__double2hiint(v) + (((k >> 5) + bits) << 20), __double2loint(v));
     // rounded to a whole number by the addition: doubles from 2^52 are 1 apart
     return (uint64_t)(__double_as_longlong(exact + 0x1p52) - __double_as_longlong(0x1p52));
   }
   __device__ inline uint64_t operator()(float x) const {
     double exact;
-    return (*this)(x, exact);
+    return counts(x) ? of(x, exact) : 0;
   }
   // ln of the share of token x in `mass`
   __device__ inline float log_share(float x, uint64_t mass) const {
@@ -204,6 +210,18 @@ __device__ inline uint64_t scaled_floor(float r, uint64_t m) {
 }
 
 // ------------------------------------------------------- workgroup reductions
+// The bins whose tokens have to be known one by one: up to three runs (where
+// top-k, top-p and the draw may fall), as first bin and length less one.
+struct Cuts {
+  uint32_t first[3], span[3];
+  __device__ inline bool has(int bin) const {
+    bool in = false;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) in |= (uint32_t)bin - first[i] <= span[i];
+    return in;
+  }
+};
+
 struct RowShared {
   uint64_t mass[BINS];
   uint32_t count[BINS];
@@ -212,7 +230,9 @@ struct RowShared {
   uint64_t part2[SAMPLE_WAVES];
   uint64_t found[4];
   double roots[32];
-  uint32_t listed;
+  Cuts cuts;
+  uint64_t total, likely;    // mass of the row, and what min-p leaves of it
+  uint32_t weighted, listed; // tokens with a weight (where top-k asks), tokens in the list
 };
 
 // Lane permutations inside rows of 16 lanes without the LDS round trip.
@@ -226,56 +246,57 @@ __device__ inline uint64_t lane64(uint64_t v, int lane) {
   return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) |
          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
-// Sum over the lanes up to this one.
-__device__ inline uint64_t wave_scan(uint64_t v) {
+// Sum over the lanes of a row of 16 up to this one.
+__device__ inline uint64_t row_scan(uint64_t v) {
   v += dpp64<0x111>(v);  // row_shr 1, 2, 4, 8
   v += dpp64<0x112>(v);
   v += dpp64<0x114>(v);
   v += dpp64<0x118>(v);
+  return v;
+}
+__device__ inline uint64_t wave_scan(uint64_t v) {
+  v = row_scan(v);
   const uint64_t a = lane64(v, 15), b = a + lane64(v, 31), c = b + lane64(v, 47);
   const int row = (threadIdx.x & 63) >> 4;
   return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
 }
-__device__ inline float wave_max(float v) {
+__device__ inline float row_max(float v) {
   v = fmaxf(v, dpp_mov<DPP_QUAD_XOR1>(v));
   v = fmaxf(v, dpp_mov<DPP_QUAD_XOR2>(v));
   v = fmaxf(v, dpp_mov<DPP_ROW_HALF_MIRROR>(v));
-  v = fmaxf(v, dpp_mov<DPP_ROW_MIRROR>(v));
-  return max_xor32(max_xor16(v));
+  return fmaxf(v, dpp_mov<DPP_ROW_MIRROR>(v));
 }
+__device__ inline float wave_max(float v) { return max_xor32(max_xor16(row_max(v))); }
 
-// Every thread of the workgroup calls these and receives the result.
+// Every thread of the workgroup calls these and receives the result. The waves'
+// values are joined in the lanes of each wave, not in a loop: these run once or
+// twice a row, and code that runs once is paid for by fetching it.
+static_assert(SAMPLE_WAVES == 16, "a row of lanes holds the waves' values");
 __device__ inline void block_extremes(float &top, float &least, RowShared &sh) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   top = wave_max(top);
-  least = -wave_max(-least);
+  least = wave_max(-least);
   float *part = reinterpret_cast<float *>(sh.part);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    part[threadIdx.x >> 6] = top;
-    part[SAMPLE_WAVES + (threadIdx.x >> 6)] = least;
+  if (lane == 0) {
+    part[wave] = top;
+    part[SAMPLE_WAVES + wave] = least;
   }
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < SAMPLE_WAVES; ++i) {
-    top = fmaxf(top, part[i]);
-    least = fminf(least, part[SAMPLE_WAVES + i]);
-  }
+  const int both = __float_as_int(row_max(part[lane & 31]));
+  top = __int_as_float(__builtin_amdgcn_readlane(both, 0));
+  least = -__int_as_float(__builtin_amdgcn_readlane(both, 16));
 }
 // Sum of the values of the threads before this one; `all` the sum of all.
 __device__ inline uint64_t block_before(uint64_t v, uint64_t *part, uint64_t &all) {
-  const int wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint64_t run = wave_scan(v);
   __syncthreads();
-  if ((threadIdx.x & 63) == 63) part[wave] = run;
+  if (lane == 63) part[wave] = run;
   __syncthreads();
-  uint64_t before = 0;
-  all = 0;
-#pragma unroll
-  for (int i = 0; i < SAMPLE_WAVES; ++i) {
-    before += i < wave ? part[i] : 0;
-    all += part[i];
-  }
-  return before + run - v;
+  const uint64_t sums = row_scan(part[lane & 15]);
+  all = lane64(sums, 15);
+  return (wave ? lane64(sums, wave - 1) : 0) + run - v;
 }
 __device__ inline uint64_t block_sum(uint64_t v, RowShared &sh) {
   uint64_t all;
@@ -414,16 +435,10 @@ __device__ inline void store_token(const SampleParams &p, int64_t b, const W &we
 struct Binner {
   float top, rate;
   __device__ inline Binner(const Weigher &weigh, float most, float least) : top(most) {
-    const double range = fmin((double)most - (double)least, 32.0 * (weigh.bits + 2) / weigh.rate);
+    const double range = fmin((double)most - (double)least, -weigh.floor);
     rate = (float)((double)BINS / range);  // inf for a row of equal logits
   }
   __device__ inline int operator()(float x) const { return (int)fminf((top - x) * rate, (float)(BINS - 1)); }
-};
-
-// A thread's share of the row's mass, of what min-p leaves of it, and of the
-// tokens with a weight (the last two where the settings need them).
-struct Totals {
-  uint64_t total = 0, likely = 0, count = 0;
 };
 
 __device__ inline void clear_histogram(RowShared &sh) {
@@ -433,101 +448,95 @@ __device__ inline void clear_histogram(RowShared &sh) {
   }
 }
 
-__device__ inline void add_token(float x, const RowSettings &set, const Weigher &weigh, const Binner &bin_of,
-                                 Totals &sums, RowShared &sh) {
+// Adds a token to the histogram, and to `likely` where min-p keeps it.
+__device__ inline void add_token(float x, const RowSettings &set, const Weigher &weigh, double least,
+                                 const Binner &bin_of, uint64_t &likely, RowShared &sh) {
+  if (!weigh.counts(x)) return;
   double exact;
-  const uint64_t w = weigh(x, exact);
-  if (w == 0) return;
-  sums.total += w;
-  sums.likely += exact >= weigh.scaled(set.min_p) ? w : 0;
-  ++sums.count;
+  const uint64_t w = weigh.of(x, exact);
   const int bin = bin_of(x);
   atomicAdd((unsigned long long *)&sh.mass[bin], (unsigned long long)w);
   if (set.top_k > 0) atomicAdd(&sh.count[bin], 1u);
+  if (set.min_p > 0.f) likely += exact >= least ? w : 0;
 }
 
-// The bins whose tokens have to be known one by one: first and last of up to
-// three runs (where top-k, top-p and the draw may fall).
-struct Cuts {
-  int first[3], last[3];
-  __device__ inline bool has(int bin) const {
-    bool in = false;
-#pragma unroll
-    for (int i = 0; i < 3; ++i) in |= bin >= first[i] && bin <= last[i];
-    return in;
-  }
-};
+// The last bin whose `before` is at most `bound`: with less than the row's total
+// for a bound, the one that the cumulative count or mass exceeds it in. By the
+// 64 lanes of a wave, in two looks.
+template <typename T>
+__device__ inline int bin_at(const T *before, uint64_t bound) {
+  constexpr int STEP = BINS / 64;
+  static_assert(STEP <= 64, "two looks");
+  const int lane = threadIdx.x & 63;
+  const int part = __popcll(__ballot((uint64_t)before[lane * STEP] <= bound)) - 1;
+  return part * STEP + __popcll(__ballot(lane < STEP && (uint64_t)before[part * STEP + lane % STEP] <= bound)) - 1;
+}
 
 // Turns the histogram in shared memory into the masses and counts before each
-// bin (counts only where top-k needs them) and finds the cuts' bins. A cut
-// that depends on an earlier one's exact place is bracketed by that one's bin.
-__device__ inline Cuts find_cuts(const RowSettings &set, uint64_t total, uint64_t likely, uint64_t count,
-                                 RowShared &sh) {
+// bin (counts only where top-k needs them), with the row's total, and finds the
+// cuts' bins, into sh.cuts. A cut that depends on an earlier one's exact place
+// is bracketed by that one's bin.
+__device__ inline void find_cuts(const RowSettings &set, RowShared &sh) {
   constexpr int PER = BINS / SAMPLE_THREADS;
-  const bool by_rank = set.top_k > 0 && (uint64_t)set.top_k < count;
-  const int first = threadIdx.x * PER;
-  uint64_t mass[PER + 1], rank[PER + 1], all, sum = 0, num = 0;
+  const int at = threadIdx.x * PER;
+  uint64_t mass[PER], total, sum = 0;
+#pragma unroll
   for (int i = 0; i < PER; ++i) {
-    mass[i + 1] = sh.mass[first + i];
-    rank[i + 1] = sh.count[first + i];
-    sum += mass[i + 1];
-    num += rank[i + 1];
+    mass[i] = sum;
+    sum += sh.mass[at + i];
   }
-  mass[0] = block_before(sum, sh.part, all);
-  rank[0] = by_rank ? block_before(num, sh.part2, all) : 0;
-  for (int i = 0; i < PER; ++i) {
-    sh.mass[first + i] = mass[i];
-    sh.count[first + i] = (uint32_t)rank[i];
-    mass[i + 1] += mass[i];
-    rank[i + 1] += rank[i];
-  }
-  Cuts c;
-  uint64_t low = total, high = total;  // the kept mass lies between
-  for (int i = 0; i < 3; ++i) {
-    c.first[i] = 1;
-    c.last[i] = 0;
-  }
-  // the bin through which the cumulative mass exceeds `bound`, for two bounds
-  const auto bins_of = [&](uint64_t a, uint64_t b, int which) {
-    __syncthreads();
+  const uint64_t before = block_before(sum, sh.part, total);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sh.mass[at + i] = before + mass[i];
+  uint64_t weighted = 0;
+  if (set.top_k > 0) {
+    uint64_t rank[PER];
+    sum = 0;
+#pragma unroll
     for (int i = 0; i < PER; ++i) {
-      if (mass[i] <= a && a < mass[i + 1]) {
-        sh.found[0] = (uint64_t)(first + i);
-        sh.found[1] = mass[i];
-      }
-      if (mass[i] <= b && b < mass[i + 1]) {
-        sh.found[2] = (uint64_t)(first + i);
-        sh.found[3] = mass[i + 1];
-      }
+      rank[i] = sum;
+      sum += sh.count[at + i];
     }
-    __syncthreads();
-    c.first[which] = (int)sh.found[0];
-    c.last[which] = (int)sh.found[2];
-  };
-  if (by_rank) {
-    __syncthreads();
-    for (int i = 0; i < PER; ++i)
-      if (rank[i] < (uint64_t)set.top_k && (uint64_t)set.top_k <= rank[i + 1]) {
-        sh.found[0] = (uint64_t)(first + i);
-        sh.found[1] = mass[i];
-        sh.found[3] = mass[i + 1];
-      }
-    __syncthreads();
-    c.first[0] = c.last[0] = (int)sh.found[0];
-    low = sh.found[1] + 1;
-    high = sh.found[3];
+    const uint64_t ahead = block_before(sum, sh.part2, weighted);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sh.count[at + i] = (uint32_t)(ahead + rank[i]);
   }
-  if (set.top_p < 1.f) {
-    bins_of(scaled_floor(set.top_p, low), scaled_floor(set.top_p, high), 1);
-    low = min(low, sh.found[1] + 1);
-    high = min(high, sh.found[3]);
+  if (threadIdx.x == 0) {
+    sh.total = total;
+    sh.weighted = (uint32_t)weighted;
   }
-  if (set.min_p > 0.f) {
-    low = min(low, likely);
-    high = min(high, likely);
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const auto end = [&](int bin) { return bin + 1 < BINS ? sh.mass[bin + 1] : total; };
+    Cuts c;
+    const auto run = [&](int i, int first, int last) {
+      c.first[i] = (uint32_t)first;
+      c.span[i] = (uint32_t)(last - first);
+    };
+    run(0, 2 * BINS, 2 * BINS);  // no bin
+    run(1, 2 * BINS, 2 * BINS);
+    uint64_t low = total, high = total;  // the kept mass lies between
+    if (set.top_k > 0 && (uint64_t)set.top_k < weighted) {
+      const int bin = bin_at(sh.count, (uint64_t)set.top_k - 1);
+      run(0, bin, bin);
+      low = sh.mass[bin] + 1;
+      high = end(bin);
+    }
+    if (set.top_p < 1.f) {
+      const int first = bin_at(sh.mass, scaled_floor(set.top_p, low));
+      const int last = bin_at(sh.mass, scaled_floor(set.top_p, high));
+      run(1, first, last);
+      low = min(low, sh.mass[first] + 1);
+      high = min(high, end(last));
+    }
+    if (set.min_p > 0.f) {
+      low = min(low, sh.likely);
+      high = min(high, sh.likely);
+    }
+    run(2, bin_at(sh.mass, scaled_floor(set.uniform, low)), bin_at(sh.mass, scaled_floor(set.uniform, high)));
+    if (threadIdx.x == 0) sh.cuts = c;
   }
-  bins_of(scaled_floor(set.uniform, low), scaled_floor(set.uniform, high), 2);
-  return c;
+  __syncthreads();
 }
 
 // A listed token: its key above its index, so that falling order of the word
@@ -537,8 +546,9 @@ __device__ inline uint64_t token_word(uint32_t key, int index) { return ((uint64
 // Puts the `n` words in sh.list in falling order, in place (n <= LIST; words
 // behind them may be overwritten). Few words take their place by counting the
 // larger ones, several threads to a word: one pass, where a sorting network
-// has 36 steps for 256 words, a barrier each.
-constexpr int RANKED = 256;
+// has 45 steps for 512 words, a barrier each.
+constexpr int RANKED = 512;
+static_assert(RANKED <= SAMPLE_THREADS, "a word has at least one thread");
 
 __device__ inline void sort_list(int n, RowShared &sh) {
   if (n <= RANKED) {
@@ -547,7 +557,13 @@ __device__ inline void sort_list(int n, RowShared &sh) {
     const int i = threadIdx.x / lanes, sub = threadIdx.x & (lanes - 1);
     const uint64_t word = sh.list[i < n ? i : 0];
     int rank = 0;
-    for (int j = sub; j < n; j += lanes) rank += sh.list[j] > word;
+    for (int j0 = sub; j0 < n; j0 += 8 * lanes) {
+      uint64_t other[8];  // eight loads on their way at a time
+#pragma unroll
+      for (int u = 0; u < 8; ++u) other[u] = sh.list[min(j0 + u * lanes, LIST - 1)];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) rank += j0 + u * lanes < n && other[u] > word;
+    }
     for (int d = 1; d < lanes; d <<= 1) rank += __shfl_xor(rank, d, 64);
     __syncthreads();
     if (sub == 0 && i < n) sh.list[rank] = word;
@@ -575,8 +591,7 @@ __device__ inline void sort_list(int n, RowShared &sh) {
 // The draw from the `n` tokens in sh.list, all those of the cuts' bins, with
 // sh.mass and sh.count as find_cuts left them.
 __device__ inline void sample_from_list(const SampleParams &p, int64_t b, const RowSettings &set, const Weigher &weigh,
-                                        const Binner &bin_of, uint64_t total, uint64_t likely, uint64_t count, int n,
-                                        RowShared &sh) {
+                                        const Binner &bin_of, int n, RowShared &sh) {
   constexpr int PER = LIST / SAMPLE_THREADS;
   sort_list(n, sh);
   const int first = threadIdx.x * PER;
@@ -602,14 +617,14 @@ __device__ inline void sample_from_list(const SampleParams &p, int64_t b, const 
   }
   if (threadIdx.x == 0) sh.found[0] = sh.found[1] = 0;
   __syncthreads();
-  const bool by_rank = set.top_k > 0 && (uint64_t)set.top_k < count;
+  const bool by_rank = set.top_k > 0 && (uint32_t)set.top_k < sh.weighted;
   for (int i = 0; i < PER; ++i) {
     if (bin[i] < 0) continue;
     before[i] += sh.mass[bin[i]];
     if (by_rank && sh.count[bin[i]] + (uint32_t)(first + i) == (uint32_t)set.top_k - 1) sh.found[0] = before[i] + w[i];
   }
   __syncthreads();
-  uint64_t kept = by_rank ? sh.found[0] : total;
+  uint64_t kept = by_rank ? sh.found[0] : sh.total;
   if (set.top_p < 1.f) {
     const uint64_t most = scaled_floor(set.top_p, kept);
     for (int i = 0; i < PER; ++i)
@@ -618,24 +633,23 @@ __device__ inline void sample_from_list(const SampleParams &p, int64_t b, const 
     __syncthreads();
     kept = min(kept, sh.found[1]);
   }
-  if (set.min_p > 0.f) kept = min(kept, likely);
+  if (set.min_p > 0.f) kept = min(kept, sh.likely);
   const uint64_t aim = scaled_floor(set.uniform, kept);
   for (int i = 0; i < PER; ++i)
     if (bin[i] >= 0 && before[i] <= aim && aim - before[i] < w[i]) {  // one token
       const uint64_t word = sh.list[first + i];
-      store_token(p, b, weigh, (int)~(uint32_t)word, key_float((uint32_t)(word >> 32)), total, kept);
+      store_token(p, b, weigh, (int)~(uint32_t)word, key_float((uint32_t)(word >> 32)), sh.total, kept);
     }
 }
 
 // The whole draw by radix selections, for rows whose cuts fall in bins of more
-// than LIST tokens: `total` the row's mass, `likely` what min-p leaves of it,
-// `count` the tokens with weight.
+// than LIST tokens; sh.total, sh.likely and sh.weighted hold the row's.
 template <typename Tag, typename W>
 __device__ inline void sample_by_radix(const SampleParams &p, int64_t b, const RowReader<Tag> &row,
-                                       const RowSettings &set, const W &weigh, uint64_t total, uint64_t likely,
-                                       uint64_t count, RowShared &sh) {
+                                       const RowSettings &set, const W &weigh, RowShared &sh) {
+  const uint64_t total = sh.total;
   uint64_t kept = total;
-  if (set.top_k > 0 && (uint64_t)set.top_k < count) {
+  if (set.top_k > 0 && (uint32_t)set.top_k < sh.weighted) {
     const Selected s = radix_select<true>(row, weigh, (uint64_t)set.top_k - 1, sh);
     kept = s.mass + ((uint64_t)set.top_k - s.count) * weigh(key_float(s.key));
   }
@@ -645,7 +659,7 @@ __device__ inline void sample_by_radix(const SampleParams &p, int64_t b, const R
     const uint64_t w = weigh(key_float(s.key));
     kept = min(kept, s.mass + ((most - s.mass) / w + 1) * w);
   }
-  if (set.min_p > 0.f) kept = min(kept, likely);
+  if (set.min_p > 0.f) kept = min(kept, sh.likely);
   const uint64_t aim = scaled_floor(set.uniform, kept);
   const Selected s = radix_select<false>(row, weigh, aim, sh);
   const float x = key_float(s.key);
@@ -661,7 +675,12 @@ __device__ inline void sample_infinite(const SampleParams &p, int64_t b, const R
   uint64_t count = 0;
   row.each(0, row.vectors, [&](int, float x) { count += x == INFINITY; });
   count = block_sum(count, sh);
-  sample_by_radix<Tag>(p, b, row, set, weigh, count << p.fraction_bits, count << p.fraction_bits, count, sh);
+  if (threadIdx.x == 0) {
+    sh.total = sh.likely = count << p.fraction_bits;
+    sh.weighted = (uint32_t)count;
+  }
+  __syncthreads();
+  sample_by_radix<Tag>(p, b, row, set, weigh, sh);
 }
 
 }  // namespace ikl
