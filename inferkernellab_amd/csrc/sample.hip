@@ -22,20 +22,41 @@
 namespace ikl {
 namespace {
 
-// One workgroup per row and three passes over it: the largest logit; the
-// histogram of the weights, in shared memory; the tokens of the bins where the
-// cuts fall.
+// The draw of a row whose cuts' bins hold `n` tokens, listed if they are at most LIST.
+template <typename Tag>
+__device__ inline void draw(const SampleParams &p, int64_t b, const RowReader<Tag> &row, const RowSettings &set,
+                            const Weigher &weigh, const Binner &bin_of, uint32_t n, RowShared &sh) {
+  if (n > LIST) sample_by_radix<Tag>(p, b, row, set, weigh, sh);
+  else if (n > 64) sample_from_list(p, b, set, weigh, bin_of, (int)n, sh);
+  else if (threadIdx.x < 64) sample_from_few(p, b, set, weigh, bin_of, (int)n, sh);
+}
+
 constexpr int MAX_PARTS = 64;
 
 // The tokens of the cuts' bins among the vectors [from, to) of the row.
 template <typename Tag>
 __device__ inline void list_tokens(const RowReader<Tag> &row, int from, int to, const Weigher &weigh,
-                                   const Binner &bin_of, RowShared &sh) {
+                                   const Candidates &cand, const Binner &bin_of, RowShared &sh) {
   const Cuts cuts = sh.cuts;
-  row.each(from, to, [&](int i, float x) {
-    if (!cuts.has(bin_of(x)) || !weigh.counts(x)) return;
-    const uint32_t at = atomicAdd(&sh.listed, 1u);
-    if (at < LIST) sh.list[at] = token_word(order_key(clean(x)), i);
+  row.each(from, to, [&](int first, const float(&x)[RowReader<Tag>::VEC]) {
+    uint32_t hits = 0;
+#pragma unroll
+    for (int j = 0; j < RowReader<Tag>::VEC; ++j) hits |= (uint32_t)cuts.has(bin_of(x[j])) << j;
+    while (hits) {
+      const int j = __ffs(hits) - 1;
+      hits &= hits - 1;
+      float y = x[0];
+#pragma unroll
+      for (int k = 1; k < RowReader<Tag>::VEC; ++k) y = j == k ? x[k] : y;
+      if (!weigh.counts(y)) continue;
+      if (cand.alone) {
+        double exact;
+        weigh.of(y, exact);
+        if (exact < cand.least) continue;
+      }
+      const uint32_t at = atomicAdd(&sh.listed, 1u);
+      if (at < LIST) sh.list[at] = token_word(order_key(clean(y)), first + j);
+    }
   });
 }
 
@@ -43,7 +64,7 @@ __device__ inline void list_tokens(const RowReader<Tag> &row, int from, int to, 
 // histogram of the weights, in shared memory; the tokens of the bins where the
 // cuts fall.
 template <typename Tag>
-__global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_row_kernel(const SampleParams p) {
+__global__ __launch_bounds__(SAMPLE_THREADS) void sample_row_kernel(const SampleParams p) {
   __shared__ RowShared sh;
   const int64_t b = blockIdx.x;
   const RowReader<Tag> row(p.logits + b * p.stride, p.vocab);
@@ -52,7 +73,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_row_kernel(const Sam
   clear_histogram(sh);
   if (threadIdx.x == 0) sh.listed = 0;
   float top = -INFINITY, least = INFINITY;
-  row.each(0, row.vectors, [&](int, float x) { extremes(x, top, least); });
+  row.each(0, row.vectors, [&](int, const float(&x)[RowReader<Tag>::VEC]) { extremes(x, top, least); });
   block_extremes(top, least, sh);
   if (top == -INFINITY) {
     if (threadIdx.x == 0) store_nothing(p, b);
@@ -63,21 +84,20 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_row_kernel(const Sam
     return;
   }
   const Weigher weigh(top, set.temperature, p.fraction_bits, sh.roots);
-  const Binner bin_of(weigh, top, least);
-  const double lowest = weigh.scaled(set.min_p);
-  uint64_t likely = 0;
-  row.each(0, row.vectors, [&](int, float x) { add_token(x, set, weigh, lowest, bin_of, likely, sh); });
-  if (set.min_p > 0.f) {
-    likely = block_sum(likely, sh);
-    if (threadIdx.x == 0) sh.likely = likely;
-  }
+  const Candidates cand(set, weigh);
+  const Binner bin_of(set, weigh, cand, top, least);
+  uint64_t others = 0;
+  row.each(0, row.vectors, [&](int, const float(&x)[RowReader<Tag>::VEC]) {
+    add_tokens(x, set, weigh, cand, bin_of, others, sh);
+  });
+  if (set.min_p > 0.f) others = block_sum(others, sh);
+  if (threadIdx.x == 0) sh.others = others;
   __syncthreads();
-  find_cuts(set, sh);
-  list_tokens(row, 0, row.vectors, weigh, bin_of, sh);
+  find_cuts(set, cand, sh);
+  list_tokens(row, 0, row.vectors, weigh, cand, bin_of, sh);
   __syncthreads();
   const uint32_t n = sh.listed;
-  if (n <= LIST) sample_from_list(p, b, set, weigh, bin_of, (int)n, sh);
-  else sample_by_radix<Tag>(p, b, row, set, weigh, sh);
+  draw(p, b, row, set, weigh, bin_of, n, sh);
 }
 
 // A row split over the launch's workgroups, `parts` to a row: three launches
@@ -86,9 +106,9 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_row_kernel(const Sam
 // order of arrival leaves no trace.
 struct SplitRow {  // of the workspace
   uint64_t mass[BINS];
-  uint64_t list[LIST];
+  double list[LIST];
   uint32_t count[BINS];
-  uint64_t likely;
+  uint64_t others;
   uint32_t listed, arrived;
   float top[MAX_PARTS], least[MAX_PARTS];
 };
@@ -142,13 +162,13 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_extremes_kernel(const S
     r.count[i] = 0;
   }
   float top = -INFINITY, least = INFINITY;
-  at.row.each(at.from, at.to, [&](int, float x) { extremes(x, top, least); });
+  at.row.each(at.from, at.to, [&](int, const float(&x)[RowReader<Tag>::VEC]) { extremes(x, top, least); });
   block_extremes(top, least, sh);
   if (threadIdx.x == 0) {
     r.top[at.part] = top;
     r.least[at.part] = least;
     if (at.part == 0) {
-      r.likely = 0;
+      r.others = 0;
       r.listed = r.arrived = 0;
     }
   }
@@ -172,14 +192,16 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_histogram_kernel(const 
   row_extremes(r, parts, top, least);
   if (top == -INFINITY || top == INFINITY) return;
   const Weigher weigh(top, set.temperature, p.fraction_bits, sh.roots);
-  const Binner bin_of(weigh, top, least);
-  const double lowest = weigh.scaled(set.min_p);
-  uint64_t likely = 0;
+  const Candidates cand(set, weigh);
+  const Binner bin_of(set, weigh, cand, top, least);
+  uint64_t others = 0;
   __syncthreads();
-  at.row.each(at.from, at.to, [&](int, float x) { add_token(x, set, weigh, lowest, bin_of, likely, sh); });
+  at.row.each(at.from, at.to, [&](int, const float(&x)[RowReader<Tag>::VEC]) {
+    add_tokens(x, set, weigh, cand, bin_of, others, sh);
+  });
   if (set.min_p > 0.f) {
-    likely = block_sum(likely, sh);
-    if (threadIdx.x == 0) atomicAdd((unsigned long long *)&r.likely, (unsigned long long)likely);
+    others = block_sum(others, sh);
+    if (threadIdx.x == 0) atomicAdd((unsigned long long *)&r.others, (unsigned long long)others);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) {
@@ -209,13 +231,14 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_pick_kernel(const Sa
   }
   if (threadIdx.x == 0) {
     sh.listed = 0;
-    sh.likely = r.likely;
+    sh.others = r.others;
   }
   const Weigher weigh(top, set.temperature, p.fraction_bits, sh.roots);
-  const Binner bin_of(weigh, top, least);
+  const Candidates cand(set, weigh);
+  const Binner bin_of(set, weigh, cand, top, least);
   __syncthreads();
-  find_cuts(set, sh);
-  list_tokens(at.row, at.from, at.to, weigh, bin_of, sh);
+  find_cuts(set, cand, sh);
+  list_tokens(at.row, at.from, at.to, weigh, cand, bin_of, sh);
   __syncthreads();
   const uint32_t mine = sh.listed;
   if (threadIdx.x == 0) sh.found[1] = mine ? atomicAdd(&r.listed, mine) : 0;
@@ -225,21 +248,17 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_pick_kernel(const Sa
     shared_store(&r.list[start + i], sh.list[i]);
   if (!last_to_arrive(&r.arrived, parts, sh)) return;
   const uint32_t n = shared_load(&r.listed);
-  if (n > LIST) {
-    sample_by_radix<Tag>(p, at.b, at.row, set, weigh, sh);
-    return;
-  }
-  for (uint32_t i = threadIdx.x; i < n; i += SAMPLE_THREADS) sh.list[i] = shared_load(&r.list[i]);
+  for (uint32_t i = threadIdx.x; i < n && i < LIST; i += SAMPLE_THREADS) sh.list[i] = shared_load(&r.list[i]);
   __syncthreads();
-  sample_from_list(p, at.b, set, weigh, bin_of, (int)n, sh);
+  draw(p, at.b, at.row, set, weigh, bin_of, n, sh);
 }
 
 // Workgroups of a row.
 int parts_of(int64_t rows, int64_t vocab, int64_t dtype) {
   const int64_t vectors = (vocab + (dtype == IKL_F32 ? 3 : 7)) / (dtype == IKL_F32 ? 4 : 8);
-  const int64_t most = (vectors + SAMPLE_THREADS - 1) / SAMPLE_THREADS, want = (512 + rows - 1) / rows;
+  const int64_t most = (vectors + SAMPLE_THREADS - 1) / SAMPLE_THREADS, want = 256 / rows;
   const int64_t n = most < want ? most : want;
-  return (int)(n < MAX_PARTS ? n : MAX_PARTS);
+  return (int)(n < 1 ? 1 : n < MAX_PARTS ? n : MAX_PARTS);
 }
 
 template <typename Tag>
