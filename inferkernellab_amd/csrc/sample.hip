@@ -62,7 +62,8 @@ __device__ inline void list_tokens(const RowReader<Tag> &row, int from, int to, 
 
 // One workgroup per row and three passes over it: the largest logit; the
 // histogram of the weights, in shared memory; the tokens of the bins where the
-// cuts fall.
+// cuts fall, unless min-p left so few candidates that the second pass has listed
+// them all.
 template <typename Tag>
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_row_kernel(const SampleParams p) {
   __shared__ RowShared sh;
@@ -87,16 +88,22 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_row_kernel(const Sample
   const Candidates cand(set, weigh);
   const Binner bin_of(set, weigh, cand, top, least);
   uint64_t others = 0;
-  row.each(0, row.vectors, [&](int, const float(&x)[RowReader<Tag>::VEC]) {
-    add_tokens(x, set, weigh, cand, bin_of, others, sh);
+  row.each(0, row.vectors, [&](int first, const float(&x)[RowReader<Tag>::VEC]) {
+    add_tokens<true>(first, x, set, weigh, cand, bin_of, others, sh);
   });
   if (set.min_p > 0.f) others = block_sum(others, sh);
   if (threadIdx.x == 0) sh.others = others;
   __syncthreads();
   find_cuts(set, cand, sh);
-  list_tokens(row, 0, row.vectors, weigh, cand, bin_of, sh);
-  __syncthreads();
-  const uint32_t n = sh.listed;
+  uint32_t n = sh.listed;
+  if (!cand.alone || n > LIST) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    list_tokens(row, 0, row.vectors, weigh, cand, bin_of, sh);
+    __syncthreads();
+    n = sh.listed;
+  }
   draw(p, b, row, set, weigh, bin_of, n, sh);
 }
 
@@ -196,8 +203,8 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_histogram_kernel(const 
   const Binner bin_of(set, weigh, cand, top, least);
   uint64_t others = 0;
   __syncthreads();
-  at.row.each(at.from, at.to, [&](int, const float(&x)[RowReader<Tag>::VEC]) {
-    add_tokens(x, set, weigh, cand, bin_of, others, sh);
+  at.row.each(at.from, at.to, [&](int first, const float(&x)[RowReader<Tag>::VEC]) {
+    add_tokens<false>(first, x, set, weigh, cand, bin_of, others, sh);
   });
   if (set.min_p > 0.f) {
     others = block_sum(others, sh);
@@ -253,10 +260,15 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_pick_kernel(const Sa
   draw(p, at.b, at.row, set, weigh, bin_of, n, sh);
 }
 
-// Workgroups of a row.
+// Workgroups of a row: one where it has up to 4 vectors a thread (us, one / split
+// by 4: 1 x 32000 bf16 17.7 / 17.7 and 16 x 32000 20.0 / 20.3, one launch for
+// three; 61 x 50257, 6.1 vectors, 31.9 / 30.0), else enough for 2 vectors a
+// thread as long as there is a compute unit for each (32 x 131072 bf16 in 1, 4, 8
+// and 16: 59.7, 33.4, 29.1, 32; 256 x 131072 fp32 in 1 and 4: 76, 110).
 int parts_of(int64_t rows, int64_t vocab, int64_t dtype) {
-  const int64_t vectors = (vocab + (dtype == IKL_F32 ? 3 : 7)) / (dtype == IKL_F32 ? 4 : 8);
-  const int64_t most = (vectors + SAMPLE_THREADS - 1) / SAMPLE_THREADS, want = 256 / rows;
+  const int64_t per = dtype == IKL_F32 ? 4 : 8, vectors = (vocab + per - 1) / per;
+  if (vectors <= 4 * SAMPLE_THREADS) return 1;
+  const int64_t most = (vectors + 2 * SAMPLE_THREADS - 1) / (2 * SAMPLE_THREADS), want = 256 / rows;
   const int64_t n = most < want ? most : want;
   return (int)(n < 1 ? 1 : n < MAX_PARTS ? n : MAX_PARTS);
 }

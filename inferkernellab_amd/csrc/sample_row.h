@@ -450,6 +450,22 @@ __device__ inline void clear_histogram(RowShared &sh) {
   }
 }
 
+// A listed token: its key above its index, so that falling order of the word
+// is the order of the tokens. Held as the double of these bits (positive,
+// finite and normal): doubles are put in order by one instruction each way.
+constexpr int INDEX_BITS = 22;
+static_assert((1 << INDEX_BITS) >= IKL_SAMPLE_MAX_VOCAB, "an index fits");
+__device__ inline double token_word(uint32_t key, int index) {
+  return __longlong_as_double((1ll << 62) | ((int64_t)key << INDEX_BITS) | ((1 << INDEX_BITS) - 1 - index));
+}
+__device__ inline float word_logit(double word) {
+  return key_float((uint32_t)((uint64_t)__double_as_longlong(word) >> INDEX_BITS));
+}
+__device__ inline int word_index(double word) {
+  const int mask = (1 << INDEX_BITS) - 1;
+  return mask - ((int)__double_as_longlong(word) & mask);
+}
+
 // What min-p makes of the tokens it leaves out. They are no candidates, and
 // where the first k need not be weighed without them, only their mass counts
 // (top-p's share is of it too): they stay out of the histogram.
@@ -480,8 +496,9 @@ struct Binner {
 // Adds tokens to the histogram, and to `others` those that are no candidates.
 // All weights first, whether they count or not (an empty asm keeps them there):
 // one takes a chain of 15 fp64 operations, and the chains overlap.
-template <int N>
-__device__ inline void add_tokens(const float (&x)[N], const RowSettings &set, const Weigher &weigh,
+// LISTED: those that are alone in the histogram go to sh.list as well.
+template <bool LISTED, int N>
+__device__ inline void add_tokens(int index, const float (&x)[N], const RowSettings &set, const Weigher &weigh,
                                   const Candidates &cand, const Binner &bin_of, uint64_t &others, RowShared &sh) {
   uint64_t w[N];
   double exact[N];
@@ -501,6 +518,10 @@ __device__ inline void add_tokens(const float (&x)[N], const RowSettings &set, c
       const int bin = bin_of(x[j]);
       atomicAdd((unsigned long long *)&sh.mass[bin], (unsigned long long)w[j]);
       if (set.top_k > 0) atomicAdd(&sh.count[bin], 1u);
+      if (LISTED && cand.alone) {
+        const uint32_t at = atomicAdd(&sh.listed, 1u);
+        if (at < LIST) sh.list[at] = token_word(order_key(clean(x[j])), index + j);
+      }
     }
   }
 }
@@ -583,22 +604,6 @@ __device__ inline void find_cuts(const RowSettings &set, const Candidates &cand,
     }
   }
   __syncthreads();
-}
-
-// A listed token: its key above its index, so that falling order of the word
-// is the order of the tokens. Held as the double of these bits (positive,
-// finite and normal): doubles are put in order by one instruction each way.
-constexpr int INDEX_BITS = 22;
-static_assert((1 << INDEX_BITS) >= IKL_SAMPLE_MAX_VOCAB, "an index fits");
-__device__ inline double token_word(uint32_t key, int index) {
-  return __longlong_as_double((1ll << 62) | ((int64_t)key << INDEX_BITS) | ((1 << INDEX_BITS) - 1 - index));
-}
-__device__ inline float word_logit(double word) {
-  return key_float((uint32_t)((uint64_t)__double_as_longlong(word) >> INDEX_BITS));
-}
-__device__ inline int word_index(double word) {
-  const int mask = (1 << INDEX_BITS) - 1;
-  return mask - ((int)__double_as_longlong(word) & mask);
 }
 
 // The word of the lane whose number differs in bit D.
