@@ -14,6 +14,7 @@ namespace ikl {
 namespace {
 
 constexpr int PAIRS = 384;  // 3 KB of the 4 KB of arguments
+constexpr int FEW = 16;
 constexpr int COPY_THREADS = 256;
 constexpr int UNITS = 4;    // pieces a thread has in flight
 
@@ -28,8 +29,9 @@ struct CopyParams {
   int32_t num_layers;
   int32_t num_tensors;
 };
+template <int N>
 struct HostPairs {
-  int32_t src[PAIRS], dst[PAIRS];
+  int32_t src[N], dst[N];
   __device__ inline int64_t from(int64_t i) const { return src[i]; }
   __device__ inline int64_t to(int64_t i) const { return dst[i]; }
 };
@@ -102,19 +104,24 @@ int check_pairs(const IdxT *src, const IdxT *dst, int64_t count, int64_t blocks)
   return IKL_OK;
 }
 
+template <int N, typename IdxT>
+int launch_host(const CopyParams &p, int unit, const IdxT *src, const IdxT *dst, int64_t count, hipStream_t s) {
+  HostPairs<N> pairs;
+  for (int64_t j = 0; j < N; ++j) {
+    pairs.src[j] = j < count ? (int32_t)src[j] : -1;
+    pairs.dst[j] = j < count ? (int32_t)dst[j] : -1;
+  }
+  return launch(p, unit, pairs, count, s);
+}
+
 template <typename IdxT>
 int copy_host(const CopyParams &p, int unit, const void *src, const void *dst, int64_t count, hipStream_t s) {
   const IdxT *from = (const IdxT *)src, *to = (const IdxT *)dst;
   if (const int bad = check_pairs(from, to, count, p.num_blocks); bad != IKL_OK) return bad;
-  for (int64_t i = 0; i < count; i += PAIRS) {
-    HostPairs pairs;
-    const int64_t n = count - i < PAIRS ? count - i : PAIRS;
-    for (int64_t j = 0; j < PAIRS; ++j) {
-      pairs.src[j] = j < n ? (int32_t)from[i + j] : -1;
-      pairs.dst[j] = j < n ? (int32_t)to[i + j] : -1;
-    }
-    if (const int bad = launch(p, unit, pairs, n, s); bad != IKL_OK) return bad;
-  }
+  if (count <= FEW) return launch_host<FEW>(p, unit, from, to, count, s);
+  for (int64_t i = 0; i < count; i += PAIRS)
+    if (const int bad = launch_host<PAIRS>(p, unit, from + i, to + i, count - i < PAIRS ? count - i : PAIRS, s); bad != IKL_OK)
+      return bad;
   return IKL_OK;
 }
 

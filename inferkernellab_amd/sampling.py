@@ -21,7 +21,7 @@ import math
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _INDEX_TYPES, _on_device, _require_backend
+from .ops import _DTYPES, _INDEX_TYPES, _on_device, _require_backend, _stream
 
 
 def _setting(value, name: str, rows: int, device: torch.device, fits, wanted: str):
@@ -111,8 +111,7 @@ class PreparedSampler:
 
     def __call__(self):
         with _on_device(self.device):
-            stream = torch.cuda.current_stream(self.device).cuda_stream
-            status = self._lib.ikl_sample_tokens(ctypes.byref(self._args), ctypes.c_void_p(stream))
+            status = self._lib.ikl_sample_tokens(ctypes.byref(self._args), _stream(self.device))
         _lib.check(status, "sample")
         return self._out
 
