@@ -1,7 +1,11 @@
 // Pages of the cache copied to other pages over all layers: the copies of a
 // forked request or of a compaction. A page is a dense run of bytes in every
 // layout of the cache, so it is copied as such; K, V and an FP8 cache's scales
-// go in one launch. Bound: memory.
+// go in one launch. Bound: memory. The stores are non-temporal: what is written
+// is not read again soon, and kept out of the caches it leaves them to the reads
+// (32 pages of 32 layers, 134 MB: 31.0 -> 24.4 us, 5.5 TB/s; 512 of 16 layers, 1.07
+// GB: 224 -> 221 us, 4.9 TB/s, where a plain copy of 1 GiB runs at 5.2). 2 or 8
+// pieces a thread and workgroups of 512 are within 3 % of these.
 //
 // A list of pairs that the host holds travels in the launch's arguments, PAIRS
 // at a time: no upload, no wait, and a captured launch keeps its pairs.
@@ -42,6 +46,14 @@ struct DevicePairs {
   __device__ inline int64_t to(int64_t i) const { return (int64_t)dst[i]; }
 };
 
+template <typename Unit>
+__device__ inline void store_out(Unit *p, const Unit &v) {
+  *p = v;
+}
+__device__ inline void store_out(u32x4 *p, const u32x4 &v) {
+  __builtin_nontemporal_store((v4u32){v.x, v.y, v.z, v.w}, reinterpret_cast<v4u32 *>(p));
+}
+
 template <typename Unit, typename Pairs>
 __global__ __launch_bounds__(COPY_THREADS) void copy_blocks_kernel(const CopyParams p, const Pairs pairs) {
   // workgroup = (pair, layer, part of the page's tensors)
@@ -63,7 +75,7 @@ __global__ __launch_bounds__(COPY_THREADS) void copy_blocks_kernel(const CopyPar
     if (first + i * COPY_THREADS < t.units) u[i] = src[first + i * COPY_THREADS];
 #pragma unroll
   for (int i = 0; i < UNITS; ++i)
-    if (first + i * COPY_THREADS < t.units) dst[first + i * COPY_THREADS] = u[i];
+    if (first + i * COPY_THREADS < t.units) store_out(dst + first + i * COPY_THREADS, u[i]);
 }
 
 template <typename Unit, typename Pairs>
