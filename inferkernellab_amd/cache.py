@@ -7,6 +7,12 @@ ids (its block table), and token position ``p`` of a request lives at slot
 ``table[p // block_size] * block_size + p % block_size``. Validation rules
 and error messages follow the reference so callers see the same failures.
 
+A page may be held by several requests (no counterpart in the reference,
+whose pages have one owner): ``fork_request`` shares the whole pages of a
+prefix and copies the page that is filled in part, and ``compact`` moves the
+pages in use to the lowest ids. Shared pages are only ever read: what a
+request appends goes to pages that it alone holds.
+
 The torch scatter/gather methods (``write``, ``write_slots``, ``read``) are
 the reference's ``append_backend="torch"`` path and its gather; the HIP
 append lives in :mod:`inferkernellab_amd.ops`.
@@ -42,7 +48,8 @@ class BlockAllocator:
 
     Free ids are kept in a stack initialised high-to-low, so fresh allocations
     come out in ascending order. ``free`` validates the whole request before
-    mutating anything.
+    mutating anything. ``share`` gives blocks in use a further holder; a block
+    is free again once every holder has freed it.
     """
 
     def __init__(self, num_blocks: int):
@@ -52,6 +59,7 @@ class BlockAllocator:
         self._free_stack: list[int] = list(reversed(range(num_blocks)))
         self._in_use: set[int] = set()
         self._owner_of: dict[int, int] = {}
+        self._sharers: dict[int, list[int]] = {}  # holders besides the owner
 
     @property
     def num_free_blocks(self) -> int:
@@ -74,7 +82,7 @@ class BlockAllocator:
             self._owner_of.update((block, owner) for block in taken)
         return taken
 
-    def free(self, block_ids, owner: int | None = None) -> None:
+    def _checked(self, block_ids) -> tuple[int, ...]:
         ids = tuple(block_ids)
         if len(set(ids)) != len(ids):
             raise ValueError("block_ids must not contain duplicates")
@@ -83,12 +91,64 @@ class BlockAllocator:
                 raise ValueError(f"invalid block id: {block}")
             if block not in self._in_use:
                 raise ValueError(f"block {block} is not allocated")
-            if owner is not None and self._owner_of.get(block) != owner:
-                raise ValueError(f"block {block} is not owned by request {owner}")
+        return ids
+
+    def holders(self, block_id: int) -> tuple[int | None, ...]:
+        """Who holds a block, its owner first (None: allocated without one); empty for a free block."""
+        if block_id not in self._in_use:
+            return ()
+        return (self._owner_of.get(block_id), *self._sharers.get(block_id, ()))
+
+    def share(self, block_ids, owner: int) -> None:
+        """Make `owner` a further holder of blocks in use."""
+        ids = self._checked(block_ids)
+        if owner is None:
+            raise ValueError("a shared block needs a named holder")
         for block in ids:
+            if owner in self.holders(block):
+                raise ValueError(f"block {block} is already held by request {owner}")
+        for block in ids:
+            self._sharers.setdefault(block, []).append(owner)
+
+    def free(self, block_ids, owner: int | None = None) -> None:
+        ids = self._checked(block_ids)
+        for block in ids:
+            if owner is not None and owner not in self.holders(block):
+                raise ValueError(f"block {block} is not owned by request {owner}")
+            if owner is None and block in self._sharers:
+                raise ValueError(f"block {block} is shared: the holder that frees it must be named")
+        for block in ids:
+            sharers = self._sharers.get(block)
+            if sharers:  # held on by the others
+                if owner in sharers:
+                    sharers.remove(owner)
+                else:
+                    self._owner_of[block] = sharers.pop(0)
+                if not sharers:
+                    del self._sharers[block]
+                continue
             self._in_use.discard(block)
             self._owner_of.pop(block, None)
             self._free_stack.append(block)
+
+    def compaction(self) -> dict[int, int]:
+        """{old id: new id} of the moves that leave the blocks in use at 0 ..
+        used - 1, the fewest there are. No block goes where another comes from."""
+        used = len(self._in_use)
+        return dict(zip(sorted(b for b in self._in_use if b >= used),
+                        (b for b in range(used) if b not in self._in_use)))
+
+    def renumber(self, moves: dict[int, int]) -> None:
+        """Take over the moves of ``compaction``."""
+        if moves != self.compaction():
+            raise ValueError("the moves are not those of the blocks in use")
+        for table in (self._owner_of, self._sharers):
+            for old, new in moves.items():
+                if old in table:
+                    table[new] = table.pop(old)
+        used = len(self._in_use)
+        self._in_use = set(range(used))
+        self._free_stack = list(reversed(range(used, self._capacity)))
 
     def owner(self, block_id: int) -> int | None:
         return self._owner_of.get(block_id)
@@ -166,6 +226,65 @@ class PagedKVCache:
 
     def release_request(self, block_table, request_id: int | None = None) -> None:
         self.allocator.free(block_table, owner=request_id)
+
+    def copy_blocks(self, src, dst) -> None:
+        """Copy the pages ``src[i]`` to ``dst[i]``, all layers (lists of block
+        ids; no page twice in dst, none in both): one launch on a GPU cache."""
+        if self.device.type == "cuda":
+            from .ops import copy_blocks_hip  # the operators need no cache, a cache on the CPU no operators
+
+            copy_blocks_hip(self, src, dst)
+            return
+        src, dst = list(src), list(dst)
+        if len(src) != len(dst):
+            raise ValueError("src and dst must have one entry per copied block")
+        if any(not 0 <= b < self.layout.num_blocks for b in src + dst):
+            raise ValueError("copy blocks: invalid block id")
+        if len(set(dst)) != len(dst) or not set(dst).isdisjoint(src):
+            raise ValueError("copy blocks: a block is written twice, or both read and written")
+        for t in (self.k, self.v) + ((self.k_scale, self.v_scale) if self.fp8 else ()):
+            for a, b in zip(src, dst):
+                t[:, b].copy_(t[:, a])
+
+    def fork_request(self, block_table, num_tokens: int, request_id: int) -> list[int]:
+        """A table for `request_id` over the first `num_tokens` tokens of
+        `block_table`: its whole pages are shared, a page filled in part is
+        copied (all layers, on the current stream), so that either request
+        appends without the other seeing it. Raises before anything changes."""
+        bs = self.layout.block_size
+        if num_tokens <= 0 or num_tokens > len(block_table) * bs:
+            raise ValueError("num_tokens must be positive and covered by the block table")
+        if request_id is None:
+            raise ValueError("a fork needs a request id")
+        whole, rest = divmod(num_tokens, bs)
+        shared = list(block_table[:whole])
+        self.allocator.share(shared, request_id)
+        if not rest:
+            return shared
+        own: list[int] = []
+        try:
+            if self.allocator.holders(block_table[whole]) == ():
+                raise ValueError(f"block {block_table[whole]} is not allocated")
+            own = self.allocator.allocate(1, owner=request_id)
+            self.copy_blocks([block_table[whole]], own)
+        except BaseException:
+            self.allocator.free(shared + own, owner=request_id)
+            raise
+        return shared + own
+
+    def compact(self, block_tables=()) -> dict[int, int]:
+        """Move the pages in use to the lowest block ids (all layers, on the
+        current stream) and renumber them in the tables given (lists, changed
+        in place; a list given twice is changed once). Returns {old id: new id}
+        of the moved pages, for every other place that names them, such as
+        device copies of the tables."""
+        moves = self.allocator.compaction()
+        if moves:
+            self.copy_blocks(list(moves), list(moves.values()))
+            self.allocator.renumber(moves)
+            for table in {id(t): t for t in block_tables}.values():
+                table[:] = [moves.get(b, b) for b in table]
+        return moves
 
     def slot_mapping(self, block_table, start: int, length: int, *, device=None) -> torch.Tensor:
         """Physical slots of logical positions ``[start, start + length)``

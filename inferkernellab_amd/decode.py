@@ -76,6 +76,12 @@ class DecodeMetadata:
                     torch.tensor(r.block_table[done:n], dtype=torch.int32), non_blocking=False)
                 self._copied[r.request_id] = n
 
+    def refresh(self, requests: Sequence[InferenceRequest]) -> None:
+        """Copy whole tables again, after their pages were renumbered."""
+        for r in requests:
+            self._copied[r.request_id] = 0
+        self.sync_tables(requests)
+
     def for_batch(self, requests: Sequence[InferenceRequest], context_lengths: Sequence[int]):
         """(tables, lens) rows of `requests` with lens set to `context_lengths`."""
         if len(requests) != len(context_lengths):

@@ -10,6 +10,8 @@ them. What callers observe, and the reference's tests pin
 * a prefill step grows every scheduled table to its cached tokens, then
   calls ``prefill_batch_fn(requests, starts, ends)`` once with the requests
   whose range is non-empty (or ``prefill_fn`` per request);
+* ``fork`` continues a running request a second time on shared pages, and
+  ``compact`` moves the pages in use together;
 * a decode step first reserves room for the token each request writes, then
   calls ``decode_fn(requests)`` — before the scheduler counts that token —
   and finally returns the blocks of finished requests to the allocator.
@@ -90,6 +92,32 @@ class InferenceRuntime:
         self._by_id[request_id] = request
         self.scheduler.add(request)
         return request
+
+    def fork(self, request_id: int, new_request_id: int, max_new_tokens: int | None = None) -> InferenceRequest:
+        """Continue a running request a second time: the new request has its
+        tokens so far, the whole pages of its cache shared and a page filled in
+        part copied (no counterpart in the reference)."""
+        if new_request_id in self._by_id:
+            raise ValueError(f"duplicate request_id: {new_request_id}")
+        parent = self._by_id.get(request_id)
+        if parent is None or parent.status != "running":
+            raise ValueError(f"request {request_id} is not running")
+        if max_new_tokens is None:
+            max_new_tokens = parent.max_new_tokens
+        child = InferenceRequest(new_request_id, parent.prompt_tokens, max_new_tokens,
+                                 generated_tokens=parent.generated_tokens, cached_tokens=parent.cached_tokens)
+        if child.finished:
+            raise ValueError("max_new_tokens leaves the fork nothing to generate")
+        child.block_table = self.cache.fork_request(parent.block_table, parent.prompt_tokens + parent.generated_tokens,
+                                                    new_request_id)
+        self._by_id[new_request_id] = child
+        self.scheduler.add_running(child)
+        return child
+
+    def compact(self) -> dict[int, int]:
+        """Move the cache's pages in use to the lowest ids and renumber every
+        request's table; {old id: new id} for device copies of the tables."""
+        return self.cache.compact([r.block_table for r in self._by_id.values()])
 
     def _reserve(self, request: InferenceRequest, tokens: int) -> None:
         """Tops the request's table up to the blocks `tokens` positions need."""

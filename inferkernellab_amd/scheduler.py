@@ -114,6 +114,13 @@ class TokenBudgetScheduler:
             raise ValueError("only waiting requests can be added")
         self.waiting.append(request)
 
+    def add_running(self, request: InferenceRequest) -> None:
+        """A request whose prompt is in the cache already, as a fork's is."""
+        if request.prompt_remaining or request.finished:
+            raise ValueError("only prefilled, unfinished requests can be added to the running set")
+        request.status = "running"
+        self.running.append(request)
+
     def schedule(self) -> ScheduleBatch:
         plan = plan_prefill(self.waiting, self.max_num_seqs, self.max_num_batched_tokens)
         prefilled = self._commit(plan)
