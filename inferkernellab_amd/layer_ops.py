@@ -64,7 +64,7 @@ def kernels_apply(x: torch.Tensor) -> bool:
     )
 
 
-def _plain_weight(w, x: torch.Tensor) -> bool:
+def plain_weight(w, x: torch.Tensor) -> bool:
     return (
         type(w) in (nn.Parameter, torch.Tensor)
         and w.dtype == x.dtype
@@ -94,7 +94,7 @@ def _stream(device: torch.device) -> int:
 def norm_fits(weight, x: torch.Tensor) -> bool:
     row = x.shape[-1] * x.element_size()
     return (x.numel() > 0 and row % 16 == 0 and row <= 16384 and weight.ndim == 1 and weight.shape[0] == x.shape[-1]
-            and _plain_weight(weight, x) and _flat_rows(x) is not None)
+            and plain_weight(weight, x) and _flat_rows(x) is not None)
 
 
 def add_rms_norm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tensor, eps: float, *,
@@ -151,7 +151,7 @@ def linear_weight_fits(linear, x: torch.Tensor) -> bool:
         return False
     w = linear.weight
     return (x.dtype in (torch.float16, torch.bfloat16) and w.shape[1] % 64 == 0 and w.shape[0] % 16 == 0
-            and 0 < w.numel() <= MAX_WEIGHT and _plain_weight(w, x))
+            and 0 < w.numel() <= MAX_WEIGHT and plain_weight(w, x))
 
 
 def linear_fits(linear, x: torch.Tensor) -> bool:

@@ -17,6 +17,12 @@ q_proj`` ..., ``model.norm``, ``lm_head``, ``config``), so it accepts either
 that class or :class:`LlamaForCausalLM` below, a dependency-free module with
 the same layout and arithmetic (RMSNorm in fp32, RoPE tables in fp32 cast
 to the activation dtype) for seeded random-weight models.
+
+Beside what the reference's runner does: attention with norms of the query
+and key heads (``self_attn.q_norm`` / ``k_norm``; one launch with the RoPE and
+the append), several samples of each prompt on shared cache pages
+(``num_samples``), and drawing tokens by the sampling kernel
+(``sampler="hip"``: top-k and min-p too, inside the captured step).
 """
 
 from __future__ import annotations
@@ -36,6 +42,7 @@ from . import layer_ops, ops
 from .cache import PagedKVCache
 from .decode import ATTENTION_BACKENDS, APPEND_BACKENDS, DecodeMetadata, percentile
 from .runtime import InferenceRuntime
+from .sampling import PreparedSampler, sample_tokens_hip
 from .scheduler import InferenceRequest, TokenBudgetScheduler
 
 
@@ -52,6 +59,7 @@ class LlamaConfig:
     rope_theta: float = 10000.0
     rms_norm_eps: float = 1e-6
     max_position_embeddings: int = 4096
+    qk_norm: bool = False  # RMSNorm of each query and key head before RoPE
 
     def __post_init__(self) -> None:
         if self.head_dim is None:
@@ -96,6 +104,9 @@ class _Attention(nn.Module):
         self.k_proj = nn.Linear(c.hidden_size, c.num_key_value_heads * c.head_dim, bias=False)
         self.v_proj = nn.Linear(c.hidden_size, c.num_key_value_heads * c.head_dim, bias=False)
         self.o_proj = nn.Linear(c.num_attention_heads * c.head_dim, c.hidden_size, bias=False)
+        if c.qk_norm:
+            self.q_norm = RMSNorm(c.head_dim, c.rms_norm_eps)
+            self.k_norm = RMSNorm(c.head_dim, c.rms_norm_eps)
 
 
 class _MLP(nn.Module):
@@ -193,6 +204,10 @@ class _StepBuffers:
     used: torch.Tensor | None = None
     graph: torch.cuda.CUDAGraph | None = None
     staged: torch.Tensor | None = None  # pinned host copy of the step's fp32 logits
+    # drawn tokens: the requests' uniform number for the step, and what draws
+    uniform: torch.Tensor | None = None
+    step: torch.Tensor | None = None
+    draw: PreparedSampler | None = None
 
 
 @dataclass(frozen=True)
@@ -252,7 +267,14 @@ class LlamaPagedDecodeRunner:
                  max_num_batched_tokens: int = 2048, prefill_mode: str = "batched",
                  temperature: float = 0.0, top_p: float = 1.0, seed: int = 2026,
                  eos_token_ids: Sequence[int] | None = None, use_graph: bool = True,
-                 prefill_attention: str = "hip", kv_cache_dtype: torch.dtype | None = None) -> None:
+                 prefill_attention: str = "hip", kv_cache_dtype: torch.dtype | None = None,
+                 num_samples: int = 1, sampler: str = "torch", top_k: int = 0, min_p: float = 0.0) -> None:
+        """``num_samples``: continuations of each prompt, which is prefilled
+        once; request ``i * num_samples + s`` is sample ``s`` of prompt ``i``
+        and draws from the seed's generator of that id. ``sampler``: ``"torch"``
+        draws as the reference's runner does, one request at a time; ``"hip"``
+        the whole batch by :func:`sample_tokens_hip` with uniform numbers from
+        the same generators, and takes ``top_k`` and ``min_p`` (0: off)."""
         if not prompts:
             raise ValueError("at least one prompt is required")
         if max_new_tokens <= 0:
@@ -269,6 +291,14 @@ class LlamaPagedDecodeRunner:
             raise ValueError("prefill_attention must be hip or torch")
         if not (math.isfinite(temperature) and temperature >= 0 and math.isfinite(top_p) and 0 < top_p <= 1):
             raise ValueError("temperature must be non-negative and top_p must be in (0, 1]")
+        if num_samples <= 0:
+            raise ValueError("num_samples must be positive")
+        if sampler not in ("torch", "hip"):
+            raise ValueError("sampler must be torch or hip")
+        if top_k < 0 or not 0 <= min_p <= 1:
+            raise ValueError("top_k must be non-negative and min_p must be in [0, 1]")
+        if sampler == "torch" and (top_k or min_p):
+            raise ValueError("top_k and min_p need the hip sampler")
         param = next(model.parameters())
         self.model, self.device, self.dtype = model, param.device, param.dtype
         if self.device.type != "cuda":
@@ -286,6 +316,7 @@ class LlamaPagedDecodeRunner:
         self.backend, self.append_backend, self.prefill_mode = backend, append_backend, prefill_mode
         self.prefill_attention = prefill_attention
         self.max_new_tokens, self.temperature, self.top_p = max_new_tokens, temperature, top_p
+        self.num_samples, self.sampler, self.top_k, self.min_p = num_samples, sampler, top_k, min_p
         self._attend = ATTENTION_BACKENDS[backend]
         self.num_layers = int(cfg.num_hidden_layers)
         self.num_heads = int(cfg.num_attention_heads)
@@ -295,7 +326,10 @@ class LlamaPagedDecodeRunner:
             raise ValueError("num_attention_heads must be divisible by num_key_value_heads")
         self.prompt_lengths = tuple(len(p) for p in self.prompts)
         width = max(-(-(n + max_new_tokens) // block_size) for n in self.prompt_lengths)
-        total_blocks = sum(-(-(n + max_new_tokens) // block_size) for n in self.prompt_lengths)
+        # a prompt's whole pages are held by all its samples
+        total_blocks = sum(n // block_size
+                           + num_samples * (-(-(n + max_new_tokens) // block_size) - n // block_size)
+                           for n in self.prompt_lengths)
         # kv_cache_dtype=torch.float8_e4m3fn: the FP8 KV format (E4M3 codes,
         # one power-of-two scale per token and head) under fp16/bf16 models
         fp8 = kv_cache_dtype == torch.float8_e4m3fn
@@ -309,30 +343,54 @@ class LlamaPagedDecodeRunner:
         batched = prefill_mode == "batched"
         self.runtime = InferenceRuntime(
             self.cache,
-            TokenBudgetScheduler(max_num_seqs=len(self.prompts), max_num_batched_tokens=max_num_batched_tokens),
+            TokenBudgetScheduler(max_num_seqs=len(self.prompts) * num_samples,
+                                 max_num_batched_tokens=max_num_batched_tokens),
             prefill_fn=None if batched else self._prefill,
             prefill_batch_fn=self._prefill_batch if batched else None,
             decode_fn=self._decode,
         )
-        self.requests = [self.runtime.submit(i, len(p), max_new_tokens) for i, p in enumerate(self.prompts)]
-        self.metadata = DecodeMetadata(len(self.requests), width, self.device)
+        self.requests = [self.runtime.submit(i * num_samples, len(p), max_new_tokens)
+                         for i, p in enumerate(self.prompts)]
+        request_ids = range(len(self.prompts) * num_samples)
+        self.metadata = DecodeMetadata(len(request_ids), width, self.device)
         self._prompt_logits: dict[int, torch.Tensor] = {}
         self._next_logits: dict[int, torch.Tensor] = {}
         self._decode_logits: list[torch.Tensor] = []
         self._staged: torch.Tensor | None = None
         self._padding = 0
-        self._generated = {r.request_id: [] for r in self.requests}
-        self._token_logprobs = {r.request_id: [] for r in self.requests}
-        self._sampling_logprobs = {r.request_id: [] for r in self.requests}
-        self._finish = {r.request_id: "length" for r in self.requests}
-        self._generators = {r.request_id: torch.Generator(device=self.device).manual_seed(seed + r.request_id)
-                            for r in self.requests}
+        self._generated = {i: [] for i in request_ids}
+        self._token_logprobs = {i: [] for i in request_ids}
+        self._sampling_logprobs = {i: [] for i in request_ids}
+        self._finish = {i: "length" for i in request_ids}
+        self._generators = {i: torch.Generator(device=self.device).manual_seed(seed + i) for i in request_ids}
+        self._uniform = None  # [requests, max_new_tokens], the hip sampler's
+        if sampler == "hip":
+            self._uniform = torch.stack([torch.rand(max_new_tokens, generator=g, device=self.device)
+                                         for g in self._generators.values()])
+        # tokens drawn by the kernel, with their log probabilities (as the torch
+        # sampler reports them)
+        self._draws = sampler == "hip" and (temperature > 0 or bool(self.eos_token_ids))
         self.use_graph = use_graph
         self._graphs: dict[tuple[int, ...], _StepBuffers] = {}
         self._max_ctx = max(self.prompt_lengths) + max_new_tokens
         self._has_run = False
 
     # ------------------------------------------------------------ helpers
+    def _prompt(self, request: InferenceRequest) -> tuple[int, ...]:
+        return self.prompts[request.request_id // self.num_samples]
+
+    def _fork_samples(self, requests) -> None:
+        """The other samples of the prompts that are in the cache now."""
+        for r in requests:
+            if r.prompt_remaining or r.request_id % self.num_samples:
+                continue
+            for i in range(r.request_id + 1, r.request_id + self.num_samples):
+                self.requests.append(self.runtime.fork(r.request_id, i))
+                self._prompt_logits[i] = self._prompt_logits[r.request_id]
+                self._next_logits[i] = self._next_logits[r.request_id]
+        # a step's rows stand in the order of the requests' ids
+        self.runtime.scheduler.running.sort(key=lambda r: r.request_id)
+
     def _rope(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
         return x * cos + rotate_half(x) * sin
 
@@ -358,6 +416,40 @@ class LlamaPagedDecodeRunner:
         if delta is not None:
             hidden = hidden + delta
         return hidden, norm(hidden)
+
+    def _head_norms(self, att, q: torch.Tensor, k: torch.Tensor):
+        """The attention's norms of q and k heads and whether the fused append
+        restates them: (q_norm, k_norm, restated), or None without norms."""
+        q_norm, k_norm = getattr(att, "q_norm", None), getattr(att, "k_norm", None)
+        if q_norm is None and k_norm is None:
+            return None
+        restated = (
+            self.append_backend != "torch" and layer_ops.kernels_apply(q) and layer_ops.kernels_apply(k)
+            and all(layer_ops.plain_module(n, RMSNorm) and n.weight.shape == (self.head_dim,)
+                    and layer_ops.plain_weight(n.weight, q) for n in (q_norm, k_norm))
+            and q_norm.variance_epsilon == k_norm.variance_epsilon
+            and self.head_dim * q.element_size() % 32 == 0 and self.head_dim * q.element_size() <= 2048
+        )
+        return q_norm, k_norm, restated
+
+    def _rope_append(self, layer: int, att, q, k, v, cos, sin, slots) -> torch.Tensor:
+        """RoPE of q and k [T, heads, D] and the append of k and v at slots [T],
+        after the heads' norms where the attention has them: one launch where
+        the norms are plain. Returns the rotated q (q itself, in place)."""
+        norms = self._head_norms(att, q, k)
+        if norms is not None and norms[2]:
+            return ops.qk_norm_rope_append_kv_hip(q, k, v, norms[0].weight, norms[1].weight, cos, sin, self.cache,
+                                                  slots, layer, eps=norms[0].variance_epsilon)
+        if norms is not None:
+            q, k = (x if norm is None else norm(x) for norm, x in zip(norms, (q, k)))
+        return ops.rope_append_kv_hip(q, k, v, cos, sin, self.cache, slots, layer=layer)
+
+    def _rope_qk(self, att, q, k, cos, sin):
+        """The same without the append, by the modules and torch."""
+        norms = self._head_norms(att, q, k)
+        if norms is not None:
+            q, k = (x if norm is None else norm(x) for norm, x in zip(norms, (q, k)))
+        return self._rope(q, cos, sin), self._rope(k, cos, sin)
 
     def _mlp(self, mlp, x: torch.Tensor) -> torch.Tensor:
         gate, up = mlp.gate_proj(x), mlp.up_proj(x)
@@ -418,9 +510,9 @@ class LlamaPagedDecodeRunner:
             k = k.view(n, self.num_kv_heads, self.head_dim)
             v = v.view(n, self.num_kv_heads, self.head_dim)
             if fused:  # RoPE of q and k + append of rope(k), v: one launch (q rotated in place)
-                ops.rope_append_kv_hip(q, k, v, cos2, sin2, self.cache, slots, layer=li)
+                q = self._rope_append(li, att, q, k, v, cos2, sin2, slots)
             else:
-                q, k = self._rope(q, cos, sin), self._rope(k, cos, sin)
+                q, k = self._rope_qk(att, q, k, cos, sin)
                 self._append(li, slots, k, v)
             o = self._attend(q.contiguous(), self.cache, tables, lens, layer=li, validate_inputs=validate and li == 0,
                              max_context_len=self._max_ctx)
@@ -508,12 +600,12 @@ class LlamaPagedDecodeRunner:
             k = att.k_proj(x).view(b, t, self.num_kv_heads, self.head_dim)
             v = att.v_proj(x).view(b, t, self.num_kv_heads, self.head_dim)
             if fused:  # q rotated in place; padding rows of k / v are skipped (slot -1)
-                ops.rope_append_kv_hip(q.view(b * t, self.num_heads, self.head_dim),
-                                       k.reshape(b * t, self.num_kv_heads, self.head_dim),
-                                       v.reshape(b * t, self.num_kv_heads, self.head_dim),
-                                       cos2, sin2, self.cache, slots, layer=li)
+                q = self._rope_append(li, att, q.view(b * t, self.num_heads, self.head_dim),
+                                      k.reshape(b * t, self.num_kv_heads, self.head_dim),
+                                      v.reshape(b * t, self.num_kv_heads, self.head_dim),
+                                      cos2, sin2, slots).view(b, t, self.num_heads, self.head_dim)
             else:
-                q, k = self._rope(q, cos, sin), self._rope(k, cos, sin)
+                q, k = self._rope_qk(att, q, k, cos, sin)
                 self._append(li, slots, torch.cat([k[i, :n] for i, n in enumerate(spans)]),
                              torch.cat([v[i, :n] for i, n in enumerate(spans)]))
             if prefill is not None:
@@ -550,11 +642,11 @@ class LlamaPagedDecodeRunner:
         width = max(spans)
         ids = torch.zeros((len(requests), width), dtype=torch.long)
         for row, (r, s, e) in enumerate(zip(requests, starts, ends)):
-            ids[row, : e - s] = torch.tensor(self.prompts[r.request_id][s:e])
+            ids[row, : e - s] = torch.tensor(self._prompt(r)[s:e])
         self._padding += len(requests) * width - sum(spans)
         logits = self._forward_prefill(ids.to(self.device), requests, starts, ends)
         for row, (r, e) in enumerate(zip(requests, ends)):
-            if e == len(self.prompts[r.request_id]):
+            if e == len(self._prompt(r)):
                 self._prompt_logits[r.request_id] = logits[row].detach()
                 self._next_logits[r.request_id] = logits[row].detach()
 
@@ -578,10 +670,11 @@ class LlamaPagedDecodeRunner:
 
     # ------------------------------------------------- graph-captured steps
     def _decode_graphed(self, requests: tuple[InferenceRequest, ...]) -> None:
-        """Greedy decode step as one HIP graph replay per batch composition.
+        """Decode step as one HIP graph replay per batch composition, greedy or
+        with tokens drawn by the sampling kernel.
 
         The graph holds the whole step on static device buffers: argmax of
-        the previous logits, lens = pos + 1 and slots from the table buffer
+        the previous logits or the draw from them, lens = pos + 1 and slots from the table buffer
         on the device, the layers (fused RoPE + append, paged attention),
         lm_head, and pos += 1. The host only publishes new table entries and
         reads the tokens back. A batch's first step runs eagerly (it is that
@@ -601,6 +694,11 @@ class LlamaPagedDecodeRunner:
                 slots=torch.zeros(n, dtype=torch.int32, device=self.device),
             )
             st.used = torch.empty_like(st.logits)
+            if self._draws:
+                st.uniform = torch.empty(n, dtype=torch.float32, device=self.device)
+                st.step = torch.tensor([r.generated_tokens for r in requests], dtype=torch.long, device=self.device)
+                st.draw = PreparedSampler(st.used, st.uniform, temperature=self.temperature, top_k=self.top_k,
+                                          top_p=self.top_p, min_p=self.min_p, logprobs=True)
             st.staged = torch.empty(st.logits.shape, dtype=torch.float32, pin_memory=True)
             side = torch.cuda.Stream(self.device)
             side.wait_stream(torch.cuda.current_stream(self.device))
@@ -617,9 +715,18 @@ class LlamaPagedDecodeRunner:
         st.staged.copy_(st.used, non_blocking=True)
         self._staged = st.staged
         toks = st.tok.tolist()
+        if st.draw is not None:
+            self._collect_logprobs(requests, st.draw.policy_logprobs, st.draw.sampling_logprobs)
         for i, r in enumerate(requests):
             self._generated[r.request_id].append(int(toks[i]))
             self._next_logits[r.request_id] = st.logits[i]
+
+    def _collect_logprobs(self, requests, policy: torch.Tensor, sampling: torch.Tensor) -> None:
+        for r, lp, ls in zip(requests, policy.tolist(), sampling.tolist()):
+            if lp == -math.inf:
+                raise RuntimeError(f"request {r.request_id} has no logit to draw a token from")
+            self._token_logprobs[r.request_id].append(lp)
+            self._sampling_logprobs[r.request_id].append(ls)
 
     def _collect_logits(self) -> None:
         """Takes the staged logits of the last captured step (whose stream
@@ -660,7 +767,12 @@ class LlamaPagedDecodeRunner:
     def _graph_body(self, st: "_StepBuffers") -> None:
         bs = self.cache.layout.block_size
         st.used.copy_(st.logits)
-        st.tok.copy_(st.used.argmax(dim=-1))
+        if st.draw is None:
+            st.tok.copy_(st.used.argmax(dim=-1))
+        else:  # the clamps keep a stray replay past the run inside its buffers
+            st.uniform.copy_(self._uniform[st.ids, st.step.clamp(max=self.max_new_tokens - 1)])
+            st.tok.copy_(st.draw()[0].clamp(min=0))
+            st.step.add_(1)
         st.lens.copy_(st.pos + 1)
         tables = self.metadata.tables.index_select(0, st.ids)
         # The runtime reserves every decoded position inside the table's
@@ -673,13 +785,20 @@ class LlamaPagedDecodeRunner:
         st.pos.add_(1)
 
     def _decode(self, requests: tuple[InferenceRequest, ...]) -> None:
-        if self.use_graph and self.temperature == 0 and not self.eos_token_ids:
+        if self.use_graph and (self.temperature == 0 or self._draws) and not self.eos_token_ids:
             self._decode_graphed(requests)
             return
         used = torch.stack([self._next_logits[r.request_id] for r in requests])
         sampled = None
         if self.temperature == 0 and not self.eos_token_ids:
             next_tokens = used.argmax(dim=-1)
+        elif self._draws:
+            ids = torch.tensor([r.request_id for r in requests], device=self.device)
+            step = torch.tensor([r.generated_tokens for r in requests], device=self.device)
+            next_tokens, policy, sampling = sample_tokens_hip(
+                used.contiguous(), self._uniform[ids, step], temperature=self.temperature, top_k=self.top_k,
+                top_p=self.top_p, min_p=self.min_p, logprobs=True)
+            next_tokens = next_tokens.clamp(min=0)
         else:
             sampled = [self._sample(used[i], self._generators[r.request_id]) for i, r in enumerate(requests)]
             next_tokens = torch.stack([s[0] for s in sampled])
@@ -688,6 +807,8 @@ class LlamaPagedDecodeRunner:
         self._collect_logits()
         self._decode_logits.append(used.float().cpu())
         toks = next_tokens.tolist()
+        if self._draws:
+            self._collect_logprobs(requests, policy, sampling)
         for i, r in enumerate(requests):
             self._generated[r.request_id].append(int(toks[i]))
             if sampled is not None:
@@ -715,6 +836,8 @@ class LlamaPagedDecodeRunner:
                 while self.runtime.scheduler.waiting or self.runtime.scheduler.running:
                     t0 = time.perf_counter()
                     batch = self.runtime.step()
+                    if batch.phase == "prefill" and self.num_samples > 1:
+                        self._fork_samples(batch.requests)
                     torch.cuda.synchronize(self.device)
                     if not (self.runtime.scheduler.waiting or self.runtime.scheduler.running):
                         self._collect_logits()  # no step follows to take them
@@ -731,6 +854,7 @@ class LlamaPagedDecodeRunner:
             # garbage collector, the graphs would die at any later moment,
             # another capture included.
             self._graphs.clear()
+        self.requests.sort(key=lambda r: r.request_id)
         if len(self._prompt_logits) != len(self.requests):
             raise RuntimeError("prefill did not produce one final logits tensor per request")
         generated = tuple(tuple(self._generated[r.request_id]) for r in self.requests)
