@@ -27,8 +27,10 @@ template <typename Tag>
 __device__ inline void draw(const SampleParams &p, int64_t b, const RowReader<Tag> &row, const RowSettings &set,
                             const Weigher &weigh, const Binner &bin_of, uint32_t n, RowShared &sh) {
   if (n > LIST) sample_by_radix<Tag>(p, b, row, set, weigh, sh);
-  else if (n > 64) sample_from_list(p, b, set, weigh, bin_of, (int)n, sh);
-  else if (threadIdx.x < 64) sample_from_few(p, b, set, weigh, bin_of, (int)n, sh);
+  else if (n > 256) sample_from_list(p, b, set, weigh, bin_of, (int)n, sh);
+  else if (threadIdx.x >= 64) return;
+  else if (n > 64) sample_from_few<4>(p, b, set, weigh, bin_of, (int)n, sh);
+  else sample_from_few<1>(p, b, set, weigh, bin_of, (int)n, sh);
 }
 
 constexpr int MAX_PARTS = 64;
@@ -36,9 +38,9 @@ constexpr int MAX_PARTS = 64;
 // The tokens of the cuts' bins among the vectors [from, to) of the row.
 template <typename Tag>
 __device__ inline void list_tokens(const RowReader<Tag> &row, int from, int to, const Weigher &weigh,
-                                   const Candidates &cand, const Binner &bin_of, RowShared &sh) {
+                                   const Candidates &cand, const Binner &bin_of, const v4u32 &begin, RowShared &sh) {
   const Cuts cuts = sh.cuts;
-  row.each(from, to, [&](int first, const float(&x)[RowReader<Tag>::VEC]) {
+  row.each(from, to, begin, [&](int first, const float(&x)[RowReader<Tag>::VEC]) {
     uint32_t hits = 0;
 #pragma unroll
     for (int j = 0; j < RowReader<Tag>::VEC; ++j) hits |= (uint32_t)cuts.has(bin_of(x[j])) << j;
@@ -100,7 +102,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_row_kernel(const Sample
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    list_tokens(row, 0, row.vectors, weigh, cand, bin_of, sh);
+    list_tokens(row, 0, row.vectors, weigh, cand, bin_of, row.begin(0, row.vectors), sh);
     __syncthreads();
     n = sh.listed;
   }
@@ -192,6 +194,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_histogram_kernel(const 
   __shared__ RowShared sh;
   const Part<Tag> at(p, parts);
   SplitRow &r = rows[at.b];
+  const v4u32 begin = at.row.begin(at.from, at.to);  // on its way meanwhile
   fill_roots(sh.roots);
   clear_histogram(sh);
   const RowSettings set = row_settings(p, at.b);
@@ -203,7 +206,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_histogram_kernel(const 
   const Binner bin_of(set, weigh, cand, top, least);
   uint64_t others = 0;
   __syncthreads();
-  at.row.each(at.from, at.to, [&](int first, const float(&x)[RowReader<Tag>::VEC]) {
+  at.row.each(at.from, at.to, begin, [&](int first, const float(&x)[RowReader<Tag>::VEC]) {
     add_tokens<false>(first, x, set, weigh, cand, bin_of, others, sh);
   });
   if (set.min_p > 0.f) {
@@ -222,6 +225,14 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_pick_kernel(const Sa
   __shared__ RowShared sh;
   const Part<Tag> at(p, parts);
   SplitRow &r = rows[at.b];
+  const v4u32 begin = at.row.begin(at.from, at.to);  // these are on their way meanwhile
+  uint64_t mass[BINS / SAMPLE_THREADS];
+  uint32_t count[BINS / SAMPLE_THREADS];
+#pragma unroll
+  for (int i = 0; i < BINS / SAMPLE_THREADS; ++i) {
+    mass[i] = r.mass[threadIdx.x + i * SAMPLE_THREADS];
+    count[i] = r.count[threadIdx.x + i * SAMPLE_THREADS];
+  }
   const RowSettings set = row_settings(p, at.b);
   float top, least;
   row_extremes(r, parts, top, least);
@@ -232,9 +243,10 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_pick_kernel(const Sa
     return;
   }
   fill_roots(sh.roots);
-  for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) {
-    sh.mass[i] = r.mass[i];
-    sh.count[i] = r.count[i];
+#pragma unroll
+  for (int i = 0; i < BINS / SAMPLE_THREADS; ++i) {
+    sh.mass[threadIdx.x + i * SAMPLE_THREADS] = mass[i];
+    sh.count[threadIdx.x + i * SAMPLE_THREADS] = count[i];
   }
   if (threadIdx.x == 0) {
     sh.listed = 0;
@@ -245,7 +257,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_pick_kernel(const Sa
   const Binner bin_of(set, weigh, cand, top, least);
   __syncthreads();
   find_cuts(set, cand, sh);
-  list_tokens(at.row, at.from, at.to, weigh, cand, bin_of, sh);
+  list_tokens(at.row, at.from, at.to, weigh, cand, bin_of, begin, sh);
   __syncthreads();
   const uint32_t mine = sh.listed;
   if (threadIdx.x == 0) sh.found[1] = mine ? atomicAdd(&r.listed, mine) : 0;

@@ -117,9 +117,17 @@ struct RowReader {
   // done to its elements can overlap.
   template <typename F>
   __device__ inline void each(int from, int to, F f) const {
+    each(from, to, begin(from, to), f);
+  }
+  // the same, with the thread's first vector loaded some time before by begin()
+  __device__ inline v4u32 begin(int from, int to) const {
+    const int v = from + threadIdx.x;
+    return v < to ? load(v) : v4u32{0, 0, 0, 0};
+  }
+  template <typename F>
+  __device__ inline void each(int from, int to, v4u32 w, F f) const {
     int v = from + threadIdx.x;
     if (v >= to) return;
-    v4u32 w = load(v);
     while (true) {
       const int ahead = v + SAMPLE_THREADS;
       v4u32 next = w;
@@ -619,6 +627,11 @@ __device__ inline double across(double v) {
   }
 }
 
+__device__ inline double across_lanes(double v, int d) {  // d known when unrolled
+  return d == 1 ? across<1>(v) : d == 2 ? across<2>(v) : d == 4 ? across<4>(v) : d == 8 ? across<8>(v)
+         : d == 16 ? across<16>(v) : across<32>(v);
+}
+
 // One step of the sorting network between lanes D apart: the lower lane of a
 // pair keeps the larger word where its run falls.
 template <int D>
@@ -628,6 +641,36 @@ __device__ inline void step_across(double (&w)[2], bool falls) {
   for (int e = 0; e < 2; ++e) {
     const double other = across<D>(w[e]);
     w[e] = larger ? fmax(w[e], other) : fmin(w[e], other);
+  }
+}
+
+// The E words of each lane of a wave in falling order, word e of lane l at place
+// l E + e.
+template <int E>
+__device__ inline void sort_wave(double (&w)[E], int lane) {
+  const int at = lane * E;
+#pragma unroll
+  for (int run = 2; run <= 64 * E; run <<= 1) {
+#pragma unroll
+    for (int d = run >> 1; d; d >>= 1) {
+      if (d >= E) {
+        const bool larger = ((at & run) == 0) == ((at & d) == 0);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const double other = across_lanes(w[e], d / E);
+          w[e] = larger ? fmax(w[e], other) : fmin(w[e], other);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if ((e & d) == 0) {
+            const bool falls = ((at + e) & run) == 0;
+            const double hi = fmax(w[e], w[e | d]), lo = fmin(w[e], w[e | d]);
+            w[e] = falls ? hi : lo;
+            w[e | d] = falls ? lo : hi;
+          }
+      }
+    }
   }
 }
 
@@ -685,43 +728,100 @@ __device__ inline void sort_list(int n, RowShared &sh) {
   __syncthreads();
 }
 
-// The draw from up to 64 tokens, by the first wave: what sample_from_list does,
-// a token a lane and without a barrier (n = 3: 4.7 -> 2.6 us).
+// The draw from up to 64 E tokens, by the first wave: what sample_from_list does,
+// E tokens a lane and without a barrier (3 tokens 4.7 -> 1.3 us). Up to 64 words
+// take their place by counting the larger ones, more by a bitonic network over
+// the registers of the wave.
+template <int E>
 __device__ inline void sample_from_few(const SampleParams &p, int64_t b, const RowSettings &set, const Weigher &weigh,
                                        const Binner &bin_of, int n, RowShared &sh) {
-  const int lane = threadIdx.x;
-  const bool on = lane < n;
-  // each word to the place that the number of larger ones gives
-  double word = sh.list[on ? lane : 0];
-  int rank = 0;
-  for (int j = 0; j < n; ++j)
-    rank += __longlong_as_double((int64_t)lane64((uint64_t)__double_as_longlong(word), j)) > word;
-  const int to = 4 * (on ? rank : lane);
-  word = __hiloint2double(__builtin_amdgcn_ds_permute(to, __double2hiint(word)),
-                          __builtin_amdgcn_ds_permute(to, __double2loint(word)));
-  const float x = word_logit(word);
-  const uint64_t w = on ? weigh(x) : 0;
-  const uint64_t ahead = wave_scan(w) - w;
-  const int bin = bin_of(x);
-  const int left = __shfl_up(bin, 1, 64);  // with every lane active
-  const bool starts = lane == 0 || left != bin;
-  const int head = 63 - __clzll(__ballot(starts) & (~0ull >> (63 - lane)));  // the first of the bin
-  const uint64_t at_head = ((uint64_t)(uint32_t)__shfl((int)(ahead >> 32), head, 64) << 32) |
-                           (uint32_t)__shfl((int)(uint32_t)ahead, head, 64);
-  const uint64_t before = sh.mass[bin] + ahead - at_head;  // of the whole row
-  uint64_t kept = sh.total;
-  if (set.top_k > 0 && (uint32_t)set.top_k < sh.weighted) {
-    const uint64_t kth = __ballot(on && sh.count[bin] + (uint32_t)(lane - head) == (uint32_t)set.top_k - 1);
-    kept = lane64(before + w, __ffsll((unsigned long long)kth) - 1);
+  const int lane = threadIdx.x, at = lane * E;  // this lane's tokens: at .. at + E - 1 of the order
+  double word[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) word[e] = at + e < n ? sh.list[at + e] : 0.0;
+  if constexpr (E == 1) {
+    int rank = 0;
+    for (int j = 0; j < n; ++j)
+      rank += __longlong_as_double((int64_t)lane64((uint64_t)__double_as_longlong(word[0]), j)) > word[0];
+    const int to = 4 * (lane < n ? rank : lane);
+    word[0] = __hiloint2double(__builtin_amdgcn_ds_permute(to, __double2hiint(word[0])),
+                               __builtin_amdgcn_ds_permute(to, __double2loint(word[0])));
+  } else {
+    sort_wave<E>(word, lane);
   }
-  // the masses before the tokens rise: a ballot counts those up to a bound
+  uint64_t w[E], before[E], sum = 0;
+  int bin[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float x = word_logit(word[e]);
+    w[e] = at + e < n ? weigh(x) : 0;
+    bin[e] = at + e < n ? bin_of(x) : BINS;  // a bin of their own behind the others
+    before[e] = sum;
+    sum += w[e];
+  }
+  const uint64_t ahead = wave_scan(sum) - sum;
+  // Where a bin's tokens begin here: what stands before that place is taken off
+  // what stands before the bin in the row.
+  const int left = __shfl_up(bin[E - 1], 1, 64);  // with every lane active
+  bool starts[E];
+  uint64_t begins = 0, offset[E];  // of the last bin that begins in this lane, then of each token's
+  int first = 0, head[E];
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    before[e] += ahead;
+    starts[e] = e == 0 ? lane == 0 || left != bin[0] : bin[e - 1] != bin[e];
+    begins = starts[e] ? before[e] : begins;
+    first = starts[e] ? at + e : first;
+    any = any || starts[e];
+  }
+  const uint64_t lower = __ballot(any) & ((1ull << lane) - 1ull);  // lane 0 begins one
+  const int from = lower ? 63 - __clzll(lower) : 0;
+  uint64_t run = ((uint64_t)(uint32_t)__shfl((int)(begins >> 32), from, 64) << 32) |
+                 (uint32_t)__shfl((int)(uint32_t)begins, from, 64);
+  int run_head = __shfl(first, from, 64);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    run = starts[e] ? before[e] : run;
+    run_head = starts[e] ? at + e : run_head;
+    offset[e] = run;
+    head[e] = run_head;
+  }
+  uint64_t kept = sh.total;
+  const bool by_rank = set.top_k > 0 && (uint32_t)set.top_k < sh.weighted;
+#pragma unroll
+  for (int e = 0; e < E; ++e) before[e] += sh.mass[min(bin[e], BINS - 1)] - offset[e];  // of the whole row
+  if (by_rank) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint64_t kth = __ballot(at + e < n && sh.count[min(bin[e], BINS - 1)] + (uint32_t)(at + e - head[e]) ==
+                                                      (uint32_t)set.top_k - 1);
+      if (kth) kept = lane64(before[e] + w[e], __ffsll((unsigned long long)kth) - 1);
+    }
+  }
+  // The masses before the tokens rise, so the tokens up to a bound are the first
+  // ones; the last of them is the one the bound falls in.
+  const auto last_up_to = [&](uint64_t bound, uint64_t &end, double &which) {
+    int count = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) count += __popcll(__ballot(at + e < n && before[e] <= bound));
+    const int place = count - 1;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (place % E == e) {
+        end = lane64(before[e] + w[e], place / E);
+        which = __longlong_as_double((int64_t)lane64((uint64_t)__double_as_longlong(word[e]), place / E));
+      }
+  };
+  uint64_t end = 0;
+  double drawn = 0.0;
   const uint64_t most = scaled_floor(set.top_p, kept);
-  if (set.top_p < 1.f && most < sh.binned)
-    kept = min(kept, lane64(before + w, __popcll(__ballot(on && before <= most)) - 1));
+  if (set.top_p < 1.f && most < sh.binned) {
+    last_up_to(most, end, drawn);
+    kept = min(kept, end);
+  }
   kept = min(kept, sh.likely);
-  const uint64_t aim = scaled_floor(set.uniform, kept);
-  const int at = __popcll(__ballot(on && before <= aim)) - 1;
-  const double drawn = __longlong_as_double((int64_t)lane64((uint64_t)__double_as_longlong(word), at));
+  last_up_to(scaled_floor(set.uniform, kept), end, drawn);
   const float share = weigh.log_share(word_logit(drawn), lane == 0 ? sh.total : kept);
   if (lane == 0) {
     p.tokens[b] = word_index(drawn);
