@@ -273,14 +273,15 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_pick_kernel(const Sa
 }
 
 // Workgroups of a row: one where it has up to 4 vectors a thread (us, one / split
-// by 4: 1 x 32000 bf16 17.7 / 17.7 and 16 x 32000 20.0 / 20.3, one launch for
-// three; 61 x 50257, 6.1 vectors, 31.9 / 30.0), else enough for 2 vectors a
-// thread as long as there is a compute unit for each (32 x 131072 bf16 in 1, 4, 8
-// and 16: 59.7, 33.4, 29.1, 32; 256 x 131072 fp32 in 1 and 4: 76, 110).
+// by 4, one launch for three: 1 x 32000 bf16 19.0 / 17.9, 64 x 32000 22.5 / 23.8,
+// 256 x 32000 23.6 / 55), else as many as have a vector a thread, as long as there
+// is a compute unit for each (bf16 x 131072, in 1, 4, 8 and 16: 1 row 60.5, 31.8,
+// 25.9, 22.9; 32 rows 71, 42, 37, 41; 128 rows 74, 65, 80, 113, in 2 59.5; 256
+// rows fp32 in 1 and 4: 72, 102).
 int parts_of(int64_t rows, int64_t vocab, int64_t dtype) {
   const int64_t per = dtype == IKL_F32 ? 4 : 8, vectors = (vocab + per - 1) / per;
   if (vectors <= 4 * SAMPLE_THREADS) return 1;
-  const int64_t most = (vectors + 2 * SAMPLE_THREADS - 1) / (2 * SAMPLE_THREADS), want = 256 / rows;
+  const int64_t most = (vectors + SAMPLE_THREADS - 1) / SAMPLE_THREADS, want = 256 / rows;
   const int64_t n = most < want ? most : want;
   return (int)(n < 1 ? 1 : n < MAX_PARTS ? n : MAX_PARTS);
 }
