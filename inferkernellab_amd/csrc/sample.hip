@@ -22,6 +22,24 @@
 namespace ikl {
 namespace {
 
+// Leaves the tokens of the cuts' bins in a list of `n` and returns their number.
+__device__ inline uint32_t drop_uncut(const Binner &bin_of, uint32_t n, RowShared &sh) {
+  constexpr int PER = LIST / SAMPLE_THREADS;
+  const Cuts cuts = sh.cuts;
+  double word[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) word[i] = sh.list[threadIdx.x + i * SAMPLE_THREADS];
+  __syncthreads();
+  if (threadIdx.x == 0) sh.listed = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (threadIdx.x + i * SAMPLE_THREADS < n && cuts.has(bin_of(word_logit(word[i]))))
+      sh.list[atomicAdd(&sh.listed, 1u)] = word[i];
+  __syncthreads();
+  return sh.listed;
+}
+
 // The draw of a row whose cuts' bins hold `n` tokens, listed if they are at most LIST.
 template <typename Tag>
 __device__ inline void draw(const SampleParams &p, int64_t b, const RowReader<Tag> &row, const RowSettings &set,
@@ -76,7 +94,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_row_kernel(const Sample
   clear_histogram(sh);
   if (threadIdx.x == 0) sh.listed = 0;
   float top = -INFINITY, least = INFINITY;
-  row.each(0, row.vectors, [&](int, const float(&x)[RowReader<Tag>::VEC]) { extremes(x, top, least); });
+  row_extremes(row, 0, row.vectors, top, least);
   block_extremes(top, least, sh);
   if (top == -INFINITY) {
     if (threadIdx.x == 0) store_nothing(p, b);
@@ -106,6 +124,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_row_kernel(const Sample
     __syncthreads();
     n = sh.listed;
   }
+  if (cand.alone && n > 64 && n <= LIST) n = drop_uncut(bin_of, n, sh);
   draw(p, b, row, set, weigh, bin_of, n, sh);
 }
 
@@ -171,7 +190,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_extremes_kernel(const S
     r.count[i] = 0;
   }
   float top = -INFINITY, least = INFINITY;
-  at.row.each(at.from, at.to, [&](int, const float(&x)[RowReader<Tag>::VEC]) { extremes(x, top, least); });
+  row_extremes(at.row, at.from, at.to, top, least);
   block_extremes(top, least, sh);
   if (threadIdx.x == 0) {
     r.top[at.part] = top;
@@ -183,7 +202,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_extremes_kernel(const S
   }
 }
 
-__device__ inline void row_extremes(const SplitRow &r, int parts, float &top, float &least) {
+__device__ inline void joined_extremes(const SplitRow &r, int parts, float &top, float &least) {
   const int lane = threadIdx.x & 63;  // MAX_PARTS lanes
   top = wave_max(lane < parts ? r.top[lane] : -INFINITY);
   least = -wave_max(lane < parts ? -r.least[lane] : -INFINITY);
@@ -199,7 +218,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_histogram_kernel(const 
   clear_histogram(sh);
   const RowSettings set = row_settings(p, at.b);
   float top, least;
-  row_extremes(r, parts, top, least);
+  joined_extremes(r, parts, top, least);
   if (top == -INFINITY || top == INFINITY) return;
   const Weigher weigh(top, set.temperature, p.fraction_bits, sh.roots);
   const Candidates cand(set, weigh);
@@ -235,7 +254,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_pick_kernel(const Sa
   }
   const RowSettings set = row_settings(p, at.b);
   float top, least;
-  row_extremes(r, parts, top, least);
+  joined_extremes(r, parts, top, least);
   if (top == -INFINITY || top == INFINITY) {  // nothing to weigh
     if (at.part != 0) return;
     if (top == INFINITY) sample_infinite(p, at.b, at.row, set, sh);

