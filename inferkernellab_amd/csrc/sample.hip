@@ -291,18 +291,21 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_pick_kernel(const Sa
   draw(p, at.b, at.row, set, weigh, bin_of, n, sh);
 }
 
-// Workgroups of a row: one where it has up to 4 vectors a thread (us, one / split
-// by 4, one launch for three: 1 x 32000 bf16 19.0 / 17.9, 64 x 32000 22.5 / 23.8,
-// 256 x 32000 23.6 / 55), else as many as have a vector a thread, as long as there
-// is a compute unit for each (bf16 x 131072, in 1, 4, 8 and 16: 1 row 60.5, 31.8,
-// 25.9, 22.9; 32 rows 71, 42, 37, 41; 128 rows 74, 65, 80, 113, in 2 59.5; 256
-// rows fp32 in 1 and 4: 72, 102).
+// Workgroups of a row. One is one launch, three where a row is split, which pays
+// from 24 tokens a thread (us, one / split by 4: 1 x 24000 bf16 16.0 / 17.6, 1 x
+// 16000 fp32 13.1 / 15.7, 1 x 32000 bf16 19.4 / 17.8, 48 x 32000 22.6 / 22.5): into
+// as many parts as have a vector a thread, as long as there is a compute unit for
+// each (bf16 x 131072, in 1, 4, 8 and 16: 1 row 60.5, 31.8, 25.9, 22.9; 32 rows 71,
+// 42, 37, 41; 128 rows 74, 65, 80, 113, in 2 59.5; 256 rows fp32 in 1 and 4: 64,
+// 102). Two parts do not pay for rows under 64 tokens a thread (100 x 50257 30.4
+// / 31.5).
 int parts_of(int64_t rows, int64_t vocab, int64_t dtype) {
+  if (vocab <= 24 * SAMPLE_THREADS) return 1;
   const int64_t per = dtype == IKL_F32 ? 4 : 8, vectors = (vocab + per - 1) / per;
-  if (vectors <= 4 * SAMPLE_THREADS) return 1;
   const int64_t most = (vectors + SAMPLE_THREADS - 1) / SAMPLE_THREADS, want = 256 / rows;
   const int64_t n = most < want ? most : want;
-  return (int)(n < 1 ? 1 : n < MAX_PARTS ? n : MAX_PARTS);
+  if (n < (vocab < 64 * SAMPLE_THREADS ? 3 : 2)) return 1;
+  return (int)(n < MAX_PARTS ? n : MAX_PARTS);
 }
 
 template <typename Tag>
