@@ -155,8 +155,10 @@ __device__ inline void shared_store(T *p, T v) {
 }
 
 // Whether this workgroup is the row's last to come here. Each wave waits for its
-// own operations to be complete before the workgroup's arrival is counted.
+// own operations to be complete before the workgroup's arrival is counted; the
+// fence keeps the compiler from moving any of them behind the wait.
 __device__ inline bool last_to_arrive(uint32_t *arrived, int parts, RowShared &sh) {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   if (threadIdx.x == 0) sh.found[0] = atomicAdd(arrived, 1u) == (uint32_t)(parts - 1);

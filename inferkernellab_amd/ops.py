@@ -27,7 +27,6 @@ from __future__ import annotations
 import array
 import contextlib
 import ctypes
-import math
 
 import torch
 
@@ -708,7 +707,8 @@ def _qk_norm_rope_args(query, key, value, q_weight, k_weight, cos, sin, cache, s
         q_weight = _head_weight(q_weight, "q_weight", query.shape[1], query, layout.head_dim)
         args.q_weight, args.q_weight_stride_h = q_weight.data_ptr(), q_weight.stride(0) if q_weight.ndim == 2 else 0
     args.eps = eps
-    return args, (query, query_out, key, value, q_weight, k_weight, cos, sin, slots, cache.k, cache.v), query_out
+    return args, (query, query_out, key, value, q_weight, k_weight, cos, sin, slots, cache,
+                  cache.k, cache.v, cache.k_scale, cache.v_scale), query_out
 
 
 def qk_norm_rope_append_kv_hip(query: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor,
@@ -775,18 +775,23 @@ def _dense_page(pages: torch.Tensor) -> bool:
 def _copy_args(cache, src: int, dst: int, count: int, index_type: int, on_host: bool):
     layout = cache.layout
     bs, heads, dim = layout.block_size, layout.num_kv_heads, layout.head_dim
-    tensors = (cache.k, cache.v, cache.k_scale, cache.v_scale) if cache.fp8 else (cache.k, cache.v)
-    base, page, layer, block = [], [], [], []
-    for t in tensors:
-        size, strides = t.element_size(), t.stride()
-        # the cache's own two layouts, else any dense one
-        if strides[2:] not in ((heads * dim, dim, 1), (dim, bs * dim, 1)) and not _dense_page(t):
+    k, v = cache.k, cache.v
+    ks, vs, size, rows = k.stride(), v.stride(), k.element_size(), bs * heads
+    for strides, t in ((ks, k), (vs, v)):  # the cache's own two layouts, else any dense one
+        if strides[2:] != (heads * dim, dim, 1) and strides[2:] != (dim, bs * dim, 1) and not _dense_page(t):
             raise ValueError("cache pages must be dense")
-        base.append(t.data_ptr())
-        page.append(math.prod(t.shape[2:]) * size)
-        layer.append(strides[0] * size)
-        block.append(strides[1] * size)
-    return _lib.CopyBlocksArgs(tuple(base), tuple(page), tuple(layer), tuple(block), len(tensors), layout.num_layers,
+    page = rows * dim * size
+    if not cache.fp8:
+        return _lib.CopyBlocksArgs((k.data_ptr(), v.data_ptr()), (page, page), (ks[0] * size, vs[0] * size),
+                                   (ks[1] * size, vs[1] * size), 2, layout.num_layers, layout.num_blocks, src, dst, count,
+                                   index_type, on_host)
+    scales = (cache.k_scale, cache.v_scale)
+    if not all(_dense_page(t) for t in scales):
+        raise ValueError("cache pages must be dense")
+    return _lib.CopyBlocksArgs((k.data_ptr(), v.data_ptr(), *(t.data_ptr() for t in scales)),
+                               (page, page, rows * 4, rows * 4),
+                               (ks[0] * size, vs[0] * size, *(t.stride(0) * 4 for t in scales)),
+                               (ks[1] * size, vs[1] * size, *(t.stride(1) * 4 for t in scales)), 4, layout.num_layers,
                                layout.num_blocks, src, dst, count, index_type, on_host)
 
 
@@ -797,10 +802,10 @@ def copy_blocks_hip(cache, src, dst, *, validate_inputs: bool = True) -> None:
     ``src`` / ``dst``: lists of block ids on the host, or int32 / int64 GPU
     tensors. Ids outside the cache, a page written twice and one that is both
     read and written raise ``ValueError``; for tensors that check reads them
-    back, and ``validate_inputs=False`` leaves it out: pairs with an id outside
-    the cache are then skipped, and keeping the written pages apart is the
-    caller's part. Lists travel with the launch (a captured one keeps them);
-    tensors are read when it runs.
+    back, and ``validate_inputs=False`` leaves it out (a capture has to): pairs
+    with an id outside the cache are then skipped, and keeping the written pages
+    apart is the caller's part. Lists travel with the launch (a captured one
+    keeps them); tensors are read when it runs.
     """
     lib = _require_backend()
     if cache.device.type != "cuda":
