@@ -80,8 +80,10 @@ __global__ __launch_bounds__(COPY_THREADS) void copy_blocks_kernel(const CopyPar
 
 template <typename Unit, typename Pairs>
 int launch(const CopyParams &p, const Pairs &pairs, int64_t count, hipStream_t s) {
-  const int64_t grid = count * p.num_layers * p.first[p.num_tensors];
-  if (grid > 0x7fffffffLL) return fail(IKL_EINVAL, "copy blocks: too many pages for one launch");
+  int64_t grid;
+  if (__builtin_mul_overflow(count, (int64_t)p.num_layers, &grid) ||
+      __builtin_mul_overflow(grid, p.first[p.num_tensors], &grid) || grid > 0x7fffffffLL)
+    return fail(IKL_EINVAL, "copy blocks: too many pages for one launch");
   copy_blocks_kernel<Unit, Pairs><<<dim3((unsigned)grid), COPY_THREADS, 0, s>>>(p, pairs);
   return check_launch("copy blocks launch");
 }

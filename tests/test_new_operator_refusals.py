@@ -109,6 +109,14 @@ def test_copy_refuses_arguments(bad):
     assert "copy blocks" in _lib.last_error()
 
 
+@pytest.mark.parametrize("pairs,layers", [(1 << 31, 1), (1 << 34, 1 << 30), ((1 << 63) - 1, 2)])
+def test_copy_refuses_more_pages_than_a_launch_holds(pairs, layers):
+    """Also where their number wraps round 64 bits (16 Gi pairs of 2^30 layers: to 0)."""
+    a, keep = _copy([0], [1], num_pairs=pairs, num_layers=layers, pairs_on_host=0)
+    assert _lib.load().ikl_copy_blocks(ctypes.byref(a), None) == _lib.IKL_EINVAL
+    assert "too many pages" in _lib.last_error()
+
+
 def test_copy_of_nothing():
     lib = _lib.load()
     assert lib.ikl_copy_blocks(None, None) == _lib.IKL_EINVAL
