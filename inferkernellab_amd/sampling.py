@@ -54,7 +54,8 @@ def _sample_args(logits, uniform, temperature, top_k, top_p, min_p):
     a = _lib.SampleArgs()
     a.temperature, heat = _setting(temperature, "temperature", rows, device,
                                    lambda v: math.isfinite(v) and v >= 0, "finite and non-negative")
-    number, first = _setting(top_k, "top_k", rows, device, lambda v: v == int(v) and v >= 0,
+    number, first = _setting(top_k, "top_k", rows, device,
+                             lambda v: (isinstance(v, int) or float(v).is_integer()) and v >= 0,
                              "a non-negative whole number")
     a.top_k = min(int(number), vocab)  # any from the vocabulary on keeps every token
     a.top_p, nucleus = _setting(top_p, "top_p", rows, device, lambda v: 0 < v <= 1, "in (0, 1]")

@@ -142,6 +142,33 @@ def test_slots_outside_the_cache_are_skipped():
         run(case)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_offsets_past_32_bits(fp8):
+    """The last pages of a cache of more than 4 GiB a tensor: the same rows as in a small one."""
+    from inferkernellab_amd import qk_norm_rope_append_kv_hip
+    from inferkernellab_amd.cache import PagedKVCache
+
+    case = make(torch.bfloat16, 20, 8, 8, 128, fp8=fp8, layers=1)
+    blocks = 280000 if fp8 else 140000
+    bits = torch.uint8 if fp8 else torch.int16
+    long = PagedKVCache(blocks, 16, 8, 128, num_layers=1, device="cuda", head_major=False,
+                        dtype=torch.float8_e4m3fn if fp8 else torch.bfloat16, act_dtype=torch.bfloat16 if fp8 else None)
+    small = case["cache"]
+    far = case["slots"] + (blocks - small.layout.num_blocks) * 16
+    rows = [case[n] for n in ("query", "key", "value", "q_weight", "k_weight", "cos", "sin")]
+    outs = [qk_norm_rope_append_kv_hip(rows[0].clone(), *rows[1:], cache, slots)
+            for cache, slots in ((small, case["slots"]), (long, far))]
+    assert torch.equal(*outs)
+    for cache, slots in ((small, case["slots"]), (long, far)):
+        at = (0, slots.long() // 16, slots.long() % 16)
+        got = [cache.k.view(bits)[at], cache.v.view(bits)[at]]
+        if fp8:
+            got += [cache.k_scale[0, at[1], :, at[2]], cache.v_scale[0, at[1], :, at[2]]]
+        if cache is small:
+            want = got
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_strided_operands():
     """Columns of one fused projection, a misaligned view and transposed rows."""
     case = make(torch.bfloat16, 18, 8, 2, 64, seed=3)

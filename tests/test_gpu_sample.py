@@ -152,6 +152,105 @@ def test_masked_and_odd_values():
     check(half, uniform, top_k=5, top_p=0.9)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [24576, 24577, 40003])
+def test_masked_and_odd_values_of_long_rows(vocab, dtype):
+    """The same on both sides of the length from which rows are split, with NaN, masks and infinities in some
+    workgroups' parts only."""
+    inf, nan = float("inf"), float("nan")
+    gen = torch.Generator().manual_seed(17)
+    low = torch.finfo(DTYPES[dtype]).min
+    x = torch.randn(14, vocab, generator=gen) * 2
+    x[0] = -inf
+    x[1] = nan
+    x[2, 5:] = -inf
+    x[3] = -inf
+    x[3, vocab - 1] = -1e30
+    x[4, ::2] = nan
+    x[5, [10, vocab // 2, vocab - 1]] = inf
+    x[6] = low
+    x[7, 1:] = low
+    x[8] = 0.0
+    x[8, ::2] = -0.0
+    x[9, :vocab // 2] = -inf
+    x[10] = inf
+    x[11, :vocab - 3000] = nan
+    x[12] = (torch.randint(0, 6, (vocab,), generator=gen)).float()   # ties at every cut
+    x[13] = 1e4                                                      # one heavy token among equal ones
+    x[13, vocab // 3] = 1e4 + 64
+    logits = x.to(DTYPES[dtype]).cuda()
+    uniform = torch.rand(14, generator=gen).cuda()
+    for settings in (dict(), dict(top_k=3), dict(top_k=3000, top_p=0.7), dict(top_p=0.7), dict(min_p=0.2),
+                     dict(top_p=0.9, min_p=0.01), dict(top_k=500, min_p=0.01), dict(top_k=20000, top_p=0.8, min_p=0.05),
+                     dict(min_p=1.0), dict(temperature=0.0), dict(temperature=1e-30),
+                     dict(temperature=1e30, top_p=0.6)):
+        print(vocab, dtype, settings, flush=True)
+        check(logits, uniform, **settings)
+
+
+@pytest.mark.parametrize("spread", [0.0, 1e-3, 0.3, 30.0])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_flat_and_steep_long_rows(spread, dtype):
+    gen = torch.Generator().manual_seed(18)
+    logits = (torch.randn(3, 40009, generator=gen) * spread).to(DTYPES[dtype]).cuda()
+    uniform = torch.rand(3, generator=gen).cuda()
+    for settings in (dict(), dict(top_p=0.9), dict(top_k=9000, top_p=0.5), dict(min_p=0.9),
+                     dict(top_k=9000, min_p=0.5)):
+        print(spread, dtype, settings, flush=True)
+        check(logits, uniform, **settings)
+
+
+def test_long_rows_with_settings_per_row_and_strides():
+    rows = 20
+    base, uniform = inputs(rows, 60100, "fp16", 19)
+    gen = torch.Generator().manual_seed(20)
+
+    def pick(values, dtype=torch.float32):
+        return torch.tensor(values, dtype=dtype)[torch.randint(0, len(values), (rows,), generator=gen)].cuda()
+
+    for view in (base[:, 3:50260], base[:, :50257], base[2:3, 1:50002].expand(rows, -1)):
+        check(view, uniform, temperature=pick([0.0, 0.5, 1.0, 2.0]), top_k=pick([0, 1, 30, 3000, 99999], torch.int64),
+              top_p=pick([1.0, 0.9, 0.2]), min_p=pick([0.0, 0.001, 0.3, 1.0]))
+
+
+def test_one_sampler_on_rows_that_change_kind():
+    """A workspace keeps nothing: the same split rows drawn from, then masked, then infinite, then drawn from again."""
+    from inferkernellab_amd import PreparedSampler
+    base, uniform = inputs(2, 50257, "bf16", 21)
+    logits = base.clone()
+    call = PreparedSampler(logits, uniform, top_p=0.9, min_p=0.01, logprobs=True)
+    for fill in (None, float("-inf"), 0.0, None, float("inf"), float("nan"), None):
+        logits.copy_(base) if fill is None else logits.fill_(fill)
+        check(logits, uniform, top_p=0.9, min_p=0.01, got=call())
+
+
+def test_more_rows_than_a_grid_dimension_of_16_bits():
+    gen = torch.Generator().manual_seed(22)
+    logits = torch.randn(70001, 3, generator=gen).cuda()
+    uniform = torch.rand(70001, generator=gen).cuda()
+    from inferkernellab_amd import sample_tokens_hip
+    got = sample_tokens_hip(logits, uniform, logprobs=True)
+    check(logits[-50:], uniform[-50:], got=[t[-50:] for t in got])
+
+
+def test_eager_call_inside_a_capture():
+    from inferkernellab_amd import sample_tokens_hip
+    logits, uniform = inputs(4, 50257, "bf16", 23)
+    sample_tokens_hip(logits, uniform, top_k=20)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        got = sample_tokens_hip(logits, uniform, top_k=20, logprobs=True)
+    gen = torch.Generator().manual_seed(24)
+    for _ in range(4):
+        uniform.copy_(torch.rand(4, generator=gen))
+        logits.copy_(torch.roll(logits, 1001, 1))
+        g.replay()
+        (logits.float().sum()).item()
+        check(logits, uniform, top_k=20, got=got)
+
+
 def test_settings_per_row_and_out_of_range():
     rows = 24
     logits, uniform = inputs(rows, 5003, "fp16", 8)
@@ -243,7 +342,8 @@ def test_refusals():
     from inferkernellab_amd import PreparedSampler, sample_tokens_hip
     logits, uniform = inputs(4, 100, "fp32", 16)
     for bad, message in ((dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
-                         (dict(top_k=-1), "top_k"), (dict(top_k=1.5), "top_k"), (dict(top_p=0.0), "top_p"),
+                         (dict(top_k=-1), "top_k"), (dict(top_k=1.5), "top_k"), (dict(top_k=float("inf")), "top_k"),
+                         (dict(top_p=0.0), "top_p"),
                          (dict(top_p=1.1), "top_p"), (dict(min_p=-0.1), "min_p"), (dict(min_p=1.1), "min_p"),
                          (dict(top_k=torch.ones(4).cuda()), "top_k"), (dict(top_p=torch.ones(3).cuda()), "top_p"),
                          (dict(min_p=torch.ones(4)), "min_p"),
