@@ -7,10 +7,14 @@
  *   - paged decode attention for MHA / GQA / MQA over a block-table
  *     addressed cache, with optional split-context partitions and a
  *     log-sum-exp reduce kernel.
+ * Around them: the rotary append (with norms of the heads where a model has
+ * them), paged prefill attention, a whole decode step, copies of pages, the
+ * drawing of tokens and a Llama layer's small kernels.
  *
  * Conventions
  *   - Every pointer is a device pointer (HBM) except the argument structs
- *     themselves, which live in host memory and are read during the call.
+ *     themselves, which live in host memory and are read during the call
+ *     (and ikl_copy_blocks' block ids where pairs_on_host says so).
  *   - Strides are in ELEMENTS of the tensor they describe, not bytes.
  *   - The cache layout is the reference's [layers, blocks, block_size,
  *     kv_heads, head_dim]; callers pass the base pointer of ONE layer

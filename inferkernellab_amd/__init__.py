@@ -1,10 +1,12 @@
 """MI355X (gfx950) paged-KV decode path for InferKernelLab.
 
-Hand-written HIP kernels (KV append, fused RoPE + append, paged decode
-attention with split partitions, paged prefill attention) behind the C ABI
-of include/ikl_paged.h, with the reference's operator surface (ops), paged
-cache (cache), scheduler and runtime hooks, and the decode runners that
-call them (decode: synthetic decoder; llama: Llama over the paged cache).
+Hand-written HIP kernels (KV append, fused RoPE + append with and without
+norms of the heads, paged decode attention with split partitions, paged
+prefill attention, page copies, token sampling) behind the C ABI of
+include/ikl_paged.h, with the reference's operator surface (ops), the drawing
+of tokens (sampling), paged cache (cache), scheduler and runtime hooks, and
+the decode runners that call them (decode: synthetic decoder; llama: Llama
+over the paged cache).
 """
 
 from .cache import BlockAllocator, CacheLayout, PagedKVCache

@@ -16,6 +16,10 @@ reference's Triton operators:
 * :func:`hip_available` / :func:`hip_append_available` —
   ``triton_available`` / ``triton_append_available``.
 
+Without a counterpart there: :func:`qk_norm_rope_append_kv_hip` (norms of the
+query and key heads, RoPE and the append) and :func:`copy_blocks_hip` (pages
+copied over all layers).
+
 The ``*_triton`` names are kept as aliases of the same functions so callers
 written against the reference bind unchanged. Every operator launches the
 HIP kernels on the current torch stream and never computes on another path:
