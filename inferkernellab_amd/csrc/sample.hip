@@ -68,11 +68,12 @@ __device__ inline void list_tokens(const RowReader<Tag> &row, int from, int to, 
       float y = x[0];
 #pragma unroll
       for (int k = 1; k < RowReader<Tag>::VEC; ++k) y = j == k ? x[k] : y;
-      if (!weigh.counts(y)) continue;
+      if (!weigh.counts(y)) continue;  // those that come to 0 all the same stand behind all others
       if (cand.alone) {
-        double exact;
-        weigh.of(y, exact);
-        if (exact < cand.least) continue;
+        const float one[1] = {y};
+        double exact[1];
+        weigh.of(one, exact);
+        if (exact[0] < cand.least) continue;
       }
       const uint32_t at = atomicAdd(&sh.listed, 1u);
       if (at < LIST) sh.list[at] = token_word(order_key(clean(y)), first + j);
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_row_kernel(const Sample
   const int64_t b = blockIdx.x;
   const RowReader<Tag> row(p.logits + b * p.stride, p.vocab);
   const RowSettings set = row_settings(p, b);
-  fill_roots(sh.roots);
+  fill_roots(sh.roots, p.fraction_bits);
   clear_histogram(sh);
   if (threadIdx.x == 0) sh.listed = 0;
   float top = -INFINITY, least = INFINITY;
@@ -216,7 +217,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_histogram_kernel(const 
   const Part<Tag> at(p, parts);
   SplitRow &r = rows[at.b];
   const v4u32 begin = at.row.begin(at.from, at.to);  // on its way meanwhile
-  fill_roots(sh.roots);
+  fill_roots(sh.roots, p.fraction_bits);
   clear_histogram(sh);
   const RowSettings set = row_settings(p, at.b);
   float top, least;
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_pick_kernel(const Sa
     else if (threadIdx.x == 0) store_nothing(p, at.b);
     return;
   }
-  fill_roots(sh.roots);
+  fill_roots(sh.roots, p.fraction_bits);
 #pragma unroll
   for (int i = 0; i < BINS / SAMPLE_THREADS; ++i) {
     sh.mass[threadIdx.x + i * SAMPLE_THREADS] = mass[i];
@@ -294,13 +295,12 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_pick_kernel(const Sa
 }
 
 // Workgroups of a row. One is one launch, three where a row is split, which pays
-// from 24 tokens a thread (us, one / split by 4: 1 x 24000 bf16 16.0 / 17.6, 1 x
-// 16000 fp32 13.1 / 15.7, 1 x 32000 bf16 19.4 / 17.8, 48 x 32000 22.6 / 22.5): into
-// as many parts as have a vector a thread, as long as there is a compute unit for
-// each (bf16 x 131072, in 1, 4, 8 and 16: 1 row 60.5, 31.8, 25.9, 22.9; 32 rows 71,
-// 42, 37, 41; 128 rows 74, 65, 80, 113, in 2 59.5; 256 rows fp32 in 1 and 4: 64,
-// 102). Two parts do not pay for rows under 64 tokens a thread (100 x 50257 30.4
-// / 31.5).
+// from 24 tokens a thread (us with top-p 0.95, one / split by 4: 1 x 24000 bf16 16.5
+// / 17.9, 1 x 16000 fp32 13.1 / 16.4, 1 x 32000 bf16 20.4 / 19.4, 48 x 32000 22.4 /
+// 23.3): into as many parts as have a vector a thread, as long as there is a compute
+// unit for each (bf16 x 131072, in 1, 4, 8 and 16: 1 row 60, 33, 28, 25; 32 rows 69,
+// 43, 38, 45; 128 rows 71, 68, 85, 126, in 2 59; 256 rows fp32 in 1 and 4: 90, 118).
+// Two parts do not pay for rows under 64 tokens a thread (100 x 50257 36.7 / 38.3).
 int parts_of(int64_t rows, int64_t vocab, int64_t dtype) {
   if (vocab <= 24 * SAMPLE_THREADS) return 1;
   const int64_t per = dtype == IKL_F32 ? 4 : 8, vectors = (vocab + per - 1) / per;

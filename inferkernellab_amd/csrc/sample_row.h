@@ -92,17 +92,17 @@ struct RowReader {
     if constexpr (EB == 4) return __uint_as_float(w[j]);
     else return (j & 1) ? elem<Tag>::hi(w[j >> 1]) : elem<Tag>::lo(w[j >> 1]);
   }
+  static constexpr uint32_t NONE = std::is_same<Tag, f32_tag>::value   ? 0xff800000u
+                                   : std::is_same<Tag, f16_tag>::value ? 0xfc00u
+                                                                       : 0xff80u;  // -inf
   __device__ inline v4u32 load(int v) const {
     const char *at = base + (int64_t)v * 16;
     if (v * VEC >= shift && (v + 1) * VEC <= vocab + shift) return load16v_global(at);
-    const uint32_t none = std::is_same<Tag, f32_tag>::value   ? 0xff800000u
-                          : std::is_same<Tag, f16_tag>::value ? 0xfc00u
-                                                              : 0xff80u;
     v4u32 w = {0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       const int i = v * VEC + j - shift;
-      uint32_t e = none;
+      uint32_t e = NONE;
       if (i >= 0 && i < vocab) {
         if constexpr (EB == 4) e = reinterpret_cast<const uint32_t *>(at)[j];
         else e = reinterpret_cast<const uint16_t *>(at)[j];
@@ -112,32 +112,49 @@ struct RowReader {
     }
     return w;
   }
-  // f(index of the first, values) for the vectors [from, to), each thread's in
-  // order; the next vector is on its way meanwhile. By vectors, so that what is
-  // done to its elements can overlap.
+  // A vector that is the row's whole: all but the first and the last are.
+  __device__ inline v4u32 load_whole(int v) const { return load16v_global(base + (int64_t)v * 16); }
+  // `to`, or the last vector before it if other elements share that one
+  __device__ inline int whole_end(int to) const { return to == vectors && (vocab + shift) % VEC ? to - 1 : to; }
+
+  // f(index of the first, values) for the vectors [from, to), by vectors, so that
+  // what is done to its elements can overlap; a thread's next one is on its way
+  // meanwhile. Vectors that are not the row's whole are loaded by begin() alone:
+  // the thread that has a last one behind the first round begins with it. (With
+  // loads of either kind in the loop, the wait for them stands before the work: 256
+  // x 131072 fp32 64 us, else 59.)
   template <typename F>
   __device__ inline void each(int from, int to, F f) const {
     each(from, to, begin(from, to), f);
   }
   // the same, with the thread's first vector loaded some time before by begin()
+  __device__ inline bool begins_at_end(int from, int to) const {
+    const int last = to - 1 - from, its = last % SAMPLE_THREADS;  // the first thread may begin with the first vector
+    return (int)threadIdx.x == (its ? its : SAMPLE_THREADS - 1) && last >= SAMPLE_THREADS && whole_end(to) != to;
+  }
   __device__ inline v4u32 begin(int from, int to) const {
-    const int v = from + threadIdx.x;
+    const int v = begins_at_end(from, to) ? to - 1 : from + (int)threadIdx.x;
     return v < to ? load(v) : v4u32{0, 0, 0, 0};
   }
   template <typename F>
   __device__ inline void each(int from, int to, v4u32 w, F f) const {
-    int v = from + threadIdx.x;
+    int v = from + threadIdx.x, ahead = v + SAMPLE_THREADS;
     if (v >= to) return;
+    if (begins_at_end(from, to)) {
+      ahead = v;
+      v = to - 1;
+    }
+    const int end = whole_end(to);
     while (true) {
-      const int ahead = v + SAMPLE_THREADS;
       v4u32 next = w;
-      if (ahead < to) next = load(ahead);
+      if (ahead < end) next = load_whole(ahead);
       float x[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) x[j] = value(w, j);
       f(v * VEC - shift, x);
-      if (ahead >= to) return;
+      if (ahead >= end) return;
       v = ahead;
+      ahead += SAMPLE_THREADS;
       w = next;
     }
   }
@@ -155,46 +172,66 @@ __host__ __device__ inline int fraction_bits(int64_t vocab) {
 // w(x) = 2^((x - m) log2(e) / T) as the nearest integer to w 2^bits, and
 // unrounded in units of 2^-bits. 2^(k/32 + r/32) for whole k and |r| <= 1/2 is
 // a power of two, one of 32 roots in shared memory (64 banks: no two entries
-// collide) and the Taylor series of 2^(r/32) up to r^5, whose next term is
-// 2.2e-15 of the value. m is finite; tokens that round to no unit, NaN and -inf
-// have no weight. The products and sums are fused where it says so and nowhere
-// else: a token weighs the same in every kernel.
+// collide; they hold the 2^bits too) and the Taylor series of 2^(r/32) up to r^5,
+// whose next term is 2.2e-15 of the value. m is finite; NaN, -inf and whatever
+// else weighs under half a unit come to 0. The products and sums are fused where
+// it says so and nowhere else: a token weighs the same in every kernel.
 struct Weigher {
-  double m, rate, floor;  // rate: 32 log2(e) / T; floor: of x - m, just above half a unit
+  double m, rate, floor;  // rate: 32 log2(e) / T; floor: of x - m, a quarter of a unit
   const double *roots;
   int bits;
   __device__ inline Weigher(float top, float temperature, int fraction, const double *table)
       : m(top), roots(table), bits(fraction) {
-    const double t = temperature;  // its reciprocal by Newton's steps: a division costs three times as much
+    const double t = fmin((double)temperature, 1e300);  // its reciprocal by Newton's steps: a division costs thrice
     double r = __builtin_amdgcn_rcp(t);
     r = fma(fma(-t, r, 1.0), r, r);
     r = fma(fma(-t, r, 1.0), r, r);
-    rate = temperature < INFINITY ? 32.0 * 1.4426950408889634 * r : 0.0;
-    floor = -(fraction + 1 - 1e-9) * 0.69314718055994531 * t;
+    rate = 32.0 * 1.4426950408889634 * r;
+    floor = -(fraction + 2) * 0.69314718055994531 * t;
   }
   __device__ inline double scaled(float w) const { return ldexp((double)w, bits); }
+  // Whether a token may weigh something: false for what is masked, NaN or -inf.
   __device__ inline bool counts(float x) const { return (double)x - m > floor; }
-  // of a token that counts
-  __device__ inline uint64_t of(float x, double &exact) const {
+  // Unrounded weights of N tokens; step by step for all of them, as their chains
+  // of 15 operations and a load are to overlap.
+  template <int N>
+  __device__ inline void of(const float (&x)[N], double (&exact)[N]) const {
 #pragma clang fp contract(off)
-    const double d = (double)x - m;
-    const double z = fma(d, rate, 0x1.8p52);  // its low word: the nearest whole number
-    const int k = (int)(uint32_t)__double_as_longlong(z);
-    const double r = fma(d, rate, -(z - 0x1.8p52));
-    double q = 3.9737099845494154e-11;  // (ln(2) / 32)^i / i!
-    q = fma(q, r, 9.172562701824643e-09);
-    q = fma(q, r, 1.6938509724371819e-06);
-    q = fma(q, r, 0.00023459619820224677);
-    q = fma(q, r, 0.02166084939249829);
-    q = fma(q, r, 1.0);
-    const double v = roots[k & 31] * q;
-    exact = __hiloint2double(__double2hiint(v) + (((k >> 5) + bits) << 20), __double2loint(v));
-    // rounded to a whole number by the addition: doubles from 2^52 are 1 apart
+    double r[N], root[N], q[N];
+    int k[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const double d = fmax((double)x[j] - m, floor);
+      const double z = fma(d, rate, 0x1.8p52);  // its low word: the nearest whole number
+      k[j] = (int)(uint32_t)__double_as_longlong(z);
+      root[j] = roots[k[j] & 31];
+      r[j] = fma(d, rate, -(z - 0x1.8p52));
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) q[j] = fma(3.9737099845494154e-11, r[j], 9.172562701824643e-09);
+#pragma unroll
+    for (int j = 0; j < N; ++j) q[j] = fma(q[j], r[j], 1.6938509724371819e-06);  // (ln(2) / 32)^i / i!
+#pragma unroll
+    for (int j = 0; j < N; ++j) q[j] = fma(q[j], r[j], 0.00023459619820224677);
+#pragma unroll
+    for (int j = 0; j < N; ++j) q[j] = fma(q[j], r[j], 0.02166084939249829);
+#pragma unroll
+    for (int j = 0; j < N; ++j) q[j] = fma(q[j], r[j], 1.0);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const double v = root[j] * q[j];
+      exact[j] = __hiloint2double(__double2hiint(v) + ((k[j] & ~31) << 15), __double2loint(v));
+    }
+  }
+  // Rounded to a whole number by the addition: doubles from 2^52 are 1 apart.
+  __device__ inline static uint64_t rounded(double exact) {
     return (uint64_t)(__double_as_longlong(exact + 0x1p52) - __double_as_longlong(0x1p52));
   }
   __device__ inline uint64_t operator()(float x) const {
-    double exact;
-    return counts(x) ? of(x, exact) : 0;
+    const float one[1] = {x};
+    double exact[1];
+    of(one, exact);
+    return rounded(exact[0]);
   }
   // ln of the share of token x in `mass`
   __device__ inline float log_share(float x, uint64_t mass) const {
@@ -209,8 +246,8 @@ struct InfiniteWeigher {
   __device__ inline float log_share(float, uint64_t mass) const { return (float)-log(ldexp((double)mass, -bits)); }
 };
 
-__device__ inline void fill_roots(double *table) {
-  if (threadIdx.x < 32) table[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
+__device__ inline void fill_roots(double *table, int bits) {
+  if (threadIdx.x < 32) table[threadIdx.x] = ldexp(exp2((double)threadIdx.x / 32.0), bits);
 }
 
 // floor(r m) for r in [0, 1): r is a whole number of at most 24 bits over a power of two.
@@ -248,7 +285,7 @@ struct RowShared {
   double roots[32];
   Cuts cuts;
   uint64_t total, likely, binned;  // mass of the row, of what min-p leaves of it, in the histogram
-  uint64_t others;                 // mass of what min-p takes
+  uint64_t others;                 // mass of what min-p takes; of all where candidates are alone
   uint32_t weighted, listed;       // tokens in the histogram (where top-k asks), in the list
 };
 
@@ -501,10 +538,11 @@ __device__ inline int word_index(double word) {
 // where the first k need not be weighed without them, only their mass counts
 // (top-p's share is of it too): they stay out of the histogram.
 struct Candidates {
-  double least;  // weight of a candidate; 0 without min-p
+  double least;  // weight of a candidate: more than half a unit, which rounds to 1
   bool alone;    // in the histogram
   __device__ inline Candidates(const RowSettings &set, const Weigher &weigh)
-      : least(weigh.scaled(set.min_p)), alone(set.min_p > 0.f && !(set.top_k > 0 && set.top_p < 1.f)) {}
+      : least(fmax(weigh.scaled(set.min_p), 0x1.0000000000001p-1)),
+        alone(set.min_p > 0.f && !(set.top_k > 0 && set.top_p < 1.f)) {}
 };
 
 // Bins are even steps of the logit from the largest down to the smallest, at
@@ -524,36 +562,50 @@ struct Binner {
   }
 };
 
-// Adds tokens to the histogram, and to `others` those that are no candidates.
-// All weights first, whether they count or not (an empty asm keeps them there):
-// one takes a chain of 15 fp64 operations, and the chains overlap.
-// LISTED: those that are alone in the histogram go to sh.list as well.
+// Adds a token to the histogram. LISTED: one that is alone there to sh.list as well.
+template <bool LISTED>
+__device__ inline void add_token(int index, float x, uint64_t w, const RowSettings &set, const Binner &bin_of,
+                                 RowShared &sh) {
+  const int bin = bin_of(x);
+  atomicAdd((unsigned long long *)&sh.mass[bin], (unsigned long long)w);
+  if (set.top_k > 0) atomicAdd(&sh.count[bin], 1u);
+  if (LISTED) {
+    const uint32_t at = atomicAdd(&sh.listed, 1u);
+    if (at < LIST) sh.list[at] = token_word(order_key(clean(x)), index);
+  }
+}
+
+// Adds tokens to the histogram, and to `others` what min-p asks for: the mass of
+// all tokens where candidates are alone in the histogram (there most waves have
+// none and are done with a sum), else that of the tokens that are none.
 template <bool LISTED, int N>
 __device__ inline void add_tokens(int index, const float (&x)[N], const RowSettings &set, const Weigher &weigh,
                                   const Candidates &cand, const Binner &bin_of, uint64_t &others, RowShared &sh) {
-  uint64_t w[N];
   double exact[N];
+  weigh.of(x, exact);
+  uint64_t w[N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) w[j] = weigh.of(x[j], exact[j]);
+  for (int j = 0; j < N; ++j) w[j] = weigh.rounded(exact[j]);
+  if (cand.alone) {
+    uint32_t hits = 0;
 #pragma unroll
-  for (int j = 0; j < N; ++j) asm volatile("" : "+v"(w[j]));
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    bool in = weigh.counts(x[j]);
-    if (cand.least > 0.0) {
-      const bool other = in && exact[j] < cand.least;
-      others += other ? w[j] : 0;
-      in = in && !(other && cand.alone);
+    for (int j = 0; j < N; ++j) {
+      others += w[j];
+      hits |= (uint32_t)(exact[j] >= cand.least) << j;
     }
-    if (in) {
-      const int bin = bin_of(x[j]);
-      atomicAdd((unsigned long long *)&sh.mass[bin], (unsigned long long)w[j]);
-      if (set.top_k > 0) atomicAdd(&sh.count[bin], 1u);
-      if (LISTED && cand.alone) {
-        const uint32_t at = atomicAdd(&sh.listed, 1u);
-        if (at < LIST) sh.list[at] = token_word(order_key(clean(x[j])), index + j);
-      }
+    if (hits) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (hits >> j & 1) add_token<LISTED>(index + j, x[j], w[j], set, bin_of, sh);
     }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (w[j]) add_token<false>(index + j, x[j], w[j], set, bin_of, sh);
+  if (set.min_p > 0.f) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) others += exact[j] < cand.least ? w[j] : 0;
   }
 }
 
@@ -598,7 +650,7 @@ __device__ inline void find_cuts(const RowSettings &set, const Candidates &cand,
 #pragma unroll
     for (int i = 0; i < PER; ++i) sh.count[at + i] = (uint32_t)(ahead + rank[i]);
   }
-  const uint64_t total = cand.alone ? binned + sh.others : binned, likely = total - sh.others;
+  const uint64_t total = cand.alone ? sh.others : binned, likely = cand.alone ? binned : total - sh.others;
   __syncthreads();
   if (threadIdx.x < 64) {
     const auto end = [&](int bin) { return bin + 1 < BINS ? sh.mass[bin + 1] : binned; };
