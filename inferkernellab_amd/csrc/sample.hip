@@ -44,10 +44,11 @@ __device__ inline uint32_t drop_uncut(const Binner &bin_of, uint32_t n, RowShare
 template <typename Tag>
 __device__ inline void draw(const SampleParams &p, int64_t b, const RowReader<Tag> &row, const RowSettings &set,
                             const Weigher &weigh, const Binner &bin_of, uint32_t n, RowShared &sh) {
-  if (n > LIST) sample_by_radix<Tag>(p, b, row, set, weigh, sh);
-  else if (n > 256) sample_from_list(p, b, set, weigh, bin_of, (int)n, sh);
-  else if (threadIdx.x >= 64) return;
-  else if (n > 64) sample_from_few<4>(p, b, set, weigh, bin_of, (int)n, sh);
+  if (n > LIST) return sample_by_radix<Tag>(p, b, row, set, weigh, sh);
+  if (n > 256) return sample_from_list(p, b, set, weigh, bin_of, (int)n, sh);
+  if (n > 64) rank_list((int)n, sh);
+  if (threadIdx.x >= 64) return;
+  if (n > 64) sample_from_few<4>(p, b, set, weigh, bin_of, (int)n, sh);
   else sample_from_few<1>(p, b, set, weigh, bin_of, (int)n, sh);
 }
 

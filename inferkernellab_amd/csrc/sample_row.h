@@ -702,11 +702,6 @@ __device__ inline double across(double v) {
   }
 }
 
-__device__ inline double across_lanes(double v, int d) {  // d known when unrolled
-  return d == 1 ? across<1>(v) : d == 2 ? across<2>(v) : d == 4 ? across<4>(v) : d == 8 ? across<8>(v)
-         : d == 16 ? across<16>(v) : across<32>(v);
-}
-
 // One step of the sorting network between lanes D apart: the lower lane of a
 // pair keeps the larger word where its run falls.
 template <int D>
@@ -719,34 +714,24 @@ __device__ inline void step_across(double (&w)[2], bool falls) {
   }
 }
 
-// The E words of each lane of a wave in falling order, word e of lane l at place
-// l E + e.
-template <int E>
-__device__ inline void sort_wave(double (&w)[E], int lane) {
-  const int at = lane * E;
-#pragma unroll
-  for (int run = 2; run <= 64 * E; run <<= 1) {
-#pragma unroll
-    for (int d = run >> 1; d; d >>= 1) {
-      if (d >= E) {
-        const bool larger = ((at & run) == 0) == ((at & d) == 0);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const double other = across_lanes(w[e], d / E);
-          w[e] = larger ? fmax(w[e], other) : fmin(w[e], other);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if ((e & d) == 0) {
-            const bool falls = ((at + e) & run) == 0;
-            const double hi = fmax(w[e], w[e | d]), lo = fmin(w[e], w[e | d]);
-            w[e] = falls ? hi : lo;
-            w[e | d] = falls ? lo : hi;
-          }
-      }
-    }
+// Puts the `n` words in sh.list in falling order, n <= 256: four threads count the
+// words above each. (By a bitonic network in one wave's registers 92 words took
+// 1.1 us more, 256 as long.)
+__device__ inline void rank_list(int n, RowShared &sh) {
+  constexpr int LANES = 4;
+  const int at = threadIdx.x / LANES;
+  double word = 0.0;
+  int rank = 0;
+  if (at < n) {
+    word = sh.list[at];
+#pragma unroll 4
+    for (int j = threadIdx.x % LANES; j < n; j += LANES) rank += sh.list[j] > word;
   }
+  rank += __builtin_amdgcn_mov_dpp(rank, DPP_QUAD_XOR1, 0xf, 0xf, false);
+  rank += __builtin_amdgcn_mov_dpp(rank, DPP_QUAD_XOR2, 0xf, 0xf, false);
+  __syncthreads();
+  if (at < n && threadIdx.x % LANES == 0) sh.list[rank] = word;
+  __syncthreads();
 }
 
 // Puts the `n` words in sh.list in falling order (n <= LIST; the words behind
@@ -803,10 +788,21 @@ __device__ inline void sort_list(int n, RowShared &sh) {
   __syncthreads();
 }
 
+// By the first wave: the token of a word and its log probabilities, each by a lane.
+__device__ inline void store_drawn(const SampleParams &p, int64_t b, const Weigher &weigh, double word, uint64_t total,
+                                   uint64_t kept) {
+  const int lane = threadIdx.x;
+  const float share = weigh.log_share(word_logit(word), lane == 0 ? total : kept);
+  if (lane == 0) {
+    p.tokens[b] = word_index(word);
+    if (p.policy) p.policy[b] = share;
+  }
+  if (lane == 1 && p.sampling) p.sampling[b] = share;
+}
+
 // The draw from up to 64 E tokens, by the first wave: what sample_from_list does,
 // E tokens a lane and without a barrier (3 tokens 4.7 -> 1.3 us). Up to 64 words
-// take their place by counting the larger ones, more by a bitonic network over
-// the registers of the wave.
+// take their place by counting the larger ones, more are in order already.
 template <int E>
 __device__ inline void sample_from_few(const SampleParams &p, int64_t b, const RowSettings &set, const Weigher &weigh,
                                        const Binner &bin_of, int n, RowShared &sh) {
@@ -821,8 +817,6 @@ __device__ inline void sample_from_few(const SampleParams &p, int64_t b, const R
     const int to = 4 * (lane < n ? rank : lane);
     word[0] = __hiloint2double(__builtin_amdgcn_ds_permute(to, __double2hiint(word[0])),
                                __builtin_amdgcn_ds_permute(to, __double2loint(word[0])));
-  } else {
-    sort_wave<E>(word, lane);
   }
   uint64_t w[E], before[E], sum = 0;
   int bin[E];
@@ -897,12 +891,7 @@ __device__ inline void sample_from_few(const SampleParams &p, int64_t b, const R
   }
   kept = min(kept, sh.likely);
   last_up_to(scaled_floor(set.uniform, kept), end, drawn);
-  const float share = weigh.log_share(word_logit(drawn), lane == 0 ? sh.total : kept);
-  if (lane == 0) {
-    p.tokens[b] = word_index(drawn);
-    if (p.policy) p.policy[b] = share;
-  }
-  if (lane == 1 && p.sampling) p.sampling[b] = share;
+  store_drawn(p, b, weigh, drawn, sh.total, kept);
 }
 
 // The draw from the `n` tokens in sh.list, all those of the cuts' bins, with
@@ -945,18 +934,16 @@ __device__ inline void sample_from_list(const SampleParams &p, int64_t b, const 
   const uint64_t most = scaled_floor(set.top_p, kept);
   if (set.top_p < 1.f && most < sh.binned) {
     for (int i = 0; i < PER; ++i)
-      if (bin[i] >= 0 && before[i] <= most)
-        atomicMax((unsigned long long *)&sh.found[1], (unsigned long long)(before[i] + w[i]));
+      if (bin[i] >= 0 && before[i] <= most && most - before[i] < w[i]) sh.found[1] = before[i] + w[i];  // one token
     __syncthreads();
     kept = min(kept, sh.found[1]);
   }
   kept = min(kept, sh.likely);
   const uint64_t aim = scaled_floor(set.uniform, kept);
   for (int i = 0; i < PER; ++i)
-    if (bin[i] >= 0 && before[i] <= aim && aim - before[i] < w[i]) {  // one token
-      const double word = sh.list[first + i];
-      store_token(p, b, weigh, word_index(word), word_logit(word), sh.total, kept);
-    }
+    if (bin[i] >= 0 && before[i] <= aim && aim - before[i] < w[i]) sh.found[2] = (uint64_t)(first + i);  // one token
+  __syncthreads();
+  if (threadIdx.x < 64) store_drawn(p, b, weigh, sh.list[sh.found[2]], sh.total, kept);
 }
 
 // The whole draw by radix selections, for rows whose cuts fall in bins of more
