@@ -611,14 +611,18 @@ __device__ inline void add_tokens(int index, const float (&x)[N], const RowSetti
 
 // The last bin whose `before` is at most `bound`: with less than the row's total
 // for a bound, the one that the cumulative count or mass exceeds it in. By the
-// 64 lanes of a wave, in two looks.
+// lanes of half a wave, in two looks; the halves have a bound each.
 template <typename T>
 __device__ inline int bin_at(const T *before, uint64_t bound) {
-  constexpr int STEP = BINS / 64;
-  static_assert(STEP <= 64, "two looks");
-  const int lane = threadIdx.x & 63;
-  const int part = __popcll(__ballot((uint64_t)before[lane * STEP] <= bound)) - 1;
-  return part * STEP + __popcll(__ballot(lane < STEP && (uint64_t)before[part * STEP + lane % STEP] <= bound)) - 1;
+  constexpr int STEP = BINS / 32;
+  static_assert(STEP == 64, "two looks");
+  const int lane = threadIdx.x & 31;
+  const auto lanes = [](bool in) {  // of this half
+    const uint64_t all = __ballot(in);
+    return __popc((threadIdx.x & 32) ? (uint32_t)(all >> 32) : (uint32_t)all);
+  };
+  const int part = (lanes((uint64_t)before[lane * STEP] <= bound) - 1) * STEP, at = part + 2 * lane;
+  return part + lanes((uint64_t)before[at] <= bound) + lanes((uint64_t)before[at + 1] <= bound) - 1;
 }
 
 // Turns the histogram in shared memory into the masses and counts before each
@@ -653,33 +657,29 @@ __device__ inline void find_cuts(const RowSettings &set, const Candidates &cand,
   const uint64_t total = cand.alone ? sh.others : binned, likely = cand.alone ? binned : total - sh.others;
   __syncthreads();
   if (threadIdx.x < 64) {
-    const auto end = [&](int bin) { return bin + 1 < BINS ? sh.mass[bin + 1] : binned; };
-    Cuts c;
-    const auto run = [&](int i, int first, int last) {
-      c.first[i] = (uint32_t)first;
-      c.span[i] = (uint32_t)(last - first);
+    // What is kept lies between two masses: one half of the wave goes by the lower
+    // one, the other by the upper. One loop for the cuts: code that runs once is
+    // paid for by fetching it.
+    uint64_t kept = total;
+    const auto run = [&](int i, int bin) {
+      const int first = __builtin_amdgcn_readlane(bin, 0);
+      const uint64_t past = bin + 1 < BINS ? sh.mass[bin + 1] : binned;
+      kept = min(kept, threadIdx.x >= 32 ? past : sh.mass[bin] + 1);
+      sh.cuts.first[i] = (uint32_t)first;
+      sh.cuts.span[i] = (uint32_t)(__builtin_amdgcn_readlane(bin, 32) - first);
     };
-    run(0, 2 * BINS, 2 * BINS);  // no bin
-    run(1, 2 * BINS, 2 * BINS);
-    uint64_t low = total, high = total;  // the kept mass lies between
-    if (set.top_k > 0 && (uint64_t)set.top_k < weighted) {
-      const int bin = bin_at(sh.count, (uint64_t)set.top_k - 1);
-      run(0, bin, bin);
-      low = sh.mass[bin] + 1;
-      high = end(bin);
+    if (threadIdx.x < 2) {  // no bin
+      sh.cuts.first[threadIdx.x] = 2 * BINS;
+      sh.cuts.span[threadIdx.x] = 0;
     }
-    if (set.top_p < 1.f && scaled_floor(set.top_p, low) < binned) {
-      const int first = bin_at(sh.mass, scaled_floor(set.top_p, low));
-      const int last = bin_at(sh.mass, scaled_floor(set.top_p, high));
-      run(1, first, last);
-      low = min(low, sh.mass[first] + 1);
-      high = min(high, end(last));
+    if (set.top_k > 0 && (uint64_t)set.top_k < weighted) run(0, bin_at(sh.count, (uint64_t)set.top_k - 1));
+#pragma unroll 1
+    for (int i = set.top_p < 1.f ? 1 : 2; i < 3; ++i) {
+      if (i == 2) kept = min(kept, likely);
+      const uint64_t bound = scaled_floor(i == 1 ? set.top_p : set.uniform, kept);
+      if (lane64(bound, 0) < binned) run(i, bin_at(sh.mass, bound));
     }
-    low = min(low, likely);
-    high = min(high, likely);
-    run(2, bin_at(sh.mass, scaled_floor(set.uniform, low)), bin_at(sh.mass, scaled_floor(set.uniform, high)));
     if (threadIdx.x == 0) {
-      sh.cuts = c;
       sh.total = total;
       sh.likely = likely;
       sh.binned = binned;
