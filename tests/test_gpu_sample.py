@@ -200,6 +200,23 @@ def test_flat_and_steep_long_rows(spread, dtype):
         check(logits, uniform, **settings)
 
 
+@pytest.mark.parametrize("vocab", [20011, 40009])
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 255, 256, 257, 511, 513, 1025, 2047, 2048, 2049])
+def test_tokens_crowded_in_one_step_of_the_histogram(n, vocab):
+    """n distinct logits within 1/5000 of the row's range, so that every cut falls among all of them."""
+    gen = torch.Generator().manual_seed(n + vocab)
+    x = torch.full((4, vocab), float("-inf"))
+    for row in x:
+        at = torch.randperm(vocab, generator=gen)[:n + 3]
+        row[at[:n]] = 5 + 2e-6 * torch.arange(n)
+        row[at[n:]] = -15.0
+    uniform = torch.rand(4, generator=gen).cuda()
+    for settings in (dict(), dict(top_p=0.37), dict(top_k=n // 2 + 1), dict(top_k=n // 2 + 1, top_p=0.61),
+                     dict(top_p=0.8, min_p=0.5), dict(top_k=n // 3 + 1, top_p=0.9, min_p=0.9995)):
+        print(n, vocab, settings, flush=True)
+        check(x.cuda(), uniform, **settings)
+
+
 def test_long_rows_with_settings_per_row_and_strides():
     rows = 20
     base, uniform = inputs(rows, 60100, "fp16", 19)
