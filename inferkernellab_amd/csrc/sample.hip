@@ -22,20 +22,35 @@
 namespace ikl {
 namespace {
 
-// Leaves the tokens of the cuts' bins in a list of `n` and returns their number.
-__device__ inline uint32_t drop_uncut(const Binner &bin_of, uint32_t n, RowShared &sh) {
-  constexpr int PER = LIST / SAMPLE_THREADS;
+// Leaves the tokens of the cuts' bins among the `n` candidates in sh.list, as far as
+// it holds them, and returns their number.
+__device__ inline uint32_t drop_uncut(const Binner &bin_of, uint32_t n, WholeRowShared &sh) {
+  constexpr int PER = CANDIDATES / SAMPLE_THREADS, FEW = LIST / SAMPLE_THREADS;
   const Cuts cuts = sh.cuts;
   double word[PER];
+  const auto fetch = [&](int i) {
+    const int at = threadIdx.x + i * SAMPLE_THREADS;
+    word[i] = i < FEW ? sh.list[at] : sh.more[at - LIST];
+  };
+  const auto keep = [&](int i) {
+    if (threadIdx.x + i * SAMPLE_THREADS < n && cuts.has(bin_of(word_logit(word[i])))) {
+      const uint32_t at = atomicAdd(&sh.listed, 1u);
+      if (at < LIST) sh.list[at] = word[i];
+    }
+  };
 #pragma unroll
-  for (int i = 0; i < PER; ++i) word[i] = sh.list[threadIdx.x + i * SAMPLE_THREADS];
+  for (int i = 0; i < FEW; ++i) fetch(i);
   __syncthreads();
   if (threadIdx.x == 0) sh.listed = 0;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < PER; ++i)
-    if (threadIdx.x + i * SAMPLE_THREADS < n && cuts.has(bin_of(word_logit(word[i]))))
-      sh.list[atomicAdd(&sh.listed, 1u)] = word[i];
+  for (int i = 0; i < FEW; ++i) keep(i);
+  if (n > LIST) {
+#pragma unroll
+    for (int i = FEW; i < PER; ++i) fetch(i);
+#pragma unroll
+    for (int i = FEW; i < PER; ++i) keep(i);
+  }
   __syncthreads();
   return sh.listed;
 }
@@ -88,7 +103,7 @@ __device__ inline void list_tokens(const RowReader<Tag> &row, int from, int to, 
 // them all.
 template <typename Tag>
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_row_kernel(const SampleParams p) {
-  __shared__ RowShared sh;
+  __shared__ WholeRowShared sh;
   const int64_t b = blockIdx.x;
   const RowReader<Tag> row(p.logits + b * p.stride, p.vocab);
   const RowSettings set = row_settings(p, b);
@@ -111,22 +126,23 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_row_kernel(const Sample
   const Binner bin_of(set, weigh, cand, top, least);
   uint64_t others = 0;
   row.each(0, row.vectors, [&](int first, const float(&x)[RowReader<Tag>::VEC]) {
-    add_tokens<true>(first, x, set, weigh, cand, bin_of, others, sh);
+    add_tokens(first, x, set, weigh, cand, bin_of, others, sh);
   });
   if (set.min_p > 0.f) others = block_sum(others, sh);
   if (threadIdx.x == 0) sh.others = others;
   __syncthreads();
   find_cuts(set, cand, sh);
   uint32_t n = sh.listed;
-  if (!cand.alone || n > LIST) {
+  if (!cand.alone || n > CANDIDATES) {
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     list_tokens(row, 0, row.vectors, weigh, cand, bin_of, row.begin(0, row.vectors), sh);
     __syncthreads();
     n = sh.listed;
+  } else if (n > 64) {
+    n = drop_uncut(bin_of, n, sh);
   }
-  if (cand.alone && n > 64 && n <= LIST) n = drop_uncut(bin_of, n, sh);
   draw(p, b, row, set, weigh, bin_of, n, sh);
 }
 
@@ -230,7 +246,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_histogram_kernel(const 
   uint64_t others = 0;
   __syncthreads();
   at.row.each(at.from, at.to, begin, [&](int first, const float(&x)[RowReader<Tag>::VEC]) {
-    add_tokens<false>(first, x, set, weigh, cand, bin_of, others, sh);
+    add_tokens(first, x, set, weigh, cand, bin_of, others, sh);
   });
   if (set.min_p > 0.f) {
     others = block_sum(others, sh);

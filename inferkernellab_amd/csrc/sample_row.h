@@ -289,6 +289,16 @@ struct RowShared {
   uint32_t weighted, listed;       // tokens in the histogram (where top-k asks), in the list
 };
 
+// Where one workgroup has the whole row, its second pass lists up to this many
+// candidates, the first LIST of them in sh.list. A row with more of them needs the
+// third pass, and the slowest row counts (256 x 131072 fp32, one row of some above
+// 2048: 65.5 -> 63.0 us, without such a row 0.2 more). A compute unit has the
+// registers for one workgroup, so its 89 KB of LDS keep none out.
+constexpr int CANDIDATES = 4 * LIST;
+struct WholeRowShared : RowShared {
+  double more[CANDIDATES - LIST];
+};
+
 // Lane permutations inside rows of 16 lanes without the LDS round trip.
 template <int CTRL>
 __device__ inline uint64_t dpp64(uint64_t v) {  // lanes without a source get 0
@@ -562,25 +572,29 @@ struct Binner {
   }
 };
 
-// Adds a token to the histogram. LISTED: one that is alone there to sh.list as well.
-template <bool LISTED>
+// Adds a token to the histogram and, where a workgroup has the whole row, a
+// candidate to the list as well.
+template <bool LISTED, typename Shared>
 __device__ inline void add_token(int index, float x, uint64_t w, const RowSettings &set, const Binner &bin_of,
-                                 RowShared &sh) {
+                                 Shared &sh) {
   const int bin = bin_of(x);
   atomicAdd((unsigned long long *)&sh.mass[bin], (unsigned long long)w);
   if (set.top_k > 0) atomicAdd(&sh.count[bin], 1u);
-  if (LISTED) {
+  if constexpr (LISTED) {
     const uint32_t at = atomicAdd(&sh.listed, 1u);
-    if (at < LIST) sh.list[at] = token_word(order_key(clean(x)), index);
+    const double word = token_word(order_key(clean(x)), index);
+    if (at < LIST) sh.list[at] = word;
+    else if (at < CANDIDATES) sh.more[at - LIST] = word;
   }
 }
 
 // Adds tokens to the histogram, and to `others` what min-p asks for: the mass of
 // all tokens where candidates are alone in the histogram (there most waves have
 // none and are done with a sum), else that of the tokens that are none.
-template <bool LISTED, int N>
+template <int N, typename Shared>
 __device__ inline void add_tokens(int index, const float (&x)[N], const RowSettings &set, const Weigher &weigh,
-                                  const Candidates &cand, const Binner &bin_of, uint64_t &others, RowShared &sh) {
+                                  const Candidates &cand, const Binner &bin_of, uint64_t &others, Shared &sh) {
+  constexpr bool LISTED = std::is_same<Shared, WholeRowShared>::value;
   double exact[N];
   weigh.of(x, exact);
   uint64_t w[N];

@@ -217,6 +217,18 @@ def test_tokens_crowded_in_one_step_of_the_histogram(n, vocab):
         check(x.cuda(), uniform, **settings)
 
 
+@pytest.mark.parametrize("min_p", [0.02, 0.005, 0.002, 1e-3, 1e-4, 1e-8, 1e-20])
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+def test_min_p_of_many_candidates(min_p, dtype):
+    """Some hundred to all of 20011 tokens are candidates."""
+    gen = torch.Generator().manual_seed(25)
+    logits = (torch.randn(5, 20011, generator=gen) * 2).to(DTYPES[dtype]).cuda()
+    uniform = torch.rand(5, generator=gen).cuda()
+    for settings in (dict(), dict(top_p=0.9), dict(top_k=700)):
+        print(min_p, dtype, settings, flush=True)
+        check(logits, uniform, min_p=min_p, **settings)
+
+
 def test_long_rows_with_settings_per_row_and_strides():
     rows = 20
     base, uniform = inputs(rows, 60100, "fp16", 19)
