@@ -81,6 +81,17 @@ def test_tokens_and_logprobs(vocab, dtype, settings):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [4093, 4095, 4096, 4097, 8185, 8190, 8192, 8193, 8199, 12287, 16385, 24583, 32769,
+                                   40961])
+def test_rows_that_end_near_a_round_of_the_threads(vocab, dtype):
+    """Rows of odd lengths one behind the other start at every alignment."""
+    logits, uniform = inputs(9, vocab, dtype, vocab)
+    check(logits, uniform)
+    check(logits, uniform, top_k=40, top_p=0.9)
+    check(logits, uniform, min_p=0.01)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("rows,vocab", [(1, 131072), (5, 131072), (300, 4001), (2, 400003)])
 def test_large_rows(rows, vocab, dtype):
     logits, uniform = inputs(rows, vocab, dtype, rows)
