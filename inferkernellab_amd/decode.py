@@ -77,7 +77,8 @@ class DecodeMetadata:
                 self._copied[r.request_id] = n
 
     def refresh(self, requests: Sequence[InferenceRequest]) -> None:
-        """Copy whole tables again, after their pages were renumbered."""
+        """Copy whole tables again, after their pages were renumbered: the
+        ``compact_fn`` of a runtime."""
         for r in requests:
             self._copied[r.request_id] = 0
         self.sync_tables(requests)
@@ -271,6 +272,7 @@ class SyntheticDecodeRunner:
             prefill_fn=None if batched else self._prefill,
             prefill_batch_fn=self._prefill_batch if batched else None,
             decode_fn=self._decode,
+            compact_fn=lambda requests: self.metadata.refresh(requests),
         )
         self.requests = [self.runtime.submit(i, len(p), max_new_tokens) for i, p in enumerate(self.prompts)]
         self._spacers = interleaved_tables(self.cache, self.requests, self.prompt_lengths)

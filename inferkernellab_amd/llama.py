@@ -348,6 +348,7 @@ class LlamaPagedDecodeRunner:
             prefill_fn=None if batched else self._prefill,
             prefill_batch_fn=self._prefill_batch if batched else None,
             decode_fn=self._decode,
+            compact_fn=lambda requests: self.metadata.refresh(requests),
         )
         self.requests = [self.runtime.submit(i * num_samples, len(p), max_new_tokens)
                          for i, p in enumerate(self.prompts)]

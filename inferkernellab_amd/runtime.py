@@ -11,7 +11,8 @@ them. What callers observe, and the reference's tests pin
   calls ``prefill_batch_fn(requests, starts, ends)`` once with the requests
   whose range is non-empty (or ``prefill_fn`` per request);
 * ``fork`` continues a running request a second time on shared pages, and
-  ``compact`` moves the pages in use together;
+  ``compact`` moves the pages in use together and calls ``compact_fn`` with
+  every request that holds pages, for device copies of their tables;
 * a decode step first reserves room for the token each request writes, then
   calls ``decode_fn(requests)`` — before the scheduler counts that token —
   and finally returns the blocks of finished requests to the allocator.
@@ -31,6 +32,7 @@ from .scheduler import InferenceRequest, ScheduleBatch, TokenBudgetScheduler
 PrefillFn = Callable[[InferenceRequest, int, int], None]
 PrefillBatchFn = Callable[[tuple[InferenceRequest, ...], tuple[int, ...], tuple[int, ...]], None]
 DecodeFn = Callable[[tuple[InferenceRequest, ...]], None]
+CompactFn = Callable[[tuple[InferenceRequest, ...]], None]
 
 
 @dataclass(frozen=True)
@@ -47,6 +49,7 @@ class _Hooks:
     prefill: PrefillFn | None
     prefill_batch: PrefillBatchFn | None
     decode: DecodeFn | None
+    compact: CompactFn | None = None
 
     def __post_init__(self):
         if self.prefill is not None and self.prefill_batch is not None:
@@ -65,8 +68,9 @@ class InferenceRuntime:
         prefill_fn: PrefillFn | None = None,
         prefill_batch_fn: PrefillBatchFn | None = None,
         decode_fn: DecodeFn | None = None,
+        compact_fn: CompactFn | None = None,
     ):
-        self._hooks = _Hooks(prefill_fn, prefill_batch_fn, decode_fn)
+        self._hooks = _Hooks(prefill_fn, prefill_batch_fn, decode_fn, compact_fn)
         self.cache = cache
         self.scheduler = scheduler
         self._by_id: dict[int, InferenceRequest] = {}
@@ -83,6 +87,10 @@ class InferenceRuntime:
     @property
     def decode_fn(self) -> DecodeFn | None:
         return self._hooks.decode
+
+    @property
+    def compact_fn(self) -> CompactFn | None:
+        return self._hooks.compact
 
     def submit(self, request_id: int, prompt_tokens: int, max_new_tokens: int) -> InferenceRequest:
         if request_id in self._by_id:
@@ -116,8 +124,14 @@ class InferenceRuntime:
 
     def compact(self) -> dict[int, int]:
         """Move the cache's pages in use to the lowest ids and renumber every
-        request's table; {old id: new id} for device copies of the tables."""
-        return self.cache.compact([r.block_table for r in self._by_id.values()])
+        request's table. Device copies of the tables are out of date then, those
+        of a prompt between two chunks too: ``compact_fn`` is called with every
+        request that holds pages. Returns {old id: new id} for other places that
+        name pages."""
+        moves = self.cache.compact([r.block_table for r in self._by_id.values()])
+        if moves and self._hooks.compact is not None:
+            self._hooks.compact(tuple(r for r in self._by_id.values() if r.block_table))
+        return moves
 
     def _reserve(self, request: InferenceRequest, tokens: int) -> None:
         """Tops the request's table up to the blocks `tokens` positions need."""
