@@ -30,6 +30,7 @@ struct CopyParams {
   CopyTensor tensor[IKL_COPY_MAX_TENSORS];
   int64_t first[IKL_COPY_MAX_TENSORS + 1];  // first workgroup of each tensor's share, of one pair and layer
   int64_t num_blocks;
+  int64_t first_pair;  // of this launch
   int32_t num_layers;
   int32_t num_tensors;
 };
@@ -59,7 +60,8 @@ __global__ __launch_bounds__(COPY_THREADS) void copy_blocks_kernel(const CopyPar
   // workgroup = (pair, layer, part of the page's tensors)
   const int64_t parts = p.first[p.num_tensors];
   const int64_t page = blockIdx.x / parts, part = blockIdx.x - page * parts;
-  const int64_t pair = page / p.num_layers, layer = page - pair * p.num_layers;
+  const int64_t in_launch = page / p.num_layers, layer = page - in_launch * p.num_layers;
+  const int64_t pair = p.first_pair + in_launch;
   int n = 0;
   while (n + 1 < p.num_tensors && part >= p.first[n + 1]) ++n;
   const int64_t from = pairs.from(pair), to = pairs.to(pair);
@@ -78,14 +80,20 @@ __global__ __launch_bounds__(COPY_THREADS) void copy_blocks_kernel(const CopyPar
     if (first + i * COPY_THREADS < t.units) store_out(dst + first + i * COPY_THREADS, u[i]);
 }
 
+// In as few launches as hold the workgroups.
 template <typename Unit, typename Pairs>
-int launch(const CopyParams &p, const Pairs &pairs, int64_t count, hipStream_t s) {
-  int64_t grid;
-  if (__builtin_mul_overflow(count, (int64_t)p.num_layers, &grid) ||
-      __builtin_mul_overflow(grid, p.first[p.num_tensors], &grid) || grid > 0x7fffffffLL)
-    return fail(IKL_EINVAL, "copy blocks: too many pages for one launch");
-  copy_blocks_kernel<Unit, Pairs><<<dim3((unsigned)grid), COPY_THREADS, 0, s>>>(p, pairs);
-  return check_launch("copy blocks launch");
+int launch(CopyParams p, const Pairs &pairs, int64_t count, hipStream_t s) {
+  int64_t each, all;  // workgroups of a pair, of all pairs
+  if (__builtin_mul_overflow((int64_t)p.num_layers, p.first[p.num_tensors], &each) || each > max_grid(COPY_THREADS) ||
+      __builtin_mul_overflow(each, count, &all) || all > 0x7fffffffLL)
+    return fail(IKL_EINVAL, "copy blocks: too many pages for one call");
+  const int64_t most = max_grid(COPY_THREADS) / each;
+  for (p.first_pair = 0; p.first_pair < count; p.first_pair += most) {
+    const int64_t n = count - p.first_pair < most ? count - p.first_pair : most;
+    copy_blocks_kernel<Unit, Pairs><<<dim3((unsigned)(n * each)), COPY_THREADS, 0, s>>>(p, pairs);
+    if (const int bad = check_launch("copy blocks launch"); bad != IKL_OK) return bad;
+  }
+  return IKL_OK;
 }
 
 // Pieces of 16, 4 or 1 bytes: the largest that addresses, strides and sizes of

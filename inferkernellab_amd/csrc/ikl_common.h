@@ -18,6 +18,9 @@ void set_error(const std::string &msg);
 int fail(int code, const std::string &msg);
 int check_launch(const char *what);
 
+// Workgroups of a launch, at most: HIP takes grids of fewer than 2^32 threads.
+constexpr int64_t max_grid(int threads) { return 0xffffffffLL / threads; }
+
 // ---------------------------------------------------------- element types
 struct f16_tag {};
 struct bf16_tag {};

@@ -801,7 +801,8 @@ def _copy_args(cache, src: int, dst: int, count: int, index_type: int, on_host: 
 
 def copy_blocks_hip(cache, src, dst, *, validate_inputs: bool = True) -> None:
     """Copy the pages ``src[i]`` of the cache to ``dst[i]``, all layers of K and
-    V (and an FP8 cache's scales), in one launch on the current stream.
+    V (and an FP8 cache's scales), on the current stream: in one launch, or in
+    several for lists of more than 384 pairs and for more pages than one holds.
 
     ``src`` / ``dst``: lists of block ids on the host, or int32 / int64 GPU
     tensors. Ids outside the cache, a page written twice and one that is both

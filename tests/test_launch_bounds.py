@@ -1,0 +1,39 @@
+"""The largest launch: HIP takes fewer than 2^32 threads of a grid. What does
+not fit is refused on the host, before anything is launched."""
+
+import ctypes
+
+import pytest
+import torch
+
+from inferkernellab_amd import _lib
+from tests.test_new_operator_refusals import _copy
+
+
+@pytest.mark.parametrize("layers,page,status", [((1 << 24) // 2, 4096, _lib.IKL_EINVAL),
+                                                ((1 << 24) // 4, 2 * 16 * 1024, _lib.IKL_EINVAL)])
+def test_copy_refuses_one_page_that_no_launch_holds(layers, page, status):
+    """2 tensors of 2^23 layers, a workgroup each, and of 2^22 layers, two each: 2^24 workgroups of 256."""
+    a, keep = _copy([0], [1], num_layers=layers)
+    for n in range(2):
+        a.page_bytes[n] = page
+    assert _lib.load().ikl_copy_blocks(ctypes.byref(a), None) == status
+    assert "too many pages" in _lib.last_error()
+
+
+@pytest.mark.gpu
+def test_copies_of_more_pages_than_one_launch_holds():
+    """4.3 million pairs of 2 layers, 17 million workgroups: in two launches."""
+    from inferkernellab_amd import PagedKVCache, copy_blocks_hip
+
+    pairs = (1 << 22) + 100001
+    cache = PagedKVCache(2 * pairs, 1, 1, 8, num_layers=2, dtype=torch.bfloat16, device="cuda")
+    for t in (cache.k, cache.v):
+        t.view(torch.int16).copy_(torch.randint(-30000, 30000, t.shape, dtype=torch.int16, device="cuda"))
+    order = torch.randperm(2 * pairs, device="cuda")
+    src, dst = order[:pairs].to(torch.int32), order[pairs:].to(torch.int32)
+    want = [t.view(torch.int16)[:, order[:pairs]] for t in (cache.k, cache.v)]
+    copy_blocks_hip(cache, src, dst, validate_inputs=False)
+    for t, w in zip((cache.k, cache.v), want):
+        assert torch.equal(t.view(torch.int16)[:, order[pairs:]], w)
+        assert torch.equal(t.view(torch.int16)[:, order[:pairs]], w)
