@@ -276,7 +276,7 @@ int ikl_copy_blocks(const ikl_copy_blocks_args *args, void *stream);
 typedef struct ikl_sample_args {
   const void *logits;        /* [rows, vocab], contiguous rows */
   int64_t logits_stride;
-  int64_t rows;
+  int64_t rows;              /* below 2^22, what a launch holds */
   int64_t vocab;             /* 1 .. IKL_SAMPLE_MAX_VOCAB */
   int32_t dtype;             /* enum ikl_dtype: F16, BF16, F32 */
   int32_t top_k_type;        /* enum ikl_index_type of top_k_rows */

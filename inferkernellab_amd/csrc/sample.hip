@@ -357,7 +357,7 @@ extern "C" int ikl_sample_tokens(const ikl_sample_args *a, void *stream) {
     default: return fail(IKL_EINVAL, "sample: unsupported dtype");
   }
   if (a->rows == 0) return IKL_OK;
-  if (a->rows > 0x7fffffffLL) return fail(IKL_EINVAL, "sample: too many rows for one launch");
+  if (a->rows > max_grid(SAMPLE_THREADS)) return fail(IKL_EINVAL, "sample: too many rows for one launch");
   if (!a->logits || !a->uniform || !a->tokens) return fail(IKL_EINVAL, "sample: null tensor pointer");
   if (a->top_k_rows && a->top_k_type != IKL_I32 && a->top_k_type != IKL_I64)
     return fail(IKL_EINVAL, "sample: top_k must use int32 or int64");

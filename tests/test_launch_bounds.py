@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from inferkernellab_amd import _lib
-from tests.test_new_operator_refusals import _copy
+from tests.test_new_operator_refusals import _copy, _sample
 
 
 @pytest.mark.parametrize("layers,page,status", [((1 << 24) // 2, 4096, _lib.IKL_EINVAL),
@@ -19,6 +19,25 @@ def test_copy_refuses_one_page_that_no_launch_holds(layers, page, status):
         a.page_bytes[n] = page
     assert _lib.load().ikl_copy_blocks(ctypes.byref(a), None) == status
     assert "too many pages" in _lib.last_error()
+
+
+@pytest.mark.parametrize("rows", [1 << 22, 1 << 30])
+def test_sample_refuses_rows_that_no_launch_holds(rows):
+    """A workgroup of 1024 a row."""
+    assert _lib.load().ikl_sample_tokens(ctypes.byref(_sample(rows=rows)), None) == _lib.IKL_EINVAL
+    assert "too many rows" in _lib.last_error()
+
+
+@pytest.mark.gpu
+def test_sample_of_the_most_rows_a_launch_holds():
+    from inferkernellab_amd import sample_tokens_hip
+
+    rows = (1 << 22) - 1
+    logits = torch.randint(0, 2, (rows, 2), device="cuda").to(torch.bfloat16)
+    tokens = sample_tokens_hip(logits, torch.full((rows,), 0.999999, device="cuda"), temperature=0.0)
+    assert torch.equal(tokens, (logits[:, 1] > logits[:, 0]).long())
+    with pytest.raises(ValueError, match="too many rows"):
+        sample_tokens_hip(logits[:1].expand(rows + 1, -1), torch.zeros(rows + 1, device="cuda"))
 
 
 @pytest.mark.gpu
