@@ -163,7 +163,7 @@ template <typename Tag, int LPR, bool FP8>
 int launch(const NormRopeParams &f, bool i64, hipStream_t s) {
   const int64_t rows = f.tokens * (f.r.num_heads + 2 * (int64_t)f.r.num_kv_heads), per = 256 / LPR;
   const int64_t grid = (rows + per - 1) / per;
-  if (rows > 0xffff0000LL) return fail(IKL_EINVAL, "norm rope append: too many rows for one launch");
+  if (grid > max_grid(256)) return fail(IKL_EINVAL, "norm rope append: too many rows for one launch");
   if (i64) norm_rope_kernel<Tag, int64_t, LPR, FP8><<<dim3((unsigned)grid), 256, 0, s>>>(f);
   else norm_rope_kernel<Tag, int32_t, LPR, FP8><<<dim3((unsigned)grid), 256, 0, s>>>(f);
   return check_launch("norm rope append launch");

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from inferkernellab_amd import _lib
-from tests.test_new_operator_refusals import _copy, _sample
+from tests.test_new_operator_refusals import _copy, _norm_rope, _sample
 
 
 @pytest.mark.parametrize("layers,page,status", [((1 << 24) // 2, 4096, _lib.IKL_EINVAL),
@@ -25,6 +25,14 @@ def test_copy_refuses_one_page_that_no_launch_holds(layers, page, status):
 def test_sample_refuses_rows_that_no_launch_holds(rows):
     """A workgroup of 1024 a row."""
     assert _lib.load().ikl_sample_tokens(ctypes.byref(_sample(rows=rows)), None) == _lib.IKL_EINVAL
+    assert "too many rows" in _lib.last_error()
+
+
+@pytest.mark.parametrize("head_dim,tokens", [(64, 1 << 27), (128, 1 << 26), (512, 1 << 24), (1024, (1 << 31) - 1)])
+def test_norm_rope_refuses_rows_that_no_launch_holds(head_dim, tokens):
+    """8 rows a token in workgroups of 64, 32 or 8 rows (bf16 heads of 64, 128, 512): 2^24 workgroups of 256."""
+    args = _norm_rope(num_tokens=tokens, head_dim=head_dim)
+    assert _lib.load().ikl_qk_norm_rope_append_kv(ctypes.byref(args), None) == _lib.IKL_EINVAL
     assert "too many rows" in _lib.last_error()
 
 
