@@ -678,7 +678,7 @@ def _fill_rope_args(a, query, query_out, key, value, cos, sin, cache, slots, lay
 
 def _head_weight(weight, name: str, heads: int, like: torch.Tensor, head_dim: int) -> torch.Tensor:
     """A head norm's weight, [D] for all heads or [heads, D], in rows the kernel can read."""
-    if tuple(weight.shape) not in ((head_dim,), (heads, head_dim)):
+    if weight is None or tuple(weight.shape) not in ((head_dim,), (heads, head_dim)):
         raise ValueError(f"{name} must have shape [head_dim] or [heads, head_dim]")
     if weight.dtype != like.dtype or weight.device != like.device:
         raise ValueError(f"{name} must have the dtype and device of the rows it scales")

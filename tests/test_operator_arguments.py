@@ -1,0 +1,24 @@
+"""Arguments of the normalised append, the page copies, the compaction and the
+sampling that were taken wrongly or refused with another error."""
+
+import pytest
+import torch
+
+from inferkernellab_amd import PagedKVCache, ops
+
+
+def operands(tokens=3, heads=4, kv=2, d=32, device="cpu"):
+    def rows(*shape):
+        return torch.ones(*shape, device=device)
+
+    cache = PagedKVCache(4, 4, kv, d, dtype=torch.float32, device=device)
+    return [rows(tokens, heads, d), rows(tokens, kv, d), rows(tokens, kv, d), rows(d), rows(d), rows(tokens, d),
+            rows(tokens, d), cache, torch.arange(tokens, dtype=torch.int32, device=device)]
+
+
+@pytest.mark.parametrize("missing", [3, 4], ids=["q_weight", "k_weight"])
+def test_a_missing_norm_weight_is_a_value_error(missing):
+    args = operands()
+    args[missing] = None
+    with pytest.raises(ValueError, match="weight must have shape"):
+        ops._qk_norm_rope_args(*args, 0, 1e-6, None)
