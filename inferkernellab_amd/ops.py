@@ -830,15 +830,21 @@ def copy_blocks_hip(cache, src, dst, *, validate_inputs: bool = True) -> None:
         src, dst = src.contiguous(), dst.contiguous()
         args = _copy_args(cache, src.data_ptr(), dst.data_ptr(), src.numel(), _INDEX_TYPES[src.dtype], False)
     else:
-        if len(src) != len(dst):
-            raise ValueError("src and dst must have one entry per copied block")
-        src, dst = array.array("q", src), array.array("q", dst)
+        src, dst = _host_pairs(src, dst)
         args = _copy_args(cache, src.buffer_info()[0], dst.buffer_info()[0], len(src), _lib.IKL_I64, True)
     if args.num_pairs == 0:
         return
     with _on_device(cache.device):
         status = lib.ikl_copy_blocks(ctypes.byref(args), _stream(cache.device))
     _lib.check(status, "copy_blocks")
+
+
+def _host_pairs(src, dst) -> tuple[array.array, array.array]:
+    """Block ids on the host as 64-bit numbers."""
+    if len(src) != len(dst):
+        raise ValueError("src and dst must have one entry per copied block")
+    # entry by entry: an array takes bytes for its memory
+    return tuple(array.array("q", x if type(x) is list else list(x)) for x in (src, dst))
 
 
 def _check_pairs(src: list[int], dst: list[int], num_blocks: int) -> None:

@@ -22,3 +22,11 @@ def test_a_missing_norm_weight_is_a_value_error(missing):
     args[missing] = None
     with pytest.raises(ValueError, match="weight must have shape"):
         ops._qk_norm_rope_args(*args, 0, 1e-6, None)
+
+
+@pytest.mark.parametrize("src,dst", [(bytes(8), [1] * 8), ([0] * 8, bytes(range(8))),
+                                     (bytearray(range(8)), bytearray(range(8, 16))), (range(8), tuple(range(8, 16)))])
+def test_block_ids_of_any_sequence_are_its_entries(src, dst):
+    """Bytes are sequences of whole numbers too, not the memory of 64-bit ones."""
+    for pairs, given in zip(ops._host_pairs(src, dst), (src, dst)):
+        assert pairs.typecode == "q" and pairs.tolist() == list(given)
