@@ -843,8 +843,10 @@ def _host_pairs(src, dst) -> tuple[array.array, array.array]:
     """Block ids on the host as 64-bit numbers."""
     if len(src) != len(dst):
         raise ValueError("src and dst must have one entry per copied block")
-    # entry by entry: an array takes bytes for its memory
-    return tuple(array.array("q", x if type(x) is list else list(x)) for x in (src, dst))
+    try:  # entry by entry: an array takes bytes for its memory
+        return tuple(array.array("q", x if type(x) is list else list(x)) for x in (src, dst))
+    except OverflowError:
+        raise ValueError("copy blocks: invalid block id") from None
 
 
 def _check_pairs(src: list[int], dst: list[int], num_blocks: int) -> None:

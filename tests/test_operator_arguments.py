@@ -30,3 +30,14 @@ def test_block_ids_of_any_sequence_are_its_entries(src, dst):
     """Bytes are sequences of whole numbers too, not the memory of 64-bit ones."""
     for pairs, given in zip(ops._host_pairs(src, dst), (src, dst)):
         assert pairs.typecode == "q" and pairs.tolist() == list(given)
+
+
+def test_block_ids_that_no_cache_has():
+    for src, dst in (([1 << 70], [1]), ([1], [-(1 << 70)])):
+        with pytest.raises(ValueError, match="invalid block id"):
+            ops._host_pairs(src, dst)
+    with pytest.raises(ValueError, match="one entry per copied block"):
+        ops._host_pairs([1, 2], [3])
+    for bad in ([1.5], ["1"], [None]):
+        with pytest.raises(TypeError):
+            ops._host_pairs(bad, [1])
