@@ -278,11 +278,14 @@ class PagedKVCache:
         in place; a list given twice is changed once). Returns {old id: new id}
         of the moved pages, for every other place that names them, such as
         device copies of the tables."""
+        tables = {id(t): t for t in block_tables}.values()
+        if not all(isinstance(t, list) for t in tables):
+            raise ValueError("block tables must be lists: they are changed in place")
         moves = self.allocator.compaction()
         if moves:
             self.copy_blocks(list(moves), list(moves.values()))
             self.allocator.renumber(moves)
-            for table in {id(t): t for t in block_tables}.values():
+            for table in tables:
                 table[:] = [moves.get(b, b) for b in table]
         return moves
 

@@ -41,3 +41,19 @@ def test_block_ids_that_no_cache_has():
     for bad in ([1.5], ["1"], [None]):
         with pytest.raises(TypeError):
             ops._host_pairs(bad, [1])
+
+
+def test_a_compaction_refuses_tables_it_cannot_change_in_place():
+    """Before a page moves: after it, the tables that were not renumbered would name other requests' pages."""
+    cache = PagedKVCache(8, 4, 2, 8)
+    gone, first, second = cache.allocate_request(0, 8), cache.allocate_request(1, 8), cache.allocate_request(2, 8)
+    cache.release_request(gone, 0)
+    cache.k.copy_(torch.randn(cache.k.shape))
+    before = cache.k.clone()
+    for bad in (tuple(second), torch.tensor(second), range(4, 6)):
+        with pytest.raises(ValueError, match="lists"):
+            cache.compact([first, bad])
+        assert (first, second) == ([2, 3], [4, 5]) and torch.equal(cache.k, before)
+        assert cache.allocator.holders(2) == (1,) and cache.allocator.holders(4) == (2,)
+    assert cache.compact(t for t in (first, second)) == {4: 0, 5: 1}
+    assert (first, second) == ([2, 3], [0, 1])
