@@ -54,6 +54,8 @@ def _sample_args(logits, uniform, temperature, top_k, top_p, min_p):
     a = _lib.SampleArgs()
     a.temperature, heat = _setting(temperature, "temperature", rows, device,
                                    lambda v: math.isfinite(v) and v >= 0, "finite and non-negative")
+    if a.temperature == 0.0 and heat is None and temperature > 0:
+        a.temperature = 2.0 ** -149  # the smallest float32: 0 would state log probabilities at 1
     number, first = _setting(top_k, "top_k", rows, device,
                              lambda v: (isinstance(v, int) or float(v).is_integer()) and v >= 0,
                              "a non-negative whole number")

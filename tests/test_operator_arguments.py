@@ -57,3 +57,22 @@ def test_a_compaction_refuses_tables_it_cannot_change_in_place():
         assert cache.allocator.holders(2) == (1,) and cache.allocator.holders(4) == (2,)
     assert cache.compact(t for t in (first, second)) == {4: 0, 5: 1}
     assert (first, second) == ([2, 3], [0, 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature", [1e-44, 1e-46, 1e-300])
+def test_a_temperature_below_float32_is_not_zero(temperature):
+    """Its log probabilities are at that temperature (all mass on the likeliest tokens), not at 1."""
+    from inferkernellab_amd import sample_tokens_hip
+
+    logits = torch.randn(5, 1000, generator=torch.Generator().manual_seed(0))
+    logits[3, [7, 70]] = 9.0
+    for dtype in (torch.float32, torch.bfloat16):
+        x = logits.to(dtype).cuda()
+        x[[0, 1, 2, 4], [1, 2, 3, 4]] = 8.0
+        uniform = torch.tensor([0.2, 0.5, 0.9, 0.75, 0.0]).cuda()
+        for settings in (dict(), dict(min_p=0.5), dict(top_k=30, top_p=0.9)):
+            tokens, policy, sampling = sample_tokens_hip(x, uniform, temperature=temperature, logprobs=True, **settings)
+            want = torch.tensor([0.0, 0.0, 0.0, -0.6931471805599453, 0.0], dtype=torch.float64).float()
+            assert tokens.tolist() == [1, 2, 3, 70, 4]
+            assert torch.equal(policy.cpu(), want) and torch.equal(sampling.cpu(), want)
