@@ -421,6 +421,9 @@ class LlamaPagedDecodeRunner:
     def _head_norms(self, att, q: torch.Tensor, k: torch.Tensor):
         """The attention's norms of q and k heads and whether the fused append
         restates them: (q_norm, k_norm, restated), or None without norms."""
+        found, plain = (att._modules, att.__dict__) if type(att) is _Attention else (None, None)
+        if found is not None and not ("q_norm" in found or "k_norm" in found or "q_norm" in plain or "k_norm" in plain):
+            return None  # looked up as attributes, the two cost 1.7 us a layer
         q_norm, k_norm = getattr(att, "q_norm", None), getattr(att, "k_norm", None)
         if q_norm is None and k_norm is None:
             return None
