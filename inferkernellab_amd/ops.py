@@ -844,7 +844,8 @@ def _host_pairs(src, dst) -> tuple[array.array, array.array]:
     if len(src) != len(dst):
         raise ValueError("src and dst must have one entry per copied block")
     try:  # entry by entry: an array takes bytes for its memory
-        return tuple(array.array("q", x if type(x) is list else list(x)) for x in (src, dst))
+        return (array.array("q", src if type(src) is list else list(src)),
+                array.array("q", dst if type(dst) is list else list(dst)))
     except OverflowError:
         raise ValueError("copy blocks: invalid block id") from None
 
