@@ -13,10 +13,10 @@
 // log2(LPR) lanes and nothing is loaded twice. v rows go through the same
 // lanes unchanged. Lane groups are numbered over the rows of all tokens: few
 // heads fill a wave as well as many. Bound: memory; 8192 tokens of 32/8 heads of
-// 128, bf16, take 42.6 us or 4.8 TB/s (a copy: 5.2), 44.5 with the row's token by
-// a 64-bit division, 50.5 with stores that stay in the caches; 32 tokens 3.0 us.
-// Three rows a group with their loads ahead are no faster (42.5) and cost few
-// tokens dearly (32: 5.1 us).
+// 128, bf16, take 44.6 us or 4.6 TB/s (a copy: 5.2), back to back. In a graph, the
+// forms in turn: 45.7 us, 45.9 with the row's token by a 64-bit division, 48.8 with
+// stores that stay in the caches; 32 tokens 2.92, 3.04 and 2.96. Three rows a group
+// with their loads ahead were no faster and cost few tokens dearly (32: 5.1 us).
 #include "fp8_row.h"
 #include "ikl_common.h"
 #include "rope_args.h"

@@ -12,10 +12,12 @@
 // A weight is held as the integer nearest to w 2^s, s so that a row's sum fits
 // 63 bits (46 at 131072 tokens): sums of integers have no rounding and no
 // order, so atomics and any split of a row give the same token, and p M and
-// u S are compared exactly. The error of a mass is at most half a unit a token,
-// 2^-47 of the likeliest token's weight; fp32 sums would move the border of a
-// token by more than what a rare token weighs. The exponential is a double
-// polynomial: fp64 multiply-adds issue at the rate of unpacked fp32 ones here.
+// u S are compared exactly. A mass is off by half a unit a token, 2^-47 of the
+// likeliest token's weight at 131072 tokens, and by 2.4e-15 of itself from the
+// exponential (11 units of a weight at s = 52, the most); fp32 sums would move
+// the border of a token by more than what a rare token weighs. The exponential is
+// a double polynomial: fp64 multiply-adds issue at the rate of unpacked fp32 ones
+// here.
 #include "ikl_common.h"
 #include "sample_row.h"
 
@@ -312,12 +314,13 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 8) void sample_pick_kernel(const Sa
 }
 
 // Workgroups of a row. One is one launch, three where a row is split, which pays
-// from 24 tokens a thread (us with top-p 0.95, one / split by 4: 1 x 24000 bf16 16.5
-// / 17.9, 1 x 16000 fp32 13.1 / 16.4, 1 x 32000 bf16 20.4 / 19.4, 48 x 32000 22.4 /
-// 23.3): into as many parts as have a vector a thread, as long as there is a compute
-// unit for each (bf16 x 131072, in 1, 4, 8 and 16: 1 row 60, 33, 28, 25; 32 rows 69,
-// 43, 38, 45; 128 rows 71, 68, 85, 126, in 2 59; 256 rows fp32 in 1 and 4: 90, 118).
-// Two parts do not pay for rows under 64 tokens a thread (100 x 50257 36.7 / 38.3).
+// from 24 tokens a thread (us with top-p 0.95, one / split by 4: 1 x 24000 bf16 17.2
+// / 18.4, 1 x 16000 fp32 13.4 / 16.4, 1 x 32000 bf16 20.6 / 19.4; not for 48 x 32000,
+// 21.7 / 23.0): into as many parts as have a vector a thread, as long as there is a
+// compute unit for each (bf16 x 131072, in 1, 4, 8 and 16: 1 row 59, 32, 27, 24; 32
+// rows 63, 37, 33, 40; 128 rows 64, 60, 76, in 2 54; in 1 and 2: 129 rows 64, 75, 192
+// rows 66, 83, 257 rows 115, 105; 256 rows fp32 in 1 and 4: 84, 108). Two parts do not
+// pay for rows under 64 tokens a thread (100 x 50257 30.3 / 33.1).
 int parts_of(int64_t rows, int64_t vocab, int64_t dtype) {
   if (vocab <= 24 * SAMPLE_THREADS) return 1;
   const int64_t per = dtype == IKL_F32 ? 4 : 8, vectors = (vocab + per - 1) / per;
