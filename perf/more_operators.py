@@ -301,11 +301,11 @@ def _bind(case, state):
     elif kind == "rows8":
         state["call"] = ikl.PreparedQuantizeRowsInt8(state["x"], group_size=group)
     else:
-        weight = ikl.pack_int4_weight(state["codes"], state["scales"], state["zeros"], group_size=group)
+        weight = ikl.pack_int4_weight(state["codes"], state["scales"], state["zeros"], group_size=group,
+                                      gated=case["epilogue"] == "silu")
         x = state["x"] if kind == "linear" else ikl.Int8Rows(state["x_codes"], state["x_scales"], group,
                                                              dtype=DTYPES[case["dtype"]])
-        state["call"] = ikl.PreparedInt4Linear(x, weight, residual=state["residual"],
-                                               silu=case["epilogue"] == "silu")
+        state["call"] = ikl.PreparedInt4Linear(x, weight, residual=state["residual"])
     if kind in ("norm8", "silu8", "rows8"):
         state["values"] = torch.empty(case["rows"], case["cols"], dtype=DTYPES[case["dtype"]], device=DEVICE)
 
