@@ -410,7 +410,7 @@ int ikl_hbm_read_probe(const void *buffer, int64_t bytes, void *sink, int64_t si
  * here). A caller compares it with IKL_ABI_VERSION of the header it was
  * built against and refuses to run on a mismatch. No counterpart in the
  * reference, whose operators are Python functions. */
-#define IKL_ABI_VERSION 4
+#define IKL_ABI_VERSION 5
 int32_t ikl_abi_version(void);
 
 /* Findings of ikl_check_metadata, a bit each. */
@@ -485,6 +485,91 @@ typedef struct ikl_decode_linear_args {
   int32_t y_packed; /* 1: y[0] of epilogue 2 in operand order */
 } ikl_decode_linear_args;
 int ikl_decode_linear(const ikl_decode_linear_args *args, void *stream);
+
+/* Rows in 8 bits: codes [rows, cols] int8 and scales [rows, cols / group]
+ * fp32, both contiguous, the codes 16-byte aligned. A value stands for
+ * code * scale; a group's scale is its largest magnitude (at least 2^-100)
+ * over 127, its codes the nearest whole numbers (ties to even) of value /
+ * scale. A group with a NaN or an infinity stands for NaN throughout. `group`
+ * is 32, 64 or 128 columns; cols is a multiple of it. */
+typedef struct ikl_int8_rows_args {
+  const void *x;     /* [rows, cols], row stride x_stride, rows 16-byte aligned */
+  const void *up;    /* NULL: the rows of x; else silu(x) * up, as x */
+  void *codes;
+  float *scales;
+  int64_t x_stride, up_stride;
+  int64_t rows, cols;
+  int32_t group;
+  int32_t dtype; /* of x and up: F16, BF16, F32 */
+} ikl_int8_rows_args;
+int ikl_quantize_rows_int8(const ikl_int8_rows_args *args, void *stream);
+
+/* out [rows, cols] (contiguous, 16-byte aligned, F16 / BF16 / F32) = code *
+ * scale, rounded once. */
+int ikl_dequantize_rows_int8(const void *codes, const float *scales, void *out, int64_t rows, int64_t cols,
+                             int32_t group, int32_t dtype, void *stream);
+
+/* ikl_add_rms_norm with its result in 8 bits: sum = x + delta (rounded to the
+ * dtype; sum may be x), the norm of it times weight in fp32, then codes and
+ * scales as ikl_quantize_rows_int8 leaves them. Rows of at most 64 KB. */
+typedef struct ikl_norm_int8_args {
+  const void *x;
+  const void *delta;  /* NULL: no residual add */
+  const void *weight; /* [cols], 16-byte aligned */
+  void *sum;          /* with delta */
+  void *codes;
+  float *scales;
+  int64_t x_stride, delta_stride, sum_stride; /* rows 16-byte aligned */
+  int64_t rows, cols;
+  int32_t group;
+  int32_t dtype;
+  float eps;
+} ikl_norm_int8_args;
+int ikl_add_rms_norm_int8(const ikl_norm_int8_args *args, void *stream);
+
+/* y = x W^T over 4-bit weights W[n][k] = scale[n][k / group] * (code[n][k] -
+ * zero[n][k / group]), code 0 .. 15, zero 0 .. 15 (8 where zeros is NULL).
+ * group is 32, 64 or 128; cols, the contraction, is a multiple of it.
+ *
+ * Weight layout: the columns of y (rows of W) in tiles of 16, the contraction
+ * in steps of 128, S = ceil(cols / 128).
+ *   codes  [tiles][S][64][16 bytes], 16-byte aligned: lane l of a step's 64
+ *          holds row l % 16 of the tile; its dword i holds 8 codes from k =
+ *          128 step + 64 (i / 2) + 16 (l / 16) + 8 (i % 2) on (group 32:
+ *          128 step + 32 i + 8 (l / 16)), of which code j < 4 is the low half
+ *          of byte j, code 4 + j the high half. Codes past the contraction or
+ *          the last column may be any.
+ *   scales [tiles][S * 128 / group][16] fp32, 16-byte aligned
+ *   zeros  the same of uint8, 4-byte aligned
+ * gated: even tiles hold a gate's rows and odd ones an up projection's, each
+ * padded to whole tiles, and y = silu(x Wgate^T) * (x Wup^T).
+ *
+ * x: F16 or BF16 rows, or rows in 8 bits with x_scales (contiguous as above).
+ * Group sums are fp32 (of 8-bit rows exact whole numbers, scaled in fp32) and
+ * their sum is fp32, rounded once to y's dtype, after the activation or
+ * residual + it (y may be residual). A row of x with a NaN or an infinity
+ * gives NaN or infinities. */
+typedef struct ikl_int4_linear_args {
+  const void *x;         /* rows 16-byte aligned */
+  const float *x_scales; /* NULL: x in `dtype` */
+  const void *codes;
+  const float *scales;
+  const void *zeros;
+  const void *residual; /* NULL, or [rows, out_cols] in `dtype`; not with gated */
+  void *y;              /* [rows, out_cols] */
+  void *workspace;      /* ikl_int4_linear_workspace_size bytes, 16-byte aligned */
+  int64_t x_stride, residual_stride, y_stride; /* elements; x_stride unused with x_scales */
+  int64_t rows, cols, out_cols;                /* gated: out_cols is half of W's rows */
+  int64_t workspace_bytes;
+  int32_t group;
+  int32_t gated;
+  int32_t dtype; /* of y and residual, and of x without x_scales: F16, BF16; F32 with x_scales */
+} ikl_int4_linear_args;
+int ikl_int4_linear(const ikl_int4_linear_args *args, void *stream);
+
+/* Bytes of workspace that ikl_int4_linear needs with these arguments (0 when
+ * it splits no contraction over workgroups). Negative on invalid arguments. */
+int64_t ikl_int4_linear_workspace_size(const ikl_int4_linear_args *args);
 
 /* KV append (in place). Slots outside [0, num_blocks*block_size) are skipped,
  * never written. Replaces append.py:69-106 / cache.py:156-189. */

@@ -27,7 +27,7 @@ IKL_PREFILL_AUTO, IKL_PREFILL_ROWS = -1, 8  # plans of ikl_paged_prefill_plan
 IKL_CHECK_LENGTH_POSITIVE, IKL_CHECK_LENGTH_CAPACITY, IKL_CHECK_BLOCK_ID, IKL_CHECK_LENGTH_MAX = 1, 2, 4, 8
 # IKL_ABI_VERSION of the header these mirrors follow; load() refuses a
 # library that reports another
-IKL_ABI_VERSION = 4
+IKL_ABI_VERSION = 5
 
 EXPORTED_SYMBOLS = (
     "ikl_last_error",
@@ -57,6 +57,11 @@ EXPORTED_SYMBOLS = (
     "ikl_hbm_read_probe",
     "ikl_qk_norm_rope_append_kv",
     "ikl_copy_blocks",
+    "ikl_add_rms_norm_int8",
+    "ikl_dequantize_rows_int8",
+    "ikl_int4_linear",
+    "ikl_int4_linear_workspace_size",
+    "ikl_quantize_rows_int8",
     "ikl_sample_tokens",
     "ikl_sample_workspace_size",
 )
@@ -362,6 +367,69 @@ class DecodeLinearArgs(ctypes.Structure):
     ]
 
 
+class Int8RowsArgs(ctypes.Structure):
+    """Mirror of ikl_int8_rows_args."""
+
+    _fields_ = [
+        ("x", _c_ptr),
+        ("up", _c_ptr),
+        ("codes", _c_ptr),
+        ("scales", _c_ptr),
+        ("x_stride", _c_i64),
+        ("up_stride", _c_i64),
+        ("rows", _c_i64),
+        ("cols", _c_i64),
+        ("group", _c_i32),
+        ("dtype", _c_i32),
+    ]
+
+
+class NormInt8Args(ctypes.Structure):
+    """Mirror of ikl_norm_int8_args."""
+
+    _fields_ = [
+        ("x", _c_ptr),
+        ("delta", _c_ptr),
+        ("weight", _c_ptr),
+        ("sum", _c_ptr),
+        ("codes", _c_ptr),
+        ("scales", _c_ptr),
+        ("x_stride", _c_i64),
+        ("delta_stride", _c_i64),
+        ("sum_stride", _c_i64),
+        ("rows", _c_i64),
+        ("cols", _c_i64),
+        ("group", _c_i32),
+        ("dtype", _c_i32),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class Int4LinearArgs(ctypes.Structure):
+    """Mirror of ikl_int4_linear_args."""
+
+    _fields_ = [
+        ("x", _c_ptr),
+        ("x_scales", _c_ptr),
+        ("codes", _c_ptr),
+        ("scales", _c_ptr),
+        ("zeros", _c_ptr),
+        ("residual", _c_ptr),
+        ("y", _c_ptr),
+        ("workspace", _c_ptr),
+        ("x_stride", _c_i64),
+        ("residual_stride", _c_i64),
+        ("y_stride", _c_i64),
+        ("rows", _c_i64),
+        ("cols", _c_i64),
+        ("out_cols", _c_i64),
+        ("workspace_bytes", _c_i64),
+        ("group", _c_i32),
+        ("gated", _c_i32),
+        ("dtype", _c_i32),
+    ]
+
+
 DECODE_LINEAR_MAX_ROWS = 16  # IKL_DECODE_LINEAR_MAX_ROWS
 
 _lock = threading.Lock()
@@ -418,6 +486,16 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ikl_paged_decode_step_workspace_size.restype = _c_i64
     lib.ikl_paged_decode_step_workspace_size.argtypes = [ctypes.POINTER(PagedAttentionArgs),
                                                          ctypes.POINTER(AppendArgs)]
+    lib.ikl_quantize_rows_int8.restype = ctypes.c_int
+    lib.ikl_quantize_rows_int8.argtypes = [ctypes.POINTER(Int8RowsArgs), _c_ptr]
+    lib.ikl_dequantize_rows_int8.restype = ctypes.c_int
+    lib.ikl_dequantize_rows_int8.argtypes = [_c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i32, _c_i32, _c_ptr]
+    lib.ikl_add_rms_norm_int8.restype = ctypes.c_int
+    lib.ikl_add_rms_norm_int8.argtypes = [ctypes.POINTER(NormInt8Args), _c_ptr]
+    lib.ikl_int4_linear.restype = ctypes.c_int
+    lib.ikl_int4_linear.argtypes = [ctypes.POINTER(Int4LinearArgs), _c_ptr]
+    lib.ikl_int4_linear_workspace_size.restype = _c_i64
+    lib.ikl_int4_linear_workspace_size.argtypes = [ctypes.POINTER(Int4LinearArgs)]
     lib.ikl_qk_norm_rope_append_kv.restype = ctypes.c_int
     lib.ikl_qk_norm_rope_append_kv.argtypes = [ctypes.POINTER(QKNormRopeArgs), _c_ptr]
     lib.ikl_copy_blocks.restype = ctypes.c_int

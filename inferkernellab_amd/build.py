@@ -26,6 +26,8 @@ SOURCES = (
     "append_kv.hip",
     "check_metadata.hip",
     "copy_blocks.hip",
+    "int4_linear.hip",
+    "int8_rows.hip",
     "layer_ops.hip",
     "norm_rope.hip",
     "paged_decode.hip",

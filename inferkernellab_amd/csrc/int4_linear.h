@@ -1,0 +1,144 @@
+// Parts that the kernels over 4-bit weights share: the parameters, the
+// unpacking of codes into matrix operands, the products of a group and the
+// stores of y.
+//
+// W[n][k] = s[n][g] (c[n][k] - z[n][g]), so with P = sum over a group of x c
+// and X = sum over it of x,  y = sum_g s (P - z X).  Codes are whole numbers
+// up to 15, exact in every operand type: what is rounded is the fp32 sums.
+// Over 16-bit rows a code reaches its operand through the E4M3 form of its
+// byte: 0 .. 15 read as E4M3 are code * 2^-9 (subnormals, then the first
+// binade, whose step is the same), so one conversion with a scale of 2^9
+// turns two of them into 16-bit numbers. Over 8-bit rows z is taken off the
+// bytes themselves.
+#pragma once
+
+#include "ikl_common.h"
+#include "mfma_ops.h"
+
+namespace ikl {
+namespace {
+
+struct i8_tag {};
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+
+struct Int4Params {
+  const char *x;
+  int64_t x_st;     // bytes
+  const float *xs;  // 8-bit rows: [rows][groups]
+  const char *codes;
+  const float *scales;
+  const uint8_t *zeros;  // nullptr: 8
+  const char *res;       // nullptr: none
+  int64_t res_st;        // bytes
+  char *y;
+  int64_t y_st;  // bytes
+  float *part;   // split contraction: [split][rows][16 * tiles]
+  int64_t rows;
+  int32_t outs;    // columns of y
+  int32_t tiles;   // 16-row tiles of W
+  int32_t steps;   // of 128 along the contraction
+  int32_t groups;  // of the contraction
+  int32_t gated;
+  int32_t dtype;  // of y
+  int32_t wide;   // y and residual take four columns in one access
+};
+
+__device__ inline float silu(float x) { return x / (1.f + expf(-x)); }
+
+// ------------------------------------------------------------- operands
+template <typename XT>
+struct codes_as;
+template <>
+struct codes_as<bf16_tag> {
+  __device__ static inline uint32_t two(uint32_t w, bool high) {
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.f, false));
+  }
+};
+template <>
+struct codes_as<f16_tag> {
+  __device__ static inline uint32_t two(uint32_t w, bool high) {
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 512.f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 512.f, false));
+  }
+};
+
+// The 8 codes of a dword as an operand of 16-bit numbers 0 .. 15.
+template <typename XT>
+__device__ inline v4u32 unpack16(uint32_t w) {
+  const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+  return v4u32{codes_as<XT>::two(lo, false), codes_as<XT>::two(lo, true), codes_as<XT>::two(hi, false),
+               codes_as<XT>::two(hi, true)};
+}
+
+// The 8 codes of a dword less the zero point (its byte in all four bytes of
+// z4), as signed bytes: the high bit keeps a byte's borrow inside it.
+__device__ inline u32x2_t unpack8(uint32_t w, uint32_t z4) {
+  const uint32_t lo = (w & 0x0f0f0f0fu) | 0x80808080u, hi = ((w >> 4) & 0x0f0f0f0fu) | 0x80808080u;
+  return u32x2_t{(lo - z4) ^ 0x80808080u, (hi - z4) ^ 0x80808080u};
+}
+
+// First k of a lane's dword i within a step; q = lane / 16.
+template <int G>
+__device__ inline int dword_k(int i, int q) {
+  return G == 32 ? 32 * i + 8 * q : 64 * (i >> 1) + 16 * q + 8 * (i & 1);
+}
+
+// ------------------------------------------------------------- the result
+template <typename Tag>
+__device__ inline float load_one(const char *p) {
+  if constexpr (__is_same(Tag, f32_tag)) return *reinterpret_cast<const float *>(p);
+  else if constexpr (__is_same(Tag, f16_tag)) return (float)*reinterpret_cast<const _Float16 *>(p);
+  else return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t *>(p) << 16);
+}
+
+template <typename Tag>
+__device__ inline void finish_as(const Int4Params &p, int64_t row, int col, f32x4_t v) {
+  constexpr int EB = __is_same(Tag, f32_tag) ? 4 : 2;
+  char *y = p.y + row * p.y_st + (int64_t)EB * col;
+  const char *r = p.res ? p.res + row * p.res_st + (int64_t)EB * col : nullptr;
+  if (p.wide && col + 4 <= p.outs) {
+    if constexpr (EB == 4) {
+      if (r) v += *reinterpret_cast<const f32x4_t *>(r);
+      *reinterpret_cast<f32x4_t *>(y) = v;
+    } else {
+      if (r) {
+        const u32x2_t w = *reinterpret_cast<const u32x2_t *>(r);
+        v += f32x4_t{mfma_ops<Tag>::lo(w[0]), mfma_ops<Tag>::hi(w[0]), mfma_ops<Tag>::lo(w[1]), mfma_ops<Tag>::hi(w[1])};
+      }
+      *reinterpret_cast<u32x2_t *>(y) = u32x2_t{mfma_ops<Tag>::pack(v[0], v[1]), mfma_ops<Tag>::pack(v[2], v[3])};
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (col + i >= p.outs) break;
+    float x = v[i];
+    if (r) x += load_one<Tag>(r + EB * i);
+    if constexpr (EB == 4) *reinterpret_cast<float *>(y + EB * i) = x;
+    else *reinterpret_cast<uint16_t *>(y + EB * i) = (uint16_t)mfma_ops<Tag>::pack(x, x);
+  }
+}
+
+// Four columns of y from `col` on, of sums v.
+__device__ inline void finish(const Int4Params &p, int64_t row, int col, f32x4_t v) {
+  if (p.dtype == IKL_BF16) finish_as<bf16_tag>(p, row, col, v);
+  else if (p.dtype == IKL_F16) finish_as<f16_tag>(p, row, col, v);
+  else finish_as<f32_tag>(p, row, col, v);
+}
+
+__device__ inline f32x4_t gate_up(f32x4_t gate, f32x4_t up) {
+  f32x4_t v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = silu(gate[i]) * up[i];
+  return v;
+}
+
+// Columns of y that lane group q holds of a tile (of a pair's first tile
+// where the weight is gated).
+__device__ inline int tile_col(const Int4Params &p, int tile, int q) {
+  return (p.gated ? tile >> 1 : tile) * 16 + 4 * q;
+}
+
+}  // namespace
+}  // namespace ikl
