@@ -27,6 +27,9 @@ SOURCES = (
     "check_metadata.hip",
     "copy_blocks.hip",
     "int4_linear.hip",
+    "int4_linear_bf16.hip",
+    "int4_linear_f16.hip",
+    "int4_linear_i8.hip",
     "int8_rows.hip",
     "layer_ops.hip",
     "norm_rope.hip",

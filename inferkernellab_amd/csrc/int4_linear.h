@@ -16,10 +16,6 @@
 #include "mfma_ops.h"
 
 namespace ikl {
-namespace {
-
-struct i8_tag {};
-typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 struct Int4Params {
   const char *x;
@@ -32,7 +28,7 @@ struct Int4Params {
   int64_t res_st;        // bytes
   char *y;
   int64_t y_st;  // bytes
-  float *part;   // split contraction: [split][rows][16 * tiles]
+  float *part;   // split contraction: [split][rows][16 * tiles]; else nullptr
   int64_t rows;
   int32_t outs;    // columns of y
   int32_t tiles;   // 16-row tiles of W
@@ -42,6 +38,22 @@ struct Int4Params {
   int32_t dtype;  // of y
   int32_t wide;   // y and residual take four columns in one access
 };
+
+// How a launch is cut: mt tiles of rows and 4 wt of columns a workgroup, `split`
+// workgroups along the contraction; mt 0: the few rows' kernel.
+struct Int4Plan {
+  int mt, wt, split;
+};
+
+// One for each type of x, in a source file of its own.
+void launch_int4_bf16(const Int4Params &p, int group, const Int4Plan &plan, hipStream_t s);
+void launch_int4_f16(const Int4Params &p, int group, const Int4Plan &plan, hipStream_t s);
+void launch_int4_i8(const Int4Params &p, int group, const Int4Plan &plan, hipStream_t s);
+
+namespace {
+
+struct i8_tag {};
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 __device__ inline float silu(float x) { return x / (1.f + expf(-x)); }
 
@@ -76,6 +88,24 @@ __device__ inline v4u32 unpack16(uint32_t w) {
 __device__ inline u32x2_t unpack8(uint32_t w, uint32_t z4) {
   const uint32_t lo = (w & 0x0f0f0f0fu) | 0x80808080u, hi = ((w >> 4) & 0x0f0f0f0fu) | 0x80808080u;
   return u32x2_t{(lo - z4) ^ 0x80808080u, (hi - z4) ^ 0x80808080u};
+}
+
+// The 8 codes less 8, times 16, as signed bytes: a code in the high half of its
+// byte, the byte's sign turned. Less than half of unpack8's instructions.
+__device__ inline u32x2_t unpack8_sixteenfold(uint32_t w) {
+  return u32x2_t{((w << 4) & 0xf0f0f0f0u) ^ 0x80808080u, (w & 0xf0f0f0f0u) ^ 0x80808080u};
+}
+
+// The 8 codes less z, times 2^-9, as 16-bit numbers, all exact: z9 = z * 2^-9.
+template <typename XT>
+__device__ inline v4u32 unpack16_less(uint32_t w, float z9) {
+  const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+  const f32x2_t f[4] = {__builtin_amdgcn_cvt_pk_f32_fp8((int)lo, false), __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, true),
+                        __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, false), __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, true)};
+  v4u32 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = mfma_ops<XT>::pack(f[i][0] - z9, f[i][1] - z9);
+  return v;
 }
 
 // First k of a lane's dword i within a step; q = lane / 16.
