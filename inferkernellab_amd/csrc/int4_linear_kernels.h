@@ -184,6 +184,7 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
   __shared__ __attribute__((aligned(16))) float xsc[2][I8 ? 256 * GPS : 4];  // the rows repeat up to the 256th
   __shared__ __attribute__((aligned(16))) float wsc[2][4][GPS][16 * WT];
   __shared__ uint32_t wz[2][Z ? 4 * GPS * 16 * WT : 1];
+  __shared__ __attribute__((aligned(16))) char codes[2][I8 ? 4 * WT * 1024 : 16];
   const int tid = threadIdx.x, lane = tid & 63, hl = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int tile0 = (blockIdx.x * 4 + wave) * WT;
@@ -248,10 +249,18 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
       }
     }
   };
-  const char *code_at = p.codes + first * p.steps * 1024;
-  auto codes_of = [&](int n, int s) {
-    const int t = n < live ? n : 0;
-    return load16v_global(code_at + ((int64_t)t * p.steps + s) * 1024 + (uint32_t)(16 * lane));
+  // Codes: of 8-bit rows by way of LDS too, of 16-bit ones, whose rows fill
+  // it, in registers.
+  const char *code_at = p.codes + first * p.steps * 1024 + 16 * lane;
+  v4u32 w[WT];
+  auto codes_ahead = [&](int s, int b) {
+#pragma unroll
+    for (int n = 0; n < WT; ++n) {
+      const char *from = code_at + ((int64_t)(n < live ? n : 0) * p.steps + s) * 1024;
+      if constexpr (I8)
+        __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)(codes[b] + 1024 * (WT * wave + n)), 16, 0, 0);
+      else w[n] = load16v_global(from);
+    }
   };
 
   f32x4_t acc[WT][MT];
@@ -259,19 +268,24 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
   for (int n = 0; n < WT; ++n)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[n][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  v4u32 w[WT];
   rows_to_lds(s0, 0);
+  codes_ahead(s0, 0);
   fetch(s0);
-#pragma unroll
-  for (int n = 0; n < WT; ++n) w[n] = codes_of(n, s0);
   put(0);
   __syncthreads();
   for (int s = s0; s < s1; ++s) {
     const int b = (s - s0) & 1;
     const int next = s + 1 < s1 ? s + 1 : s;
-    // the other buffer was last read before the barrier that ended step s - 1
-    if (s + 1 < s1) rows_to_lds(s + 1, b ^ 1);
+    // the other buffers were last read before the barrier that ended step s - 1
+    if (s + 1 < s1) {
+      rows_to_lds(s + 1, b ^ 1);
+      if constexpr (I8) codes_ahead(s + 1, b ^ 1);
+    }
     fetch(next);
+    if constexpr (I8) {
+#pragma unroll
+      for (int n = 0; n < WT; ++n) w[n] = *reinterpret_cast<const v4u32 *>(codes[b] + 1024 * (WT * wave + n) + 16 * lane);
+    }
 #pragma unroll
     for (int g = 0; g < GPS; ++g) {
       if (GPS > 1 && s * GPS + g >= p.groups) continue;  // the contraction ends inside the step
@@ -292,40 +306,18 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
           }
         }
       }
-      if (g == GPS - 1) {
-#pragma unroll
-        for (int n = 0; n < WT; ++n) w[n] = codes_of(n, next);
-      }
+      if (!I8 && g == GPS - 1) codes_ahead(next, 0);
       f32x4_t sc[WT];
 #pragma unroll
       for (int n = 0; n < WT; ++n) sc[n] = *reinterpret_cast<const f32x4_t *>(&wsc[b][wave][g][16 * n + 4 * q]);
-      constexpr int XV = I8 ? (DPG + 1) / 2 : DPG;
-      // 8-bit rows: the next tile's rows are read ahead; 16-bit ones are twice the registers
-      v4u32 ahead[XV];
-      auto read = [&](int m) {
-        const int r = 16 * m + hl;
-        const char *xr = mem + b * (BM * RB) + r * RB;
-        if constexpr (I8 && G == 32) {
-          const int k = dword_k<G>(g, q);
-          const u32x2_t h = *reinterpret_cast<const u32x2_t *>(xr + 16 * ((k / 16) ^ (r & 7)) + (k & 8));
-          ahead[0] = v4u32{h[0], h[1], 0u, 0u};
-        } else {
+      const char *xrow = mem + b * (BM * RB) + hl * RB;
+      if constexpr (!I8) {
 #pragma unroll
-          for (int i = 0; i < XV; ++i) {
-            const int k = I8 ? dword_k<G>(g * DPG + 2 * i, q) / 16 : dword_k<G>(g * DPG + i, q) / 8;
-            ahead[i] = *reinterpret_cast<const v4u32 *>(xr + 16 * (k ^ (r & 7)));
-          }
-        }
-      };
-      if (I8) read(0);
+        for (int m = 0; m < MT; ++m) {
+          v4u32 xv[DPG];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (!I8) read(m);
-        v4u32 xv[XV];
-#pragma unroll
-        for (int i = 0; i < XV; ++i) xv[i] = ahead[i];
-        if (I8 && m + 1 < MT) read(m + 1);
-        if constexpr (!I8) {
+          for (int i = 0; i < DPG; ++i)
+            xv[i] = *reinterpret_cast<const v4u32 *>(xrow + 16 * m * RB + 16 * ((dword_k<G>(g * DPG + i, q) / 8) ^ (hl & 7)));
 #pragma unroll
           for (int n = 0; n < WT; ++n) {
             f32x4_t P = {0.f, 0.f, 0.f, 0.f};
@@ -334,25 +326,60 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(sc[n][i], P[i], acc[n][m][i]);
           }
-        } else {
-          const float sx = xsc[b][256 * g + 16 * m + hl], off = sx * -12582912.f;
+          __builtin_amdgcn_sched_barrier(0);  // or all tiles' rows are read at once, into registers that are not there
+        }
+      } else {
+        // Tile m's sums are scaled while the matrix core works on m + 1, whose
+        // rows were read an iteration before.
+        constexpr int XV = (DPG + 1) / 2;
+        v4u32 xv[2][XV];
+        float sx[3];
+        i32x4_t P[2][WT];
+        auto read = [&](int m) {
+          sx[m % 3] = xsc[b][256 * g + 16 * m + hl];
+          const char *xr = xrow + 16 * m * RB;
+          if constexpr (G == 32) {
+            const int k = dword_k<G>(g, q);
+            const u32x2_t h = *reinterpret_cast<const u32x2_t *>(xr + 16 * ((k / 16) ^ (hl & 7)) + (k & 8));
+            xv[m & 1][0] = v4u32{h[0], h[1], 0u, 0u};
+          } else {
+#pragma unroll
+            for (int i = 0; i < XV; ++i)
+              xv[m & 1][i] = *reinterpret_cast<const v4u32 *>(xr + 16 * ((dword_k<G>(g * DPG + 2 * i, q) / 16) ^ (hl & 7)));
+          }
+        };
+        auto multiply = [&](int m) {
 #pragma unroll
           for (int n = 0; n < WT; ++n) {
-            i32x4_t P = {MAGIC, MAGIC, MAGIC, MAGIC};
+            i32x4_t v = {MAGIC, MAGIC, MAGIC, MAGIC};
             if constexpr (G >= 64) {
 #pragma unroll
-              for (int i = 0; i < DPG / 2; ++i)
-                P = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a[n][i]),
-                                                          __builtin_bit_cast(i32x4_t, xv[i]), P, 0, 0, 0);
+              for (int i = 0; i < XV; ++i)
+                v = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a[n][i]),
+                                                          __builtin_bit_cast(i32x4_t, xv[m & 1][i]), v, 0, 0, 0);
             } else {
-              P = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, u32x2_t{a[n][0][0], a[n][0][1]}),
-                                                        __builtin_bit_cast(long, u32x2_t{xv[0][0], xv[0][1]}), P, 0, 0, 0);
+              v = __builtin_amdgcn_mfma_i32_16x16x32_i8(
+                  __builtin_bit_cast(long, u32x2_t{a[n][0][0], a[n][0][1]}),
+                  __builtin_bit_cast(long, u32x2_t{xv[m & 1][0][0], xv[m & 1][0][1]}), v, 0, 0, 0);
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(sc[n][i], fmaf(__int_as_float(P[i]), sx, off), acc[n][m][i]);
+            P[m & 1][n] = v;
           }
+        };
+        read(0);
+        if (MT > 1) read(1);
+        multiply(0);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if (m + 1 < MT) multiply(m + 1);
+          if (m + 2 < MT) read(m + 2);
+          const float s0x = sx[m % 3], off = s0x * -12582912.f;
+#pragma unroll
+          for (int n = 0; n < WT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[n][m][i] = fmaf(sc[n][i], fmaf(__int_as_float(P[m & 1][n][i]), s0x, off), acc[n][m][i]);
+          __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);  // or all tiles' rows are read at once, into registers that are not there
       }
     }
     put(b ^ 1);
