@@ -51,8 +51,8 @@ int check_args(const ikl_int4_linear_args *a) {
   if (a->dtype == IKL_F32 && !a->x_scales) return fail(IKL_EUNSUPPORTED, "int4 linear: rows of fp16, bf16 or 8 bits only");
   if (a->group != 32 && a->group != 64 && a->group != 128)
     return fail(IKL_EUNSUPPORTED, "int4 linear: groups of 32, 64 or 128 only");
-  if (a->cols % a->group != 0 || a->cols > (1 << 24) || a->out_cols > (1 << 24))
-    return fail(IKL_EUNSUPPORTED, "int4 linear: cols must be whole groups; cols and out_cols at most 2^24");
+  if (a->cols % a->group != 0 || a->cols >= (1 << 24) || a->out_cols >= (1 << 24))
+    return fail(IKL_EUNSUPPORTED, "int4 linear: cols must be whole groups; cols and out_cols below 2^24");
   if (a->gated && a->residual) return fail(IKL_EUNSUPPORTED, "int4 linear: a gated weight takes no residual");
   if (a->rows > 128LL * 65535) return fail(IKL_EINVAL, "int4 linear: too many rows for a launch");
   return IKL_OK;

@@ -160,13 +160,24 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
 // MAGIC, the bits of 1.5 * 2^23 as a float: the number as a float, without a
 // conversion. What turns it into its share of y are two multiply-adds: first
 // times a of its row less MAGIC times a, which is exact because a is held to
-// 22 significant bits (2^-23 of it lost at most, what one fp32 operation
-// loses), then times s of its column. a carries 2^-16 and s 2^16, so that
+// 22 significant bits (less than 2^-21 of it lost, as in four fp32 operations),
+// then times s of its column. a carries 2^-16 and s 2^16, so that
 // MAGIC * a stays finite for rows up to 2^127.
 constexpr int MAGIC = 0x4b400000;
 
 typedef const __attribute__((address_space(1))) void *global_ptr;
 typedef __attribute__((address_space(3))) void *lds_ptr;
+
+template <bool FIRST, typename A, typename B>
+struct pick {
+  using type = A;
+};
+template <typename A, typename B>
+struct pick<false, A, B> {
+  using type = B;
+};
+__device__ inline f32x2_t with_offset(f32x2_t a) { return a; }
+__device__ inline f32x2_t with_offset(float a) { return f32x2_t{a, a * -12582912.f}; }
 
 template <typename XT, int G, int MT, int WT, bool Z>
 __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, const int split) {
@@ -178,12 +189,16 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
   static_assert(LOADS >= 1, "every wave loads");
   // what s carries beside the column's scale
   constexpr float SCALE = !I8 ? 512.f : Z ? 65536.f : 4096.f;
-  // the rows' two steps; at the end each wave's accumulators of two row tiles
-  constexpr int PITCH = 16 * WT + 4, TAIL = 4 * 32 * PITCH * 4;
+  // At most 80 KB, for two workgroups on a CU: the rows' two steps (at the end
+  // each wave's accumulators of two row tiles), a of the rows and less MAGIC
+  // times it (groups of 32: a alone), the columns' scales and zero points, the
+  // codes.
+  constexpr int TAIL = 4 * 32 * 16 * WT * 4;
+  using scale_t = typename pick<(G >= 64), f32x2_t, float>::type;
   __shared__ __attribute__((aligned(16))) char mem[2 * BM * RB > TAIL ? 2 * BM * RB : TAIL];
-  __shared__ __attribute__((aligned(16))) float xsc[2][I8 ? 256 * GPS : 4];  // the rows repeat up to the 256th
+  __shared__ __attribute__((aligned(16))) scale_t xsc[2][I8 ? BM * GPS : 4];
   __shared__ __attribute__((aligned(16))) float wsc[2][4][GPS][16 * WT];
-  __shared__ uint32_t wz[2][Z ? 4 * GPS * 16 * WT : 1];
+  __shared__ uint8_t wz[2][Z ? 4 * GPS * 16 * WT : 1];
   __shared__ __attribute__((aligned(16))) char codes[2][I8 ? 4 * WT * 1024 : 16];
   const int tid = threadIdx.x, lane = tid & 63, hl = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -194,31 +209,41 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
   const int s1 = split > 1 ? (int)((int64_t)(blockIdx.z + 1) * p.steps / split) : p.steps;
 
   // This thread's chunk of its first row; its others are 256 / RC rows apart.
+  // Rows past the last: the last again.
   const int r0 = tid / RC, chunk = (tid % RC) ^ (r0 & 7);
-  const int64_t left = p.rows - 1 - row0;  // rows behind the block's first
-  const int behind = (int)(left < BM ? left : BM) - r0;
-  const char *const xthread = p.x + (row0 + (behind < 0 ? left : r0)) * p.x_st + 16 * chunk;
+  const int left = (int)(p.rows - 1 - row0 < BM ? p.rows - 1 - row0 : BM);  // rows behind the block's first
+  // 8-bit rows are contiguous: a block's offsets have 31 bits
+  const char *xthread = p.x + row0 * p.x_st;
+  if constexpr (!I8) xthread += (int64_t)(r0 < left ? r0 : left) * p.x_st + 16 * chunk;
   auto rows_to_lds = [&](int s, int b) {
-    const char *from = xthread + (int64_t)s * RB;
     // past the contraction: the row's last chunk, for groups that are skipped
+    int over = 0;
     if (GPS > 1 && (s + 1) * RC > chunks) {
-      const int over = s * RC + chunk - (chunks - 1);
-      from -= 16 * (over > 0 ? over : 0);
+      over = s * RC + chunk - (chunks - 1);
+      over = 16 * (over > 0 ? over : 0);
     }
-    // rows past the last: the last again. Computed anew each step: kept, the
-    // addresses take registers that the accumulators need.
-    int most = behind < 0 ? 0 : behind;
-    asm volatile("" : "+v"(most));
+    const char *from = xthread + (int64_t)s * RB;
+    // The rows' offsets are computed anew each step: kept, they take registers
+    // that the accumulators need.
+    int r = r0;
+    asm volatile("" : "+v"(r));
+    const int most = left > r ? left - r : 0;
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
-      const int64_t down = u * (256 / RC) < most ? u * (256 / RC) : most;
-      __builtin_amdgcn_global_load_lds((global_ptr)(from + down * p.x_st),
-                                       (lds_ptr)(mem + b * (BM * RB) + 4096 * u + 1024 * wave), 16, 0, 0);
+      const char *at;
+      if constexpr (I8) {
+        const int row = r + u * (256 / RC) < left ? r + u * (256 / RC) : left;
+        at = from + (uint32_t)(__umul24((uint32_t)row, (uint32_t)p.x_st) + 16u * chunk - over);
+      } else {
+        const int64_t down = u * (256 / RC) < most ? u * (256 / RC) : most;
+        at = from + down * p.x_st - over;
+      }
+      __builtin_amdgcn_global_load_lds((global_ptr)at, (lds_ptr)(mem + b * (BM * RB) + 4096 * u + 1024 * wave), 16, 0, 0);
     }
   };
   // Scales (and zero points) of a step: a lane each, on their way in registers
   const float *xs = I8 ? p.xs + row0 * p.groups : nullptr;
-  const uint32_t xs_at = (uint32_t)(tid % BM < left ? tid % BM : (int)left) * (uint32_t)p.groups;
+  const uint32_t xs_at = (uint32_t)(tid % BM < left ? tid % BM : left) * (uint32_t)p.groups;
   const int live = p.tiles - tile0 < 1 ? 1 : p.tiles - tile0;  // tiles that this wave has, or would read
   const int64_t first = p.tiles - tile0 < 1 ? p.tiles - 1 : tile0;
   const int64_t wbase = first * p.steps * GPS * 16;
@@ -238,25 +263,26 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
 #pragma unroll
     for (int g = 0; g < GPS; ++g) {
       if constexpr (I8) {
-        const uint32_t v = __float_as_uint(held_x[g]);
-        xsc[b][256 * g + tid] = __uint_as_float(v < 0x7f800000u ? (v + 2u) & ~3u : v) * 0x1p-16f;
+        const float a = __uint_as_float(__float_as_uint(held_x[g]) & ~3u) * 0x1p-16f;
+        if constexpr (G >= 64) xsc[b][g * BM + tid % BM] = f32x2_t{a, a * -12582912.f};
+        else xsc[b][g * BM + tid % BM] = a;  // by every thread of the row, the same
       }
       if (lane < 16 * WT) {
         wsc[b][wave][g][lane] = held_w[g] * SCALE;
         if constexpr (Z) {
-          wz[b][(wave * GPS + g) * 16 * WT + lane] = I8 ? held_z[g] * 0x01010101u : __float_as_uint((float)held_z[g] * 0x1p-9f);
+          wz[b][(wave * GPS + g) * 16 * WT + lane] = (uint8_t)held_z[g];
         }
       }
     }
   };
   // Codes: of 8-bit rows by way of LDS too, of 16-bit ones, whose rows fill
   // it, in registers.
-  const char *code_at = p.codes + first * p.steps * 1024 + 16 * lane;
+  const char *code_at = p.codes + first * p.steps * 1024;
   v4u32 w[WT];
   auto codes_ahead = [&](int s, int b) {
 #pragma unroll
     for (int n = 0; n < WT; ++n) {
-      const char *from = code_at + ((int64_t)(n < live ? n : 0) * p.steps + s) * 1024;
+      const char *from = code_at + ((int64_t)(n < live ? n : 0) * p.steps + s) * 1024 + (uint32_t)(16 * lane);
       if constexpr (I8)
         __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)(codes[b] + 1024 * (WT * wave + n)), 16, 0, 0);
       else w[n] = load16v_global(from);
@@ -293,7 +319,10 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
 #pragma unroll
       for (int n = 0; n < WT; ++n) {
         uint32_t z = 0;
-        if constexpr (Z) z = wz[b][(wave * GPS + g) * 16 * WT + 16 * n + hl];  // of this lane's row of W
+        if constexpr (Z) {  // of this lane's row of W
+          z = wz[b][(wave * GPS + g) * 16 * WT + 16 * n + hl];
+          z = I8 ? z * 0x01010101u : __float_as_uint((float)z * 0x1p-9f);
+        }
 #pragma unroll
         for (int i = 0; i < DPG; ++i) {
           const uint32_t d = w[n][g * DPG + i];
@@ -332,52 +361,49 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
         // Tile m's sums are scaled while the matrix core works on m + 1, whose
         // rows were read an iteration before.
         constexpr int XV = (DPG + 1) / 2;
-        v4u32 xv[2][XV];
-        float sx[3];
+        v4u32 xv[XV];
+        f32x2_t sx[3];  // a of the row, and less MAGIC times it
         i32x4_t P[2][WT];
         auto read = [&](int m) {
-          sx[m % 3] = xsc[b][256 * g + 16 * m + hl];
+          sx[m % 3] = with_offset(xsc[b][g * BM + 16 * m + hl]);
           const char *xr = xrow + 16 * m * RB;
           if constexpr (G == 32) {
             const int k = dword_k<G>(g, q);
             const u32x2_t h = *reinterpret_cast<const u32x2_t *>(xr + 16 * ((k / 16) ^ (hl & 7)) + (k & 8));
-            xv[m & 1][0] = v4u32{h[0], h[1], 0u, 0u};
+            xv[0] = v4u32{h[0], h[1], 0u, 0u};
           } else {
 #pragma unroll
             for (int i = 0; i < XV; ++i)
-              xv[m & 1][i] = *reinterpret_cast<const v4u32 *>(xr + 16 * ((dword_k<G>(g * DPG + 2 * i, q) / 16) ^ (hl & 7)));
+              xv[i] = *reinterpret_cast<const v4u32 *>(xr + 16 * ((dword_k<G>(g * DPG + 2 * i, q) / 16) ^ (hl & 7)));
           }
         };
-        auto multiply = [&](int m) {
+        auto multiply = [&](int m, int n) {
+          i32x4_t v = {MAGIC, MAGIC, MAGIC, MAGIC};
+          if constexpr (G >= 64) {
 #pragma unroll
-          for (int n = 0; n < WT; ++n) {
-            i32x4_t v = {MAGIC, MAGIC, MAGIC, MAGIC};
-            if constexpr (G >= 64) {
-#pragma unroll
-              for (int i = 0; i < XV; ++i)
-                v = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a[n][i]),
-                                                          __builtin_bit_cast(i32x4_t, xv[m & 1][i]), v, 0, 0, 0);
-            } else {
-              v = __builtin_amdgcn_mfma_i32_16x16x32_i8(
-                  __builtin_bit_cast(long, u32x2_t{a[n][0][0], a[n][0][1]}),
-                  __builtin_bit_cast(long, u32x2_t{xv[m & 1][0][0], xv[m & 1][0][1]}), v, 0, 0, 0);
-            }
-            P[m & 1][n] = v;
+            for (int i = 0; i < XV; ++i)
+              v = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a[n][i]),
+                                                        __builtin_bit_cast(i32x4_t, xv[i]), v, 0, 0, 0);
+          } else {
+            v = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, u32x2_t{a[n][0][0], a[n][0][1]}),
+                                                      __builtin_bit_cast(long, u32x2_t{xv[0][0], xv[0][1]}), v, 0, 0, 0);
           }
+          P[m & 1][n] = v;
         };
         read(0);
+#pragma unroll
+        for (int n = 0; n < WT; ++n) multiply(0, n);
         if (MT > 1) read(1);
-        multiply(0);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          if (m + 1 < MT) multiply(m + 1);
-          if (m + 2 < MT) read(m + 2);
-          const float s0x = sx[m % 3], off = s0x * -12582912.f;
 #pragma unroll
-          for (int n = 0; n < WT; ++n)
+          for (int n = 0; n < WT; ++n) {
+            if (m + 1 < MT) multiply(m + 1, n);
+            if (n == WT - 1 && m + 2 < MT) read(m + 2);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              acc[n][m][i] = fmaf(sc[n][i], fmaf(__int_as_float(P[m & 1][n][i]), s0x, off), acc[n][m][i]);
+              acc[n][m][i] = fmaf(sc[n][i], fmaf(__int_as_float(P[m & 1][n][i]), sx[m % 3][0], sx[m % 3][1]), acc[n][m][i]);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -386,7 +412,8 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
     __syncthreads();
   }
   // Through LDS, so that a row's columns leave side by side
-  float *mine = reinterpret_cast<float *>(mem) + wave * 32 * PITCH;
+  float *mine = reinterpret_cast<float *>(mem) + wave * 32 * 16 * WT;
+  constexpr int CHUNKS = 4 * WT;  // of four columns, exchanged by row as the rows' are
   const int tiles = p.tiles - tile0;  // that this wave has
 #pragma unroll
   for (int m0 = 0; m0 < MT; m0 += 2) {
@@ -394,7 +421,7 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
     for (int m = m0; m < m0 + 2 && m < MT; ++m)
 #pragma unroll
       for (int n = 0; n < WT; ++n)
-        *reinterpret_cast<f32x4_t *>(mine + (16 * (m - m0) + hl) * PITCH + 16 * n + 4 * q) = acc[n][m];
+        *reinterpret_cast<f32x4_t *>(mine + (16 * (m - m0) + hl) * 16 * WT + 4 * ((4 * n + q) ^ (hl % CHUNKS))) = acc[n][m];
     wave_lds_sync();
     const int units = (p.gated && !p.part) ? WT / 2 : WT;  // results of 16 columns
 #pragma unroll 1
@@ -402,15 +429,15 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
       const int r = i / (4 * units), c = i % (4 * units), n = c / 4 * (WT / units);
       const int64_t row = row0 + 16 * m0 + r;
       if (row >= p.rows || n >= tiles || 16 * m0 + r >= BM) continue;
-      const float *at = mine + r * PITCH + 16 * n + 4 * (c & 3);
-      const f32x4_t v = *reinterpret_cast<const f32x4_t *>(at);
+      const float *at = mine + r * 16 * WT;
+      const f32x4_t v = *reinterpret_cast<const f32x4_t *>(at + 4 * ((4 * n + (c & 3)) ^ (r % CHUNKS)));
       if (p.part) {
         float *to = p.part + ((int64_t)blockIdx.z * p.rows + row) * 16 * p.tiles + 16 * (tile0 + n) + 4 * (c & 3);
         *reinterpret_cast<f32x4_t *>(to) = v;
         continue;
       }
       const int col = tile_col(p, tile0 + n, c & 3);
-      if (col < p.outs) finish(p, row, col, p.gated ? gate_up(v, *reinterpret_cast<const f32x4_t *>(at + 16)) : v);
+      if (col < p.outs) finish(p, row, col, p.gated ? gate_up(v, *reinterpret_cast<const f32x4_t *>(at + 4 * ((4 * n + 4 + (c & 3)) ^ (r % CHUNKS)))) : v);
     }
     wave_lds_sync();
   }
