@@ -39,10 +39,12 @@ struct Int4Params {
   int32_t wide;   // y and residual take four columns in one access
 };
 
-// How a launch is cut: mt tiles of rows and 4 wt of columns a workgroup, `split`
-// workgroups along the contraction; mt 0: the few rows' kernel.
+// How a launch is cut: `few`: the few rows' kernel, else the many rows'; mt
+// tiles of 16 rows and nt of 16 columns a workgroup, `split` workgroups along
+// the contraction.
 struct Int4Plan {
-  int mt, wt, split;
+  bool few;
+  int mt, nt, split;
 };
 
 // One for each type of x, in a source file of its own.

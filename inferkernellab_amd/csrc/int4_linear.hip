@@ -24,13 +24,58 @@ __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Params p, cons
   if (col < p.outs) finish(p, row, col, p.gated ? gate_up(v, u) : v);
 }
 
-Int4Plan plan_of(int64_t rows, int tiles, int steps) {
-  if (rows <= 64) return {0, 0, 1};
-  const int mt = rows <= 128 ? 4 : 8, wt = 4;
-  const int64_t groups = ((rows + 16 * mt - 1) / (16 * mt)) * ((tiles + 4 * wt - 1) / (4 * wt));
-  int split = 1;
-  while (split < 16 && groups * split * 2 <= 512 && steps / (split * 2) >= 4) split *= 2;
-  return {mt, wt, split};
+// Few rows: one workgroup a CU where that covers the columns, the narrowest
+// that does, of one row tile where they fit. us at 16 rows of bf16, weights
+// from memory, column tiles a workgroup 1 / 2 / 4: 4096 x 4096 7.0 / 7.5 / 9.1;
+// 2048 columns from 5632 7.9 / 9.1 / 10.8; 14336 from 4096 21 / 13 / 9.9. 41
+// rows of 1408 to 3144 columns: 5.5 by one row tile, 6.3 by two; 32 of 4096 to
+// 14336, where one does not fit, 17.5 and 16.2.
+bool few_rows(int64_t rows, int tiles, int steps, bool gated, Int4Plan &plan) {
+  auto fits = [&](int mt, int nt) { return ((tiles + nt - 1) / nt) * ((rows + 16 * mt - 1) / (16 * mt)) <= 256; };
+  if (rows <= 64) {
+    for (int nt = gated ? 2 : 1; nt <= 4; nt *= 2)
+      if (fits(1, nt)) return plan = {true, 1, nt, 1}, true;
+    if (rows <= 32) return plan = {true, rows <= 16 ? 1 : 2, 4, 1}, true;
+  }
+  // 64 rows: 4096 x 4096 bf16 11.2 us, against 13.4 of the many rows' kernel;
+  // 14336 from 4096 28 against 25
+  if (rows <= 64 && fits(2, 2)) return plan = {true, 2, 2, 1}, true;
+  // 256 rows of 2048 x 2048 8-bit 9.3 us against 11.9; from 5632 17.1 against 16.9
+  if (steps <= 24 && fits(4, 2)) return plan = {true, 4, 2, 1}, true;
+  return false;
+}
+
+// Many rows: the cheapest by an estimate of what bounds a launch. A CU runs
+// `slots` workgroups of a form at once; a step of them takes the longer of one
+// workgroup's own time and of their tiles' work. A split contraction saves
+// steps and pays for a second launch and for the parts' way through memory.
+// Times in us from launches of 8192 and of 1024 rows of 4096, groups of 128.
+Int4Plan plan_of(int64_t rows, int tiles, int steps, bool gated, bool eight) {
+  Int4Plan best{};
+  if (few_rows(rows, tiles, steps, gated, best)) return best;
+  struct Form {
+    int mt, nt, slots;
+    double alone[2], tile[2];  // of a step: 16-bit rows, 8-bit rows
+  };
+  static const Form forms[] = {{2, 8, 4, {0.8, 0.5}, {0.0255, 0.0172}},
+                               {4, 8, 3, {1.1, 0.75}, {0.0195, 0.0137}},
+                               {4, 16, 2, {1.8, 1.3}, {0.0185, 0.0125}},
+                               {8, 16, 2, {3.3, 2.0}, {0.0166, 0.0101}}};
+  double least = 1e30;
+  for (const Form &f : forms) {
+    const double blocks = (double)((rows + 16 * f.mt - 1) / (16 * f.mt)) * ((tiles + f.nt - 1) / f.nt);
+    auto step = [&](int n) {
+      const double work = n * f.mt * f.nt * f.tile[eight];
+      return n == 0 ? 0. : work > f.alone[eight] ? work : f.alone[eight];
+    };
+    for (int split = 1; split <= 16 && (split == 1 || 2 * split <= steps); split *= 2) {
+      const int64_t per_cu = (int64_t)((blocks * split + 255) / 256);
+      double us = ((per_cu / f.slots) * step(f.slots) + step((int)(per_cu % f.slots))) * ((steps + split - 1) / split);
+      if (split > 1) us += 2.5 + split * (double)rows * tiles * 16 * 8 / 6e6;
+      if (us < least) least = us, best = {false, f.mt, f.nt, split};
+    }
+  }
+  return best;
 }
 
 int tiles_of(const ikl_int4_linear_args *a) { return (int)((a->out_cols + 15) / 16) * (a->gated ? 2 : 1); }
@@ -65,7 +110,7 @@ using namespace ikl;
 
 extern "C" int64_t ikl_int4_linear_workspace_size(const ikl_int4_linear_args *a) {
   if (const int bad = check_args(a)) return bad;
-  return part_bytes(a, plan_of(a->rows, tiles_of(a), steps_of(a)));
+  return part_bytes(a, plan_of(a->rows, tiles_of(a), steps_of(a), a->gated != 0, a->x_scales != nullptr));
 }
 
 extern "C" int ikl_int4_linear(const ikl_int4_linear_args *a, void *stream) {
@@ -98,7 +143,7 @@ extern "C" int ikl_int4_linear(const ikl_int4_linear_args *a, void *stream) {
   p.gated = a->gated != 0;
   p.dtype = a->dtype;
   p.wide = (((uintptr_t)p.y | (uintptr_t)p.y_st | (uintptr_t)p.res | (p.res ? (uintptr_t)p.res_st : 0)) & (uintptr_t)(4 * eb - 1)) == 0;
-  const Int4Plan plan = plan_of(a->rows, p.tiles, p.steps);
+  const Int4Plan plan = plan_of(a->rows, p.tiles, p.steps, a->gated != 0, a->x_scales != nullptr);
   if (const int64_t need = part_bytes(a, plan)) {
     if (!a->workspace || off16(a->workspace) || a->workspace_bytes < need)
       return fail(IKL_EWORKSPACE, "int4 linear: the workspace is missing, too small or not 16-byte aligned");

@@ -10,12 +10,29 @@ namespace {
 // --------------------------------------------------------------- few rows
 constexpr int ROW_WAVES = 8;
 
-// A workgroup owns NT tiles of 16 columns and MT tiles of 16 rows; its waves
-// split the contraction in steps of 128 and meet in LDS.
+// What a wave loads of one step, all of it on its way at once.
 template <typename XT, int G, int MT, int NT>
+struct RowsStep {
+  static constexpr bool I8 = __is_same(XT, i8_tag);
+  static constexpr int GPS = 128 / G;
+  static constexpr int XP = I8 ? 2 : 4;  // 16-byte pieces of a row
+  v4u32 w[NT], x[MT][XP];
+  f32x4_t sc[NT][GPS];
+  uint32_t z[NT][GPS];  // 16-bit rows: of the lane's four columns, a byte each; 8-bit rows: of its row of W
+  float sx[MT][I8 ? GPS : 1];
+};
+
+// A workgroup owns NT tiles of 16 columns and MT tiles of 16 rows; its waves
+// split the contraction in steps of 128 and meet in LDS. Bound: the read of W once, and below some 8 MB of it
+// the latency of that read: DEPTH steps are on their way in registers.
+//
+// 16-bit rows: z X of a group comes from a matrix product with a row operand
+// of ones, which lands in the same lanes as P; the matrix cores have the time.
+template <typename XT, int G, int MT, int NT, int DEPTH, bool Z>
 __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Params p) {
-  constexpr bool I8 = __is_same(XT, i8_tag);
-  constexpr int GPS = 128 / G, DPG = 4 / GPS;  // groups a step, dwords a group
+  using Step = RowsStep<XT, G, MT, NT>;
+  constexpr bool I8 = Step::I8;
+  constexpr int GPS = Step::GPS, DPG = 4 / GPS;  // groups a step, dwords a group
   __shared__ __attribute__((aligned(16))) float red[ROW_WAVES][NT * MT][64][4];
   const int tid = threadIdx.x, lane = tid & 63, hl = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -30,80 +47,88 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
     xrow[m] = p.x + r * p.x_st;
     xs[m] = p.xs + (I8 ? r * p.groups : 0);
   }
+  int64_t tile[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) tile[n] = tile0 + n < p.tiles ? tile0 + n : p.tiles - 1;
   f32x4_t acc[NT][MT];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[n][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  for (int s = wave; s < p.steps; s += ROW_WAVES) {
-    v4u32 w[NT];
+  auto load = [&](int s, Step &t) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int t = tile0 + n < p.tiles ? tile0 + n : p.tiles - 1;
-      w[n] = load16v_global(p.codes + (((int64_t)t * p.steps + s) * 64 + lane) * 16);
+      t.w[n] = load16v_global(p.codes + (tile[n] * p.steps + s) * 1024 + (uint32_t)(16 * lane));
+#pragma unroll
+      for (int g = 0; g < GPS; ++g) {
+        const int64_t at = (tile[n] * p.steps * GPS + s * GPS + g) * 16;
+        t.sc[n][g] = *reinterpret_cast<const f32x4_t *>(p.scales + at + (uint32_t)(4 * q));
+        if constexpr (Z) {
+          if constexpr (I8) t.z[n][g] = p.zeros[at + (uint32_t)hl];
+          else t.z[n][g] = *reinterpret_cast<const uint32_t *>(p.zeros + at + (uint32_t)(4 * q));
+        }
+      }
     }
 #pragma unroll
-    for (int g = 0; g < GPS; ++g) {
-      const int gk = s * GPS + g;
-      if (gk >= p.groups) continue;  // the contraction ends inside the step
-      v4u32 xv[MT][DPG];
-      float sx[MT];
+    for (int m = 0; m < MT; ++m) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
+      for (int g = 0; g < GPS; ++g) {
+        // past the contraction: the row's start, for groups that are skipped
+        const int step = s * GPS + g < p.groups ? s : 0, u = s * GPS + g < p.groups ? g : 0;
         if constexpr (!I8) {
 #pragma unroll
           for (int i = 0; i < DPG; ++i)
-            xv[m][i] = load16v_global(xrow[m] + 2 * ((int64_t)s * 128 + dword_k<G>(g * DPG + i, q)));
+            t.x[m][g * DPG + i] = load16v_global(xrow[m] + 2 * ((int64_t)step * 128 + dword_k<G>(u * DPG + i, q)));
         } else if constexpr (G >= 64) {
 #pragma unroll
           for (int i = 0; i < DPG / 2; ++i)
-            xv[m][i] = load16v_global(xrow[m] + (int64_t)s * 128 + dword_k<G>(g * DPG + 2 * i, q));
-          sx[m] = xs[m][gk];
+            t.x[m][g * DPG / 2 + i] = load16v_global(xrow[m] + (int64_t)step * 128 + dword_k<G>(u * DPG + 2 * i, q));
         } else {
-          const u32x2_t h = *reinterpret_cast<const u32x2_t *>(xrow[m] + (int64_t)s * 128 + dword_k<G>(g, q));
-          xv[m][0] = v4u32{h[0], h[1], 0u, 0u};
-          sx[m] = xs[m][gk];
+          const u32x2_t h = *reinterpret_cast<const u32x2_t *>(xrow[m] + (int64_t)step * 128 + dword_k<G>(u, q));
+          t.x[m][g / 2][2 * (g & 1)] = h[0];
+          t.x[m][g / 2][2 * (g & 1) + 1] = h[1];
         }
+        if constexpr (I8) t.sx[m][g] = xs[m][step * GPS + u];
       }
-      f32x4_t X[MT];
+    }
+  };
+  auto compute = [&](int s, const Step &t) {
+#pragma unroll
+    for (int g = 0; g < GPS; ++g) {
+      if (GPS > 1 && s * GPS + g >= p.groups) continue;  // the contraction ends inside the step
       if constexpr (!I8) {
         const v4u32 ones = {mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2};
+        f32x4_t X[MT];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           X[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < DPG; ++i) X[m] = mfma_ops<XT>::mma_k32(ones, xv[m][i], X[m]);
+          for (int i = 0; i < DPG; ++i) X[m] = mfma_ops<XT>::mma_k32(ones, t.x[m][g * DPG + i], X[m]);
         }
-      }
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int t = tile0 + n < p.tiles ? tile0 + n : p.tiles - 1;
-        const int64_t at = ((int64_t)t * p.steps * GPS + gk) * 16;
-        const f32x4_t sc = *reinterpret_cast<const f32x4_t *>(p.scales + at + 4 * q);
-        if constexpr (!I8) {
-          f32x4_t z = {8.f, 8.f, 8.f, 8.f};
-          if (p.zeros) {
-            const uint32_t zw = *reinterpret_cast<const uint32_t *>(p.zeros + at + 4 * q);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] = (float)((zw >> (8 * i)) & 0xffu);
-          }
+        for (int n = 0; n < NT; ++n) {
           v4u32 a[DPG];
 #pragma unroll
-          for (int i = 0; i < DPG; ++i) a[i] = unpack16<XT>(w[n][g * DPG + i]);
+          for (int i = 0; i < DPG; ++i) a[i] = unpack16<XT>(t.w[n][g * DPG + i]);
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             f32x4_t P = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < DPG; ++i) P = mfma_ops<XT>::mma_k32(a[i], xv[m][i], P);
+            for (int i = 0; i < DPG; ++i) P = mfma_ops<XT>::mma_k32(a[i], t.x[m][g * DPG + i], P);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(sc[i], fmaf(-z[i], X[m][i], P[i]), acc[n][m][i]);
+            for (int i = 0; i < 4; ++i) {
+              const float z = Z ? (float)((t.z[n][g] >> (8 * i)) & 0xffu) : 8.f;
+              acc[n][m][i] = fmaf(t.sc[n][g][i], fmaf(-z, X[m][i], P[i]), acc[n][m][i]);
+            }
           }
-        } else {
-          const uint32_t z4 = (p.zeros ? (uint32_t)p.zeros[at + hl] : 8u) * 0x01010101u;
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
           u32x2_t a[DPG];
 #pragma unroll
-          for (int i = 0; i < DPG; ++i) a[i] = unpack8(w[n][g * DPG + i], z4);
+          for (int i = 0; i < DPG; ++i) a[i] = unpack8(t.w[n][g * DPG + i], (Z ? t.z[n][g] : 8u) * 0x01010101u);
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             i32x4_t P = {0, 0, 0, 0};
@@ -112,16 +137,32 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
               for (int i = 0; i < DPG / 2; ++i)
                 P = __builtin_amdgcn_mfma_i32_16x16x64_i8(
                     i32x4_t{(int)a[2 * i][0], (int)a[2 * i][1], (int)a[2 * i + 1][0], (int)a[2 * i + 1][1]},
-                    __builtin_bit_cast(i32x4_t, xv[m][i]), P, 0, 0, 0);
+                    __builtin_bit_cast(i32x4_t, t.x[m][g * DPG / 2 + i]), P, 0, 0, 0);
             } else {
-              P = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a[0]),
-                                                        __builtin_bit_cast(long, u32x2_t{xv[m][0][0], xv[m][0][1]}), P, 0, 0, 0);
+              const v4u32 x = t.x[m][g / 2];
+              P = __builtin_amdgcn_mfma_i32_16x16x32_i8(
+                  __builtin_bit_cast(long, a[0]), __builtin_bit_cast(long, u32x2_t{x[2 * (g & 1)], x[2 * (g & 1) + 1]}), P, 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(sc[i] * sx[m], (float)P[i], acc[n][m][i]);
+            for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(t.sc[n][g][i] * t.sx[m][g], (float)P[i], acc[n][m][i]);
           }
         }
       }
+    }
+  };
+
+  Step steps[DEPTH];
+#pragma unroll
+  for (int j = 0; j < DEPTH; ++j) {
+    const int s = wave + ROW_WAVES * j;
+    if (s < p.steps) load(s, steps[j]);
+  }
+  for (int base = wave; base < p.steps; base += ROW_WAVES * DEPTH) {
+#pragma unroll
+    for (int j = 0; j < DEPTH; ++j) {
+      const int s = base + ROW_WAVES * j, next = s + ROW_WAVES * DEPTH;
+      if (s < p.steps) compute(s, steps[j]);
+      if (next < p.steps) load(next, steps[j]);
     }
   }
 #pragma unroll
@@ -132,7 +173,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
   // lane l of an accumulator: columns 4 (l / 16) + i, row l % 16
   const int per = p.gated ? 2 : 1;
   for (int u = tid; u < NT * MT * 64 / per; u += 64 * ROW_WAVES) {
-    const int l = u & 63, tm = u >> 6, n = tm / MT * per, m = tm % MT;
+    // four threads of a row side by side, tile by tile
+    const int c = u % (4 * NT / per), r = u / (4 * NT / per), n = c / 4 * per, m = r / 16, l = 16 * (c & 3) + r % 16;
     f32x4_t v[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -141,9 +183,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
 #pragma unroll
       for (int h = 0; h < ROW_WAVES; ++h) v[k] += *reinterpret_cast<const f32x4_t *>(red[h][(n + k) * MT + m][l]);
     }
-    const int64_t row = row0 + 16 * m + (l & 15);
-    const int col = tile_col(p, tile0 + n, l >> 4);
-    if (row < p.rows && col < p.outs) finish(p, row, col, p.gated ? gate_up(v[0], v[1]) : v[0]);
+    const int64_t row = row0 + r;
+    if (row >= p.rows || tile0 + n >= p.tiles) continue;
+    const int col = tile_col(p, tile0 + n, c & 3);
+    if (col < p.outs) finish(p, row, col, p.gated ? gate_up(v[0], v[1]) : v[0]);
   }
 }
 
@@ -179,8 +222,8 @@ struct pick<false, A, B> {
 __device__ inline f32x2_t with_offset(f32x2_t a) { return a; }
 __device__ inline f32x2_t with_offset(float a) { return f32x2_t{a, a * -12582912.f}; }
 
-template <typename XT, int G, int MT, int WT, bool Z>
-__global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, const int split) {
+template <typename XT, int G, int MT, int WT, int NST, bool Z>
+__global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const Int4Params p, const int split) {
   constexpr bool I8 = __is_same(XT, i8_tag);
   constexpr int GPS = 128 / G, DPG = 4 / GPS;
   constexpr int BM = 16 * MT;
@@ -189,17 +232,16 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
   static_assert(LOADS >= 1, "every wave loads");
   // what s carries beside the column's scale
   constexpr float SCALE = !I8 ? 512.f : Z ? 65536.f : 4096.f;
-  // At most 80 KB, for two workgroups on a CU: the rows' two steps (at the end
-  // each wave's accumulators of two row tiles), a of the rows and less MAGIC
-  // times it (groups of 32: a alone), the columns' scales and zero points, the
-  // codes.
-  constexpr int TAIL = 4 * 32 * 16 * WT * 4;
+  // At most 80 KB, for two workgroups on a CU: the rows' steps (at the end each
+  // wave's accumulators of a row tile), a of the rows and less MAGIC times it
+  // (groups of 32: a alone), the columns' scales and zero points, the codes.
+  constexpr int TAIL = 4 * 16 * 16 * WT * 4;
   using scale_t = typename pick<(G >= 64), f32x2_t, float>::type;
-  __shared__ __attribute__((aligned(16))) char mem[2 * BM * RB > TAIL ? 2 * BM * RB : TAIL];
+  __shared__ __attribute__((aligned(16))) char mem[NST * BM * RB > TAIL ? NST * BM * RB : TAIL];
   __shared__ __attribute__((aligned(16))) scale_t xsc[2][I8 ? BM * GPS : 4];
   __shared__ __attribute__((aligned(16))) float wsc[2][4][GPS][16 * WT];
   __shared__ uint8_t wz[2][Z ? 4 * GPS * 16 * WT : 1];
-  __shared__ __attribute__((aligned(16))) char codes[2][I8 ? 4 * WT * 1024 : 16];
+  __shared__ __attribute__((aligned(16))) char codes[NST][I8 ? 4 * WT * 1024 : 16];
   const int tid = threadIdx.x, lane = tid & 63, hl = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int tile0 = (blockIdx.x * 4 + wave) * WT;
@@ -294,20 +336,30 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
   for (int n = 0; n < WT; ++n)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[n][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  rows_to_lds(s0, 0);
-  codes_ahead(s0, 0);
+  // A step's rows and codes are NST - 1 steps on their way, its scales one. The
+  // scales' loads of a step are issued before the rows' of a later one, and
+  // loads return in order: who has the first waits for no more.
+  constexpr int FLIGHT = LOADS + (I8 ? WT : 0);  // a step's loads to LDS
+  auto ahead = [&](int s, int b) {
+    rows_to_lds(s, b);
+    if constexpr (I8) codes_ahead(s, b);
+  };
+#pragma unroll
+  for (int j = 0; j < NST - 1; ++j) ahead(s0 + j < s1 ? s0 + j : s1 - 1, j);
+  if constexpr (!I8) codes_ahead(s0, 0);
   fetch(s0);
   put(0);
   __syncthreads();
+  int b = 0;  // s's buffer of rows and codes
   for (int s = s0; s < s1; ++s) {
-    const int b = (s - s0) & 1;
+    const int sb = (s - s0) & 1, last = b == 0 ? NST - 1 : b - 1;
     const int next = s + 1 < s1 ? s + 1 : s;
-    // the other buffers were last read before the barrier that ended step s - 1
-    if (s + 1 < s1) {
-      rows_to_lds(s + 1, b ^ 1);
-      if constexpr (I8) codes_ahead(s + 1, b ^ 1);
-    }
+    // past the last step: the last again, so that every step asks for as much
+    const int later = s + NST - 1 < s1 ? s + NST - 1 : s1 - 1;
     fetch(next);
+    asm volatile("" ::: "memory");
+    // buffer `last` was last read before the barrier that ended step s - 1
+    if (I8) ahead(later, last);
     if constexpr (I8) {
 #pragma unroll
       for (int n = 0; n < WT; ++n) w[n] = *reinterpret_cast<const v4u32 *>(codes[b] + 1024 * (WT * wave + n) + 16 * lane);
@@ -320,7 +372,7 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
       for (int n = 0; n < WT; ++n) {
         uint32_t z = 0;
         if constexpr (Z) {  // of this lane's row of W
-          z = wz[b][(wave * GPS + g) * 16 * WT + 16 * n + hl];
+          z = wz[sb][(wave * GPS + g) * 16 * WT + 16 * n + hl];
           z = I8 ? z * 0x01010101u : __float_as_uint((float)z * 0x1p-9f);
         }
 #pragma unroll
@@ -335,10 +387,14 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
           }
         }
       }
-      if (!I8 && g == GPS - 1) codes_ahead(next, 0);
+      if (!I8 && g == GPS - 1) {  // (a step that ends early is the last)
+        codes_ahead(next, 0);
+        asm volatile("" ::: "memory");
+        ahead(later, last);
+      }
       f32x4_t sc[WT];
 #pragma unroll
-      for (int n = 0; n < WT; ++n) sc[n] = *reinterpret_cast<const f32x4_t *>(&wsc[b][wave][g][16 * n + 4 * q]);
+      for (int n = 0; n < WT; ++n) sc[n] = *reinterpret_cast<const f32x4_t *>(&wsc[sb][wave][g][16 * n + 4 * q]);
       const char *xrow = mem + b * (BM * RB) + hl * RB;
       if constexpr (!I8) {
 #pragma unroll
@@ -365,7 +421,7 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
         f32x2_t sx[3];  // a of the row, and less MAGIC times it
         i32x4_t P[2][WT];
         auto read = [&](int m) {
-          sx[m % 3] = with_offset(xsc[b][g * BM + 16 * m + hl]);
+          sx[m % 3] = with_offset(xsc[sb][g * BM + 16 * m + hl]);
           const char *xr = xrow + 16 * m * RB;
           if constexpr (G == 32) {
             const int k = dword_k<G>(g, q);
@@ -408,27 +464,33 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
         }
       }
     }
-    put(b ^ 1);
-    __syncthreads();
+    put(sb ^ 1);
+    // step s + 1's rows and codes are there when no more is on its way than
+    // what was asked for after them (vmcnt of s_waitcnt: bits 0-3 and 14-15)
+    constexpr int LATER = (NST - 2) * FLIGHT;
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (LATER & 15) | (LATER >> 4) << 14);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    b = b + 1 == NST ? 0 : b + 1;
   }
+  if constexpr (NST > 2) __syncthreads();  // the last loads write where the tail does
   // Through LDS, so that a row's columns leave side by side
-  float *mine = reinterpret_cast<float *>(mem) + wave * 32 * 16 * WT;
+  float *mine = reinterpret_cast<float *>(mem) + wave * 16 * 16 * WT;
   constexpr int CHUNKS = 4 * WT;  // of four columns, exchanged by row as the rows' are
   const int tiles = p.tiles - tile0;  // that this wave has
 #pragma unroll
-  for (int m0 = 0; m0 < MT; m0 += 2) {
+  for (int m = 0; m < MT; ++m) {
 #pragma unroll
-    for (int m = m0; m < m0 + 2 && m < MT; ++m)
-#pragma unroll
-      for (int n = 0; n < WT; ++n)
-        *reinterpret_cast<f32x4_t *>(mine + (16 * (m - m0) + hl) * 16 * WT + 4 * ((4 * n + q) ^ (hl % CHUNKS))) = acc[n][m];
+    for (int n = 0; n < WT; ++n)
+      *reinterpret_cast<f32x4_t *>(mine + hl * 16 * WT + 4 * ((4 * n + q) ^ (hl % CHUNKS))) = acc[n][m];
     wave_lds_sync();
     const int units = (p.gated && !p.part) ? WT / 2 : WT;  // results of 16 columns
 #pragma unroll 1
-    for (int i = lane; i < 32 * 4 * units; i += 64) {
+    for (int i = lane; i < 16 * 4 * units; i += 64) {
       const int r = i / (4 * units), c = i % (4 * units), n = c / 4 * (WT / units);
-      const int64_t row = row0 + 16 * m0 + r;
-      if (row >= p.rows || n >= tiles || 16 * m0 + r >= BM) continue;
+      const int64_t row = row0 + 16 * m + r;
+      if (row >= p.rows || n >= tiles) continue;
       const float *at = mine + r * 16 * WT;
       const f32x4_t v = *reinterpret_cast<const f32x4_t *>(at + 4 * ((4 * n + (c & 3)) ^ (r % CHUNKS)));
       if (p.part) {
@@ -444,31 +506,37 @@ __global__ __launch_bounds__(256, 2) void int4_tiles_kernel(const Int4Params p, 
 }
 
 template <typename XT, int G, bool Z>
-void launch_tiles(const Int4Params &p, const Int4Plan &plan, hipStream_t s) {
-  const dim3 grid((unsigned)((p.tiles + 4 * plan.wt - 1) / (4 * plan.wt)),
-                  (unsigned)((p.rows + 16 * plan.mt - 1) / (16 * plan.mt)), (unsigned)plan.split);
-  if (plan.mt == 4) int4_tiles_kernel<XT, G, 4, 4, Z><<<grid, 256, 0, s>>>(p, plan.split);
-  else int4_tiles_kernel<XT, G, 8, 4, Z><<<grid, 256, 0, s>>>(p, plan.split);
+void launch_tiles(const Int4Params &p, const Int4Plan &plan, dim3 grid, hipStream_t s) {
+  constexpr int STAGES = __is_same(XT, i8_tag) && G == 32 ? 2 : 3;
+  if (plan.mt == 2 && plan.nt == 8) int4_tiles_kernel<XT, G, 2, 2, 3, Z><<<grid, 256, 0, s>>>(p, plan.split);
+  else if (plan.mt == 4 && plan.nt == 8) int4_tiles_kernel<XT, G, 4, 2, 3, Z><<<grid, 256, 0, s>>>(p, plan.split);
+  else if (plan.mt == 4) int4_tiles_kernel<XT, G, 4, 4, STAGES, Z><<<grid, 256, 0, s>>>(p, plan.split);
+  else int4_tiles_kernel<XT, G, 8, 4, 2, Z><<<grid, 256, 0, s>>>(p, plan.split);
+}
+
+template <typename XT, int G, bool Z>
+void launch_rows(const Int4Params &p, const Int4Plan &plan, dim3 grid, hipStream_t s) {
+  constexpr int WIDE = G == 32 ? 1 : 2;  // groups of 32: their scales take the registers
+  const dim3 wg(64 * ROW_WAVES);
+  if (plan.mt == 1 && plan.nt == 1) int4_rows_kernel<XT, G, 1, 1, 4, Z><<<grid, wg, 0, s>>>(p);
+  else if (plan.mt == 1 && plan.nt == 2) int4_rows_kernel<XT, G, 1, 2, 3, Z><<<grid, wg, 0, s>>>(p);
+  else if (plan.mt == 1) int4_rows_kernel<XT, G, 1, 4, WIDE, Z><<<grid, wg, 0, s>>>(p);
+  else if (plan.mt == 2 && plan.nt == 2) int4_rows_kernel<XT, G, 2, 2, 2, Z><<<grid, wg, 0, s>>>(p);
+  else if (plan.mt == 2) int4_rows_kernel<XT, G, 2, 4, __is_same(XT, i8_tag) ? WIDE : 1, Z><<<grid, wg, 0, s>>>(p);
+  else int4_rows_kernel<XT, G, 4, 2, 1, Z><<<grid, wg, 0, s>>>(p);
+}
+
+template <typename XT, int G, bool Z>
+void launch(const Int4Params &p, const Int4Plan &plan, hipStream_t s) {
+  const dim3 grid((unsigned)((p.tiles + plan.nt - 1) / plan.nt), (unsigned)((p.rows + 16 * plan.mt - 1) / (16 * plan.mt)),
+                  (unsigned)plan.split);
+  if (plan.few) launch_rows<XT, G, Z>(p, plan, grid, s);
+  else launch_tiles<XT, G, Z>(p, plan, grid, s);
 }
 
 template <typename XT, int G>
 void launch(const Int4Params &p, const Int4Plan &plan, hipStream_t s) {
-  if (plan.mt == 0) {
-    const int tiles = p.gated ? p.tiles / 2 : p.tiles;
-    const dim3 wg(64 * ROW_WAVES);
-    const unsigned n = (unsigned)tiles;
-    if (p.rows <= 16) {
-      if (p.gated) int4_rows_kernel<XT, G, 1, 2><<<dim3(n), wg, 0, s>>>(p);
-      else int4_rows_kernel<XT, G, 1, 1><<<dim3(n), wg, 0, s>>>(p);
-    } else {
-      const unsigned m = (unsigned)((p.rows + 31) / 32);
-      if (p.gated) int4_rows_kernel<XT, G, 2, 2><<<dim3(n, m), wg, 0, s>>>(p);
-      else int4_rows_kernel<XT, G, 2, 1><<<dim3(n, m), wg, 0, s>>>(p);
-    }
-    return;
-  }
-  if (p.zeros) launch_tiles<XT, G, true>(p, plan, s);
-  else launch_tiles<XT, G, false>(p, plan, s);
+  p.zeros ? launch<XT, G, true>(p, plan, s) : launch<XT, G, false>(p, plan, s);
 }
 
 template <typename XT>
