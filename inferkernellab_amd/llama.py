@@ -22,7 +22,9 @@ Beside what the reference's runner does: attention with norms of the query
 and key heads (``self_attn.q_norm`` / ``k_norm``; one launch with the RoPE and
 the append), several samples of each prompt on shared cache pages
 (``num_samples``), and drawing tokens by the sampling kernel
-(``sampler="hip"``: top-k and min-p too, inside the captured step).
+(``sampler="hip"``: top-k and min-p too, inside the captured step), and layers
+over 4-bit weights (``int4_weights``, made once by :func:`quantize_llama_int4`),
+their rows in 16 bits or in 8 (``int8_rows``).
 """
 
 from __future__ import annotations
@@ -41,6 +43,8 @@ from torch import nn
 from . import layer_ops, ops
 from .cache import PagedKVCache
 from .decode import ATTENTION_BACKENDS, APPEND_BACKENDS, DecodeMetadata, percentile
+from .quantized import (Int4Weight, add_rms_norm_int8_hip, int4_linear_hip, quantize_int4_weight,
+                        quantize_rows_int8_hip)
 from .runtime import InferenceRuntime
 from .sampling import PreparedSampler, sample_tokens_hip
 from .scheduler import InferenceRequest, TokenBudgetScheduler
@@ -164,6 +168,53 @@ def random_llama(config: LlamaConfig, *, seed: int = 0, device="cuda",
     return model
 
 
+# --------------------------------------------------------- 4-bit weights
+@dataclass(frozen=True)
+class Int4LlamaLayer:
+    """A layer's linears in 4 bits: q, k and v as one weight, gate and up as one."""
+
+    qkv: Int4Weight
+    o: Int4Weight
+    gate_up: Int4Weight
+    down: Int4Weight
+
+
+@dataclass(frozen=True)
+class Int4LlamaWeights:
+    """The decoder layers' linears of a model in 4 bits; runners may share it."""
+
+    layers: tuple[Int4LlamaLayer, ...]
+    group_size: int
+
+
+def _replaceable_linears(layer) -> tuple:
+    """The linears of a layer that 4-bit weights stand in for: (q, k, v, o,
+    gate, up, down). Refuses what the kernels would not restate."""
+    att, mlp = layer.self_attn, layer.mlp
+    linears = (att.q_proj, att.k_proj, att.v_proj, att.o_proj, mlp.gate_proj, mlp.up_proj, mlp.down_proj)
+    if not all(layer_ops.plain_module(m, nn.Linear) and m.bias is None for m in linears):
+        raise ValueError("4-bit weights stand in for plain nn.Linear modules without bias and hooks")
+    if not layer_ops.plain_module(mlp.act_fn, nn.SiLU):
+        raise ValueError("4-bit weights need a plain SiLU between the MLP's linears")
+    return linears
+
+
+def quantize_llama_int4(model: Any, *, group_size: int = 128, symmetric: bool = True) -> Int4LlamaWeights:
+    """The decoder layers' linear weights of ``model`` rounded to 4 bits
+    (:func:`quantize_int4_weight`), for ``LlamaPagedDecodeRunner(...,
+    int4_weights=...)``. The embedding, the norms and the head stay as they are."""
+    layers = []
+    for layer in model.model.layers:
+        q, k, v, o, gate, up, down = (m.weight.detach() for m in _replaceable_linears(layer))
+        kw = dict(group_size=group_size, symmetric=symmetric)
+        layers.append(Int4LlamaLayer(
+            qkv=quantize_int4_weight(torch.cat((q, k, v)), **kw),
+            o=quantize_int4_weight(o, **kw),
+            gate_up=quantize_int4_weight(torch.cat((gate, up)), gated=True, **kw),
+            down=quantize_int4_weight(down, **kw)))
+    return Int4LlamaWeights(tuple(layers), group_size)
+
+
 # --------------------------------------------------------------- the runner
 def _plain_row_norm(norm) -> bool:
     """True when calling `norm` normalises each row by itself and nothing else
@@ -268,13 +319,17 @@ class LlamaPagedDecodeRunner:
                  temperature: float = 0.0, top_p: float = 1.0, seed: int = 2026,
                  eos_token_ids: Sequence[int] | None = None, use_graph: bool = True,
                  prefill_attention: str = "hip", kv_cache_dtype: torch.dtype | None = None,
-                 num_samples: int = 1, sampler: str = "torch", top_k: int = 0, min_p: float = 0.0) -> None:
+                 num_samples: int = 1, sampler: str = "torch", top_k: int = 0, min_p: float = 0.0,
+                 int4_weights: Int4LlamaWeights | None = None, int8_rows: bool = False) -> None:
         """``num_samples``: continuations of each prompt, which is prefilled
         once; request ``i * num_samples + s`` is sample ``s`` of prompt ``i``
         and draws from the seed's generator of that id. ``sampler``: ``"torch"``
         draws as the reference's runner does, one request at a time; ``"hip"``
         the whole batch by :func:`sample_tokens_hip` with uniform numbers from
-        the same generators, and takes ``top_k`` and ``min_p`` (0: off)."""
+        the same generators, and takes ``top_k`` and ``min_p`` (0: off).
+        ``int4_weights`` stand in for the decoder layers' linear modules of an
+        fp16 or bf16 model; with ``int8_rows`` the rows that enter them are in
+        8 bits, of prompts and of decoded tokens alike."""
         if not prompts:
             raise ValueError("at least one prompt is required")
         if max_new_tokens <= 0:
@@ -299,6 +354,8 @@ class LlamaPagedDecodeRunner:
             raise ValueError("top_k must be non-negative and min_p must be in [0, 1]")
         if sampler == "torch" and (top_k or min_p):
             raise ValueError("top_k and min_p need the hip sampler")
+        if int8_rows and int4_weights is None:
+            raise ValueError("int8_rows needs int4_weights")
         param = next(model.parameters())
         self.model, self.device, self.dtype = model, param.device, param.dtype
         if self.device.type != "cuda":
@@ -324,6 +381,9 @@ class LlamaPagedDecodeRunner:
         self.head_dim = int(getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads)
         if self.num_heads % self.num_kv_heads != 0:
             raise ValueError("num_attention_heads must be divisible by num_key_value_heads")
+        self._int4, self.int8_rows = int4_weights, int8_rows
+        if int4_weights is not None:
+            self._check_int4(int4_weights)
         self.prompt_lengths = tuple(len(p) for p in self.prompts)
         width = max(-(-(n + max_new_tokens) // block_size) for n in self.prompt_lengths)
         # a prompt's whole pages are held by all its samples
@@ -377,6 +437,46 @@ class LlamaPagedDecodeRunner:
         self._has_run = False
 
     # ------------------------------------------------------------ helpers
+    def _check_int4(self, weights: Int4LlamaWeights) -> None:
+        if self.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("int4_weights need an fp16 or bf16 model")
+        layers = self.model.model.layers
+        if len(weights.layers) != len(layers):
+            raise ValueError("int4_weights have another number of layers than the model")
+        for layer, w in zip(layers, weights.layers):
+            q, k, v, o, gate, up, down = _replaceable_linears(layer)
+            sizes = ((w.qkv, q.out_features + k.out_features + v.out_features, q.in_features),
+                     (w.o, o.out_features, o.in_features), (w.gate_up, gate.out_features, gate.in_features),
+                     (w.down, down.out_features, down.in_features))
+            if any((t.out_features, t.in_features) != (rows, cols) or t.group_size != weights.group_size
+                   or t.gated != (t is w.gate_up) for t, rows, cols in sizes):
+                raise ValueError("int4_weights have other sizes than the model")
+            if any(t.device != self.device for t, _, _ in sizes):
+                raise ValueError("int4_weights must be on the model's device")
+
+    def _int4_rows(self, x: torch.Tensor):
+        return quantize_rows_int8_hip(x, group_size=self._int4.group_size) if self.int8_rows else x
+
+    def _int4_norm(self, norm, hidden: torch.Tensor, delta: torch.Tensor | None = None):
+        """(hidden + delta, norm of it as the 4-bit linears take it)."""
+        if self.int8_rows and self._norm_restated(norm, hidden, delta):
+            return add_rms_norm_int8_hip(hidden, delta, norm.weight, eps=norm.variance_epsilon,
+                                         group_size=self._int4.group_size)
+        hidden, x = self._add_norm(norm, hidden, delta)
+        return hidden, self._int4_rows(x.to(self.dtype))
+
+    def _int4_qkv(self, w: Int4LlamaLayer, x):
+        """q [..., H, D], k and v [..., Hkv, D], column ranges of one product."""
+        d, sizes = self.head_dim, (self.num_heads, self.num_kv_heads, self.num_kv_heads)
+        parts = int4_linear_hip(x, w.qkv).split([h * d for h in sizes], dim=-1)
+        return tuple(t.unflatten(-1, (h, d)) for t, h in zip(parts, sizes))
+
+    def _int4_tail(self, layer, w: Int4LlamaLayer, hidden: torch.Tensor, attended: torch.Tensor) -> torch.Tensor:
+        """The layer behind its attention."""
+        hidden = int4_linear_hip(self._int4_rows(attended), w.o, residual=hidden)
+        _, x = self._int4_norm(layer.post_attention_layernorm, hidden)
+        return int4_linear_hip(self._int4_rows(int4_linear_hip(x, w.gate_up)), w.down, residual=hidden)
+
     def _prompt(self, request: InferenceRequest) -> tuple[int, ...]:
         return self.prompts[request.request_id // self.num_samples]
 
@@ -439,14 +539,15 @@ class LlamaPagedDecodeRunner:
     def _rope_append(self, layer: int, att, q, k, v, cos, sin, slots) -> torch.Tensor:
         """RoPE of q and k [T, heads, D] and the append of k and v at slots [T],
         after the heads' norms where the attention has them: one launch where
-        the norms are plain. Returns the rotated q (q itself, in place)."""
+        the norms are plain. Returns the rotated q (a contiguous q in place)."""
         norms = self._head_norms(att, q, k)
         if norms is not None and norms[2]:
             return ops.qk_norm_rope_append_kv_hip(q, k, v, norms[0].weight, norms[1].weight, cos, sin, self.cache,
                                                   slots, layer, eps=norms[0].variance_epsilon)
         if norms is not None:
             q, k = (x if norm is None else norm(x) for norm, x in zip(norms, (q, k)))
-        return ops.rope_append_kv_hip(q, k, v, cos, sin, self.cache, slots, layer=layer)
+        out = None if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return ops.rope_append_kv_hip(q, k, v, cos, sin, self.cache, slots, layer=layer, query_out=out)
 
     def _rope_qk(self, att, q, k, cos, sin):
         """The same without the append, by the modules and torch."""
@@ -503,16 +604,22 @@ class LlamaPagedDecodeRunner:
         delta = None  # the last block's output, not yet added to `hidden`
         for li, layer in enumerate(m.layers):
             att = layer.self_attn
-            kernels = self._decode_linears(layer, hidden, delta)
-            hidden, x = self._add_norm(layer.input_layernorm, hidden, delta, packed=kernels)
-            delta = None
-            if kernels:
-                q, k, v = layer_ops.decode_linear(x, (att.q_proj.weight, att.k_proj.weight, att.v_proj.weight), rows=n)
+            int4 = None if self._int4 is None else self._int4.layers[li]
+            kernels = int4 is None and self._decode_linears(layer, hidden, delta)
+            if int4 is not None:
+                hidden, x = self._int4_norm(layer.input_layernorm, hidden)
+                q, k, v = self._int4_qkv(int4, x)
             else:
-                q, k, v = att.q_proj(x), att.k_proj(x), att.v_proj(x)
-            q = q.view(n, self.num_heads, self.head_dim)
-            k = k.view(n, self.num_kv_heads, self.head_dim)
-            v = v.view(n, self.num_kv_heads, self.head_dim)
+                hidden, x = self._add_norm(layer.input_layernorm, hidden, delta, packed=kernels)
+                delta = None
+                if kernels:
+                    q, k, v = layer_ops.decode_linear(x, (att.q_proj.weight, att.k_proj.weight, att.v_proj.weight),
+                                                      rows=n)
+                else:
+                    q, k, v = att.q_proj(x), att.k_proj(x), att.v_proj(x)
+                q = q.view(n, self.num_heads, self.head_dim)
+                k = k.view(n, self.num_kv_heads, self.head_dim)
+                v = v.view(n, self.num_kv_heads, self.head_dim)
             if fused:  # RoPE of q and k + append of rope(k), v: one launch (q rotated in place)
                 q = self._rope_append(li, att, q, k, v, cos2, sin2, slots)
             else:
@@ -521,7 +628,9 @@ class LlamaPagedDecodeRunner:
             o = self._attend(q.contiguous(), self.cache, tables, lens, layer=li, validate_inputs=validate and li == 0,
                              max_context_len=self._max_ctx)
             o = o.reshape(n, self.num_heads * self.head_dim)
-            if kernels:
+            if int4 is not None:
+                hidden = self._int4_tail(layer, int4, hidden, o)
+            elif kernels:
                 hidden = layer_ops.decode_linear(o, (att.o_proj.weight,), residual=hidden)
                 _, x = self._add_norm(layer.post_attention_layernorm, hidden, None, packed=True)
                 x = layer_ops.decode_linear(x, (layer.mlp.gate_proj.weight, layer.mlp.up_proj.weight), rows=n,
@@ -598,11 +707,16 @@ class LlamaPagedDecodeRunner:
                                                num_heads=self.num_heads, query_width=t)
         delta = None  # the last block's output, not yet added to `hidden`
         for li, layer in enumerate(m.layers):
-            hidden, x = self._add_norm(layer.input_layernorm, hidden, delta)
             att = layer.self_attn
-            q = att.q_proj(x).view(b, t, self.num_heads, self.head_dim)
-            k = att.k_proj(x).view(b, t, self.num_kv_heads, self.head_dim)
-            v = att.v_proj(x).view(b, t, self.num_kv_heads, self.head_dim)
+            int4 = None if self._int4 is None else self._int4.layers[li]
+            if int4 is not None:
+                hidden, x = self._int4_norm(layer.input_layernorm, hidden)
+                q, k, v = self._int4_qkv(int4, x)
+            else:
+                hidden, x = self._add_norm(layer.input_layernorm, hidden, delta)
+                q = att.q_proj(x).view(b, t, self.num_heads, self.head_dim)
+                k = att.k_proj(x).view(b, t, self.num_kv_heads, self.head_dim)
+                v = att.v_proj(x).view(b, t, self.num_kv_heads, self.head_dim)
             if fused:  # q rotated in place; padding rows of k / v are skipped (slot -1)
                 q = self._rope_append(li, att, q.view(b * t, self.num_heads, self.head_dim),
                                       k.reshape(b * t, self.num_kv_heads, self.head_dim),
@@ -617,8 +731,11 @@ class LlamaPagedDecodeRunner:
                 prefill(q.transpose(1, 2), li, out=o.transpose(1, 2))
             else:
                 o = self._prefix_attention(q, li, tables, starts, ends)
-            hidden, x = self._add_norm(layer.post_attention_layernorm, hidden,
-                                       att.o_proj(o.reshape(b, t, self.num_heads * self.head_dim)))
+            o = o.reshape(b, t, self.num_heads * self.head_dim)
+            if int4 is not None:
+                hidden = self._int4_tail(layer, int4, hidden, o)
+                continue
+            hidden, x = self._add_norm(layer.post_attention_layernorm, hidden, att.o_proj(o))
             delta = self._mlp(layer.mlp, x)
         return self._last_logits(hidden, delta, spans)
 
