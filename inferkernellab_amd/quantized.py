@@ -31,9 +31,19 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _on_device, _require_backend, _stream
+from .ops import _DTYPES, _require_backend
 
 GROUP_SIZES = (32, 64, 128)
+
+
+def _launch(device: torch.device, call, *args) -> int:
+    """`call(*args, stream)` on the current stream of `device` (of a tensor,
+    so that torch has a GPU and the device an index)."""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        return call(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(device):
+        return call(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _check_group(group_size: int, cols: int) -> None:
@@ -82,44 +92,50 @@ class Int8Rows:
             raise ValueError("scales must be on the codes' device")
         if dtype not in _DTYPES:
             raise ValueError("dtype must be float16, bfloat16 or float32")
-        self.codes = codes if codes.is_contiguous() and codes.data_ptr() % 16 == 0 else codes.clone(
+        codes = codes if codes.is_contiguous() and codes.data_ptr() % 16 == 0 else codes.clone(
             memory_format=torch.contiguous_format)
-        self.scales = scales.contiguous()
-        self.group_size, self.dtype = group_size, dtype
+        self._hold(codes, scales.contiguous(), group_size, dtype)
 
     @classmethod
     def empty(cls, shape, group_size: int, dtype: torch.dtype, device: torch.device) -> "Int8Rows":
         rows = cls.__new__(cls)
-        rows.codes = torch.empty(shape, dtype=torch.int8, device=device)
-        rows.scales = torch.empty((*shape[:-1], shape[-1] // group_size), dtype=torch.float32, device=device)
-        rows.group_size, rows.dtype = group_size, dtype
+        rows._hold(torch.empty(shape, dtype=torch.int8, device=device),
+                   torch.empty((*shape[:-1], shape[-1] // group_size), dtype=torch.float32, device=device),
+                   group_size, dtype)
         return rows
 
-    @property
-    def shape(self) -> torch.Size:
-        return self.codes.shape
+    def _hold(self, codes, scales, group_size, dtype) -> None:
+        self._codes, self._scales, self.group_size, self.dtype = codes, scales, group_size, dtype
+        self.shape, self.device = codes.shape, codes.device
+        cols = codes.shape[-1]
+        self._read = (codes.data_ptr(), scales.data_ptr())
+        self._sizes = (codes.numel() // cols, cols, group_size)
 
     @property
-    def device(self) -> torch.device:
-        return self.codes.device
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
 
     def dequantize(self, dtype: torch.dtype | None = None, *, out: torch.Tensor | None = None) -> torch.Tensor:
         """What the codes stand for, in ``dtype`` (the rows' own), rounded once."""
-        lib = _require_backend()
+        if self.device.type != "cuda":
+            raise ValueError("rows must be on a GPU (torch 'cuda' device)")
         if out is None:
             dtype = self.dtype if dtype is None else dtype
             if dtype not in _DTYPES:
                 raise ValueError("dtype must be float16, bfloat16 or float32")
-            out = torch.empty(self.codes.shape, dtype=dtype, device=self.codes.device)
-        elif (out.shape != self.codes.shape or out.device != self.codes.device or out.dtype not in _DTYPES
+            out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        elif (out.shape != self.shape or out.device != self.device or out.dtype not in _DTYPES
               or not out.is_contiguous() or dtype not in (None, out.dtype)):
             raise ValueError("out must be contiguous float16, bfloat16 or float32 with the rows' shape and device")
-        cols = self.codes.shape[-1]
-        with _on_device(out.device):
-            status = lib.ikl_dequantize_rows_int8(self.codes.data_ptr(), self.scales.data_ptr(), out.data_ptr(),
-                                                  self.codes.numel() // cols, cols, self.group_size,
-                                                  _DTYPES[out.dtype], _stream(out.device))
-        _lib.check(status, "dequantize rows")
+        lib = _lib._lib or _require_backend()
+        status = _launch(self.device, lib.ikl_dequantize_rows_int8, *self._read, out.data_ptr(), *self._sizes,
+                         _DTYPES[out.dtype])
+        if status:
+            _lib.check(status, "dequantize rows")
         return out
 
 
@@ -131,8 +147,7 @@ class _Prepared:
         self._ref = ctypes.byref(args)
 
     def __call__(self):
-        with _on_device(self.device):
-            status = self._run(self._ref, _stream(self.device))
+        status = _launch(self.device, self._run, self._ref)
         if status:
             _lib.check(status, self._what)
         return self._out
