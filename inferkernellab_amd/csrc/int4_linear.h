@@ -57,7 +57,21 @@ namespace {
 struct i8_tag {};
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
-__device__ inline float silu(float x) { return x / (1.f + expf(-x)); }
+// 8-bit rows: each sum of a group leaves the matrix core as a whole number
+// below 2^22 (of codes times 16 without zero points: below 2^21) on top of
+// MAGIC, the bits of 1.5 * 2^23 as a float: the number as a float, without a
+// conversion. What turns it into its share of y are two multiply-adds: first
+// times a of its row less MAGIC times a, which is exact because a is held to
+// 22 significant bits (less than 2^-21 of it lost, as in four fp32 operations),
+// then times s of its column. a carries 2^-16 and s 2^16 (without zero points
+// 2^12), so that MAGIC * a stays finite for rows up to 2^127.
+constexpr int MAGIC = 0x4b400000;
+template <bool Z>
+constexpr float S_CARRIES = Z ? 65536.f : 4096.f;
+__device__ inline f32x2_t row_scale(float a) {
+  a = __uint_as_float(__float_as_uint(a) & ~3u) * 0x1p-16f;
+  return f32x2_t{a, a * -12582912.f};
+}
 
 // ------------------------------------------------------------- operands
 template <typename XT>
@@ -162,7 +176,7 @@ __device__ inline void finish(const Int4Params &p, int64_t row, int col, f32x4_t
 __device__ inline f32x4_t gate_up(f32x4_t gate, f32x4_t up) {
   f32x4_t v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = silu(gate[i]) * up[i];
+  for (int i = 0; i < 4; ++i) v[i] = silu_fast(gate[i]) * up[i];
   return v;
 }
 

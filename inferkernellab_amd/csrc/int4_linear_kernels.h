@@ -124,14 +124,18 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
           }
         }
       } else {
+        f32x2_t sx[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) sx[m] = row_scale(t.sx[m][g]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           u32x2_t a[DPG];
 #pragma unroll
-          for (int i = 0; i < DPG; ++i) a[i] = unpack8(t.w[n][g * DPG + i], (Z ? t.z[n][g] : 8u) * 0x01010101u);
+          for (int i = 0; i < DPG; ++i)
+            a[i] = Z ? unpack8(t.w[n][g * DPG + i], t.z[n][g] * 0x01010101u) : unpack8_sixteenfold(t.w[n][g * DPG + i]);
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
-            i32x4_t P = {0, 0, 0, 0};
+            i32x4_t P = {MAGIC, MAGIC, MAGIC, MAGIC};
             if constexpr (G >= 64) {
 #pragma unroll
               for (int i = 0; i < DPG / 2; ++i)
@@ -144,7 +148,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
                   __builtin_bit_cast(long, a[0]), __builtin_bit_cast(long, u32x2_t{x[2 * (g & 1)], x[2 * (g & 1) + 1]}), P, 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(t.sc[n][g][i] * t.sx[m][g], (float)P[i], acc[n][m][i]);
+            for (int i = 0; i < 4; ++i)
+              acc[n][m][i] = fmaf(t.sc[n][g][i], fmaf(__int_as_float(P[i]), sx[m][0], sx[m][1]), acc[n][m][i]);
           }
         }
       }
@@ -168,7 +173,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) *reinterpret_cast<f32x4_t *>(red[wave][n * MT + m][lane]) = acc[n][m];
+    for (int m = 0; m < MT; ++m)
+      *reinterpret_cast<f32x4_t *>(red[wave][n * MT + m][lane]) = I8 ? acc[n][m] * S_CARRIES<Z> : acc[n][m];
   __syncthreads();
   // lane l of an accumulator: columns 4 (l / 16) + i, row l % 16
   const int per = p.gated ? 2 : 1;
@@ -198,16 +204,9 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
 // operand lie in different banks. Codes go from memory to the wave that
 // unpacks them: no other wave reads them.
 //
-// 8-bit rows: each sum of a group leaves the matrix core as a whole number
-// below 2^22 (of codes times 16 without zero points: below 2^21) on top of
-// MAGIC, the bits of 1.5 * 2^23 as a float: the number as a float, without a
-// conversion. What turns it into its share of y are two multiply-adds: first
-// times a of its row less MAGIC times a, which is exact because a is held to
-// 22 significant bits (less than 2^-21 of it lost, as in four fp32 operations),
-// then times s of its column. a carries 2^-16 and s 2^16, so that
-// MAGIC * a stays finite for rows up to 2^127.
-constexpr int MAGIC = 0x4b400000;
-
+// 16-bit rows: codes less their zero points, exact, by way of fp32, or (up to
+// 64 rows a workgroup, where that costs more than it saves) the codes and X as
+// in the few rows' kernel.
 typedef const __attribute__((address_space(1))) void *global_ptr;
 typedef __attribute__((address_space(3))) void *lds_ptr;
 
@@ -231,7 +230,8 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
   constexpr int LOADS = BM * RC / 256;
   static_assert(LOADS >= 1, "every wave loads");
   // what s carries beside the column's scale
-  constexpr float SCALE = !I8 ? 512.f : Z ? 65536.f : 4096.f;
+  constexpr bool LESS = !I8 && MT > 4;  // codes less their zero points
+  constexpr float SCALE = I8 ? S_CARRIES<Z> : LESS ? 512.f : 1.f;
   // At most 80 KB, for two workgroups on a CU: the rows' steps (at the end each
   // wave's accumulators of a row tile), a of the rows and less MAGIC times it
   // (groups of 32: a alone), the columns' scales and zero points, the codes.
@@ -240,7 +240,7 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
   __shared__ __attribute__((aligned(16))) char mem[NST * BM * RB > TAIL ? NST * BM * RB : TAIL];
   __shared__ __attribute__((aligned(16))) scale_t xsc[2][I8 ? BM * GPS : 4];
   __shared__ __attribute__((aligned(16))) float wsc[2][4][GPS][16 * WT];
-  __shared__ uint8_t wz[2][Z ? 4 * GPS * 16 * WT : 1];
+  __shared__ __attribute__((aligned(4))) uint8_t wz[2][Z ? 4 * GPS * 16 * WT : 1];
   __shared__ __attribute__((aligned(16))) char codes[NST][I8 ? 4 * WT * 1024 : 16];
   const int tid = threadIdx.x, lane = tid & 63, hl = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -305,9 +305,9 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
 #pragma unroll
     for (int g = 0; g < GPS; ++g) {
       if constexpr (I8) {
-        const float a = __uint_as_float(__float_as_uint(held_x[g]) & ~3u) * 0x1p-16f;
-        if constexpr (G >= 64) xsc[b][g * BM + tid % BM] = f32x2_t{a, a * -12582912.f};
-        else xsc[b][g * BM + tid % BM] = a;  // by every thread of the row, the same
+        const f32x2_t a = row_scale(held_x[g]);  // by every thread of the row, the same
+        if constexpr (G >= 64) xsc[b][g * BM + tid % BM] = a;
+        else xsc[b][g * BM + tid % BM] = a[0];
       }
       if (lane < 16 * WT) {
         wsc[b][wave][g][lane] = held_w[g] * SCALE;
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
 #pragma unroll
       for (int n = 0; n < WT; ++n) {
         uint32_t z = 0;
-        if constexpr (Z) {  // of this lane's row of W
+        if constexpr (Z && (I8 || LESS)) {  // of this lane's row of W
           z = wz[sb][(wave * GPS + g) * 16 * WT + 16 * n + hl];
           z = I8 ? z * 0x01010101u : __float_as_uint((float)z * 0x1p-9f);
         }
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
             a[n][i / 2][2 * (i & 1)] = v[0];
             a[n][i / 2][2 * (i & 1) + 1] = v[1];
           } else {
-            a[n][i] = unpack16_less<XT>(d, Z ? __uint_as_float(z) : 8.f * 0x1p-9f);
+            a[n][i] = LESS ? unpack16_less<XT>(d, Z ? __uint_as_float(z) : 8.f * 0x1p-9f) : unpack16<XT>(d);
           }
         }
       }
@@ -395,6 +395,16 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
       f32x4_t sc[WT];
 #pragma unroll
       for (int n = 0; n < WT; ++n) sc[n] = *reinterpret_cast<const f32x4_t *>(&wsc[sb][wave][g][16 * n + 4 * q]);
+      float zc[WT][4];  // zero points of the lane's columns
+      if constexpr (!I8 && !LESS) {
+#pragma unroll
+        for (int n = 0; n < WT; ++n) {
+          uint32_t z4 = 0;
+          if constexpr (Z) z4 = *reinterpret_cast<const uint32_t *>(&wz[sb][(wave * GPS + g) * 16 * WT + 16 * n + 4 * q]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) zc[n][i] = Z ? (float)((z4 >> (8 * i)) & 0xffu) : 8.f;
+        }
+      }
       const char *xrow = mem + b * (BM * RB) + hl * RB;
       if constexpr (!I8) {
 #pragma unroll
@@ -403,13 +413,22 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
 #pragma unroll
           for (int i = 0; i < DPG; ++i)
             xv[i] = *reinterpret_cast<const v4u32 *>(xrow + 16 * m * RB + 16 * ((dword_k<G>(g * DPG + i, q) / 8) ^ (hl & 7)));
+          f32x4_t X = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (!LESS) {
+            const v4u32 ones = {mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2};
+#pragma unroll
+            for (int i = 0; i < DPG; ++i) X = mfma_ops<XT>::mma_k32(ones, xv[i], X);
+          }
 #pragma unroll
           for (int n = 0; n < WT; ++n) {
             f32x4_t P = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < DPG; ++i) P = mfma_ops<XT>::mma_k32(a[n][i], xv[i], P);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(sc[n][i], P[i], acc[n][m][i]);
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (!LESS) P[i] = fmaf(-zc[n][i], X[i], P[i]);
+              acc[n][m][i] = fmaf(sc[n][i], P[i], acc[n][m][i]);
+            }
           }
           __builtin_amdgcn_sched_barrier(0);  // or all tiles' rows are read at once, into registers that are not there
         }

@@ -100,8 +100,6 @@ __device__ inline float quantize(const float *v, uint32_t *codes) {
   return most / 127.f;
 }
 
-__device__ inline float silu(float x) { return x / (1.f + expf(-x)); }
-
 template <int N>
 __device__ inline void store_codes(char *p, const uint32_t *codes) {
   if constexpr (N == 8) *reinterpret_cast<u32x2_t *>(p) = u32x2_t{codes[0], codes[1]};
@@ -132,7 +130,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const RowsParams p) 
     float u[N];
     piece<Tag>::get(load16v_global(p.up + row * p.up_st + 16 * (int64_t)c), u);
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = silu(v[e]) * u[e];
+    for (int e = 0; e < N; ++e) v[e] = silu_fast(v[e]) * u[e];
   }
   uint32_t codes[N / 4];
   const float scale = quantize<N, LANES, !SILU>(v, codes);
