@@ -68,7 +68,7 @@ Int4Plan plan_of(int64_t rows, int tiles, int steps, bool gated, bool eight) {
       const double work = n * f.mt * f.nt * f.tile[eight];
       return n == 0 ? 0. : work > f.alone[eight] ? work : f.alone[eight];
     };
-    for (int split = 1; split <= 16 && (split == 1 || 2 * split <= steps); split *= 2) {
+    for (int split = 1; split <= 16 && (split == 1 || 2 * split <= steps); ++split) {
       const int64_t per_cu = (int64_t)((blocks * split + 255) / 256);
       double us = ((per_cu / f.slots) * step(f.slots) + step((int)(per_cu % f.slots))) * ((steps + split - 1) / split);
       if (split > 1) us += 2.5 + split * (double)rows * tiles * 16 * 8 / 6e6;

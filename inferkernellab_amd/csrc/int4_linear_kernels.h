@@ -254,9 +254,9 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
   // Rows past the last: the last again.
   const int r0 = tid / RC, chunk = (tid % RC) ^ (r0 & 7);
   const int left = (int)(p.rows - 1 - row0 < BM ? p.rows - 1 - row0 : BM);  // rows behind the block's first
-  // 8-bit rows are contiguous: a block's offsets have 31 bits
-  const char *xthread = p.x + row0 * p.x_st;
-  if constexpr (!I8) xthread += (int64_t)(r0 < left ? r0 : left) * p.x_st + 16 * chunk;
+  const char *const xblock = p.x + row0 * p.x_st;
+  // rows less than 16 MB apart (8-bit ones are): a block's offsets have 31 bits
+  const bool near = I8 || (uint64_t)p.x_st < 1u << 24;
   auto rows_to_lds = [&](int s, int b) {
     // past the contraction: the row's last chunk, for groups that are skipped
     int over = 0;
@@ -264,23 +264,26 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
       over = s * RC + chunk - (chunks - 1);
       over = 16 * (over > 0 ? over : 0);
     }
-    const char *from = xthread + (int64_t)s * RB;
+    const char *from = xblock + (int64_t)s * RB;
     // The rows' offsets are computed anew each step: kept, they take registers
     // that the accumulators need.
     int r = r0;
     asm volatile("" : "+v"(r));
-    const int most = left > r ? left - r : 0;
-#pragma unroll
-    for (int u = 0; u < LOADS; ++u) {
-      const char *at;
-      if constexpr (I8) {
-        const int row = r + u * (256 / RC) < left ? r + u * (256 / RC) : left;
-        at = from + (uint32_t)(__umul24((uint32_t)row, (uint32_t)p.x_st) + 16u * chunk - over);
-      } else {
-        const int64_t down = u * (256 / RC) < most ? u * (256 / RC) : most;
-        at = from + down * p.x_st - over;
-      }
+    auto load = [&](int u, const char *at) {
       __builtin_amdgcn_global_load_lds((global_ptr)at, (lds_ptr)(mem + b * (BM * RB) + 4096 * u + 1024 * wave), 16, 0, 0);
+    };
+    if (near) {
+#pragma unroll
+      for (int u = 0; u < LOADS; ++u) {
+        const int row = r + u * (256 / RC) < left ? r + u * (256 / RC) : left;
+        load(u, from + (uint32_t)(__umul24((uint32_t)row, (uint32_t)p.x_st) + 16u * chunk - over));
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < LOADS; ++u) {
+        const int row = r + u * (256 / RC) < left ? r + u * (256 / RC) : left;
+        load(u, from + ((int64_t)row * p.x_st + (16 * chunk - over)));
+      }
     }
   };
   // Scales (and zero points) of a step: a lane each, on their way in registers
