@@ -41,10 +41,11 @@ struct Int4Params {
 
 // How a launch is cut: `few`: the few rows' kernel, else the many rows'; mt
 // tiles of 16 rows and nt of 16 columns a workgroup, `split` workgroups along
-// the contraction.
+// the contraction; `blocks`: workgroups of a part of it, columns first.
 struct Int4Plan {
   bool few;
   int mt, nt, split;
+  int64_t blocks;
 };
 
 // One for each type of x, in a source file of its own.

@@ -9,10 +9,9 @@ namespace {
 // Sums of a split contraction's parts, in their order, and the epilogue: a
 // thread four columns of a row.
 __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Params p, const int split, const int quads) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = blockIdx.y;
-  if (i >= quads) return;
-  const int per = p.gated ? 2 : 1, tile = i / 4 * per, q = i & 3;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / quads;
+  if (row >= p.rows) return;
+  const int c = (int)(i - row * quads), per = p.gated ? 2 : 1, tile = c / 4 * per, q = c & 3;
   const float *part = p.part + row * 16 * p.tiles + 16 * tile + 4 * q;
   const int64_t step = p.rows * 16 * p.tiles;
   f32x4_t v = {0.f, 0.f, 0.f, 0.f}, u = v;
@@ -24,25 +23,28 @@ __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Params p, cons
   if (col < p.outs) finish(p, row, col, p.gated ? gate_up(v, u) : v);
 }
 
-// Few rows: one workgroup a CU where that covers the columns, the narrowest
-// that does, of one row tile where they fit. us at 16 rows of bf16, weights
-// from memory, column tiles a workgroup 1 / 2 / 4: 4096 x 4096 7.0 / 7.5 / 9.1;
-// 2048 columns from 5632 7.9 / 9.1 / 10.8; 14336 from 4096 21 / 13 / 9.9. 41
-// rows of 1408 to 3144 columns: 5.5 by one row tile, 6.3 by two; 32 of 4096 to
-// 14336, where one does not fit, 17.5 and 16.2.
-bool few_rows(int64_t rows, int tiles, int steps, bool gated, Int4Plan &plan) {
-  auto fits = [&](int mt, int nt) { return ((tiles + nt - 1) / nt) * ((rows + 16 * mt - 1) / (16 * mt)) <= 256; };
-  if (rows <= 64) {
-    for (int nt = gated ? 2 : 1; nt <= 4; nt *= 2)
-      if (fits(1, nt)) return plan = {true, 1, nt, 1}, true;
-    if (rows <= 32) return plan = {true, rows <= 16 ? 1 : 2, 4, 1}, true;
-  }
-  // 64 rows: 4096 x 4096 bf16 11.2 us, against 13.4 of the many rows' kernel;
-  // 14336 from 4096 28 against 25
-  if (rows <= 64 && fits(2, 2)) return plan = {true, 2, 2, 1}, true;
-  // 256 rows of 2048 x 2048 8-bit 9.3 us against 11.9; from 5632 17.1 against 16.9
-  if (steps <= 24 && fits(4, 2)) return plan = {true, 4, 2, 1}, true;
-  return false;
+int64_t blocks_of(int64_t rows, int tiles, int mt, int nt) {
+  return ((rows + 16 * mt - 1) / (16 * mt)) * ((tiles + nt - 1) / nt);
+}
+
+// Few rows or few columns: one workgroup a CU where that covers y, of one row
+// tile and the fewest column tiles that do, else of two row tiles. us of bf16
+// rows, weights from memory, by 1 / 2 / 4 column tiles: 16 x 4096 x 4096 7.0 /
+// 7.5 / 9.1; 2048 columns from 5632 7.9 / 9.1 / 10.8; 14336 from 4096 21 / 13 /
+// 9.9. Against the many rows' kernel: 64 x 4096 x 4096 9.2 and 13.0; 1024 x 4096
+// x 256 9.3 and 13.1; 128 x 4096 x 4096 by two row tiles 14.8 and 16.3. 8-bit
+// rows of short contractions stay ahead to three rounds of workgroups: 300 x
+// 2048 x 2048 12.1 and 15.4 (16-bit ones 15.5 and 13.7).
+bool few_rows(int64_t rows, int tiles, int steps, bool gated, bool eight, Int4Plan &plan) {
+  auto take = [&](int mt, int nt, int64_t most) {
+    const int64_t blocks = blocks_of(rows, tiles, mt, nt);
+    plan = {true, mt, nt, 1, blocks};
+    return blocks <= most;
+  };
+  for (int nt = gated ? 2 : 1; nt <= 4; nt *= 2)
+    if (take(1, nt, 256)) return true;
+  if (rows <= 16 || (eight && steps <= 16 && take(1, 4, 768))) return take(1, 4, INT64_MAX);
+  return take(2, 4, rows <= 32 ? INT64_MAX : 256);
 }
 
 // Many rows: the cheapest by an estimate of what bounds a launch. A CU runs
@@ -52,7 +54,7 @@ bool few_rows(int64_t rows, int tiles, int steps, bool gated, Int4Plan &plan) {
 // Times in us from launches of 8192 and of 1024 rows of 4096, groups of 128.
 Int4Plan plan_of(int64_t rows, int tiles, int steps, bool gated, bool eight) {
   Int4Plan best{};
-  if (few_rows(rows, tiles, steps, gated, best)) return best;
+  if (few_rows(rows, tiles, steps, gated, eight, best)) return best;
   struct Form {
     int mt, nt, slots;
     double alone[2], tile[2];  // of a step: 16-bit rows, 8-bit rows
@@ -63,16 +65,17 @@ Int4Plan plan_of(int64_t rows, int tiles, int steps, bool gated, bool eight) {
                                {8, 16, 2, {3.3, 2.0}, {0.0166, 0.0101}}};
   double least = 1e30;
   for (const Form &f : forms) {
-    const double blocks = (double)((rows + 16 * f.mt - 1) / (16 * f.mt)) * ((tiles + f.nt - 1) / f.nt);
+    const int64_t blocks = blocks_of(rows, tiles, f.mt, f.nt);
     auto step = [&](int n) {
       const double work = n * f.mt * f.nt * f.tile[eight];
       return n == 0 ? 0. : work > f.alone[eight] ? work : f.alone[eight];
     };
-    for (int split = 1; split <= 16 && (split == 1 || 2 * split <= steps); ++split) {
-      const int64_t per_cu = (int64_t)((blocks * split + 255) / 256);
+    const int most = rows * tiles < 1 << 28 ? 16 : 1;  // the join's launch holds that many
+    for (int split = 1; split <= most && (split == 1 || 2 * split <= steps); ++split) {
+      const int64_t per_cu = (blocks * split + 255) / 256;
       double us = ((per_cu / f.slots) * step(f.slots) + step((int)(per_cu % f.slots))) * ((steps + split - 1) / split);
       if (split > 1) us += 2.5 + split * (double)rows * tiles * 16 * 8 / 6e6;
-      if (us < least) least = us, best = {false, f.mt, f.nt, split};
+      if (us < least) least = us, best = {false, f.mt, f.nt, split, blocks};
     }
   }
   return best;
@@ -99,7 +102,7 @@ int check_args(const ikl_int4_linear_args *a) {
   if (a->cols % a->group != 0 || a->cols >= (1 << 24) || a->out_cols >= (1 << 24))
     return fail(IKL_EUNSUPPORTED, "int4 linear: cols must be whole groups; cols and out_cols below 2^24");
   if (a->gated && a->residual) return fail(IKL_EUNSUPPORTED, "int4 linear: a gated weight takes no residual");
-  if (a->rows > 128LL * 65535) return fail(IKL_EINVAL, "int4 linear: too many rows for a launch");
+  if (a->rows > max_grid(256) / ((a->out_cols + 15) / 16)) return fail(IKL_EINVAL, "int4 linear: too many rows for a launch");
   return IKL_OK;
 }
 
@@ -122,6 +125,7 @@ extern "C" int ikl_int4_linear(const ikl_int4_linear_args *a, void *stream) {
     return fail(IKL_EINVAL, "int4 linear: x rows must be 16-byte aligned");
   if (off16(a->codes) || off16(a->scales) || ((uintptr_t)a->zeros & 3u))
     return fail(IKL_EINVAL, "int4 linear: the weight must be 16-byte aligned");
+  if (a->rows > 1 && a->y_stride < a->out_cols) return fail(IKL_EINVAL, "int4 linear: rows of y must not overlap");
   if (((uintptr_t)a->y | (uintptr_t)a->residual) & (uintptr_t)(eb - 1))
     return fail(IKL_EINVAL, "int4 linear: y and residual must be aligned to their elements");
   Int4Params p{};
@@ -155,7 +159,7 @@ extern "C" int ikl_int4_linear(const ikl_int4_linear_args *a, void *stream) {
   else launch_int4_f16(p, a->group, plan, s);
   if (plan.split > 1) {
     const int quads = 4 * (p.gated ? p.tiles / 2 : p.tiles);
-    int4_join_kernel<<<dim3((unsigned)((quads + 255) / 256), (unsigned)p.rows), 256, 0, s>>>(p, plan.split, quads);
+    int4_join_kernel<<<dim3((unsigned)((p.rows * quads + 255) / 256)), 256, 0, s>>>(p, plan.split, quads);
   }
   return check_launch("int4 linear");
 }

@@ -36,8 +36,9 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
   __shared__ __attribute__((aligned(16))) float red[ROW_WAVES][NT * MT][64][4];
   const int tid = threadIdx.x, lane = tid & 63, hl = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int tile0 = blockIdx.x * NT;
-  const int64_t row0 = (int64_t)blockIdx.y * (16 * MT);
+  const unsigned across = (unsigned)(p.tiles + NT - 1) / NT, down = blockIdx.x / across;
+  const int tile0 = (int)(blockIdx.x - down * across) * NT;
+  const int64_t row0 = (int64_t)down * (16 * MT);
   const char *xrow[MT];
   const float *xs[MT];
 #pragma unroll
@@ -244,11 +245,12 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
   __shared__ __attribute__((aligned(16))) char codes[NST][I8 ? 4 * WT * 1024 : 16];
   const int tid = threadIdx.x, lane = tid & 63, hl = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int tile0 = (blockIdx.x * 4 + wave) * WT;
-  const int64_t row0 = (int64_t)blockIdx.y * BM;
+  const unsigned across = (unsigned)(p.tiles + 4 * WT - 1) / (4 * WT), down = blockIdx.x / across;
+  const int tile0 = ((int)(blockIdx.x - down * across) * 4 + wave) * WT;
+  const int64_t row0 = (int64_t)down * BM;
   const int chunks = p.groups * (G * (I8 ? 1 : 2) / 16);  // of a row
-  const int s0 = split > 1 ? (int)((int64_t)blockIdx.z * p.steps / split) : 0;
-  const int s1 = split > 1 ? (int)((int64_t)(blockIdx.z + 1) * p.steps / split) : p.steps;
+  const int s0 = split > 1 ? (int)((int64_t)blockIdx.y * p.steps / split) : 0;
+  const int s1 = split > 1 ? (int)((int64_t)(blockIdx.y + 1) * p.steps / split) : p.steps;
 
   // This thread's chunk of its first row; its others are 256 / RC rows apart.
   // Rows past the last: the last again.
@@ -516,7 +518,7 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
       const float *at = mine + r * 16 * WT;
       const f32x4_t v = *reinterpret_cast<const f32x4_t *>(at + 4 * ((4 * n + (c & 3)) ^ (r % CHUNKS)));
       if (p.part) {
-        float *to = p.part + ((int64_t)blockIdx.z * p.rows + row) * 16 * p.tiles + 16 * (tile0 + n) + 4 * (c & 3);
+        float *to = p.part + ((int64_t)blockIdx.y * p.rows + row) * 16 * p.tiles + 16 * (tile0 + n) + 4 * (c & 3);
         *reinterpret_cast<f32x4_t *>(to) = v;
         continue;
       }
@@ -543,15 +545,12 @@ void launch_rows(const Int4Params &p, const Int4Plan &plan, dim3 grid, hipStream
   if (plan.mt == 1 && plan.nt == 1) int4_rows_kernel<XT, G, 1, 1, 4, Z><<<grid, wg, 0, s>>>(p);
   else if (plan.mt == 1 && plan.nt == 2) int4_rows_kernel<XT, G, 1, 2, 3, Z><<<grid, wg, 0, s>>>(p);
   else if (plan.mt == 1) int4_rows_kernel<XT, G, 1, 4, WIDE, Z><<<grid, wg, 0, s>>>(p);
-  else if (plan.mt == 2 && plan.nt == 2) int4_rows_kernel<XT, G, 2, 2, 2, Z><<<grid, wg, 0, s>>>(p);
-  else if (plan.mt == 2) int4_rows_kernel<XT, G, 2, 4, __is_same(XT, i8_tag) ? WIDE : 1, Z><<<grid, wg, 0, s>>>(p);
-  else int4_rows_kernel<XT, G, 4, 2, 1, Z><<<grid, wg, 0, s>>>(p);
+  else int4_rows_kernel<XT, G, 2, 4, __is_same(XT, i8_tag) ? WIDE : 1, Z><<<grid, wg, 0, s>>>(p);
 }
 
 template <typename XT, int G, bool Z>
 void launch(const Int4Params &p, const Int4Plan &plan, hipStream_t s) {
-  const dim3 grid((unsigned)((p.tiles + plan.nt - 1) / plan.nt), (unsigned)((p.rows + 16 * plan.mt - 1) / (16 * plan.mt)),
-                  (unsigned)plan.split);
+  const dim3 grid((unsigned)(plan.blocks), (unsigned)plan.split);
   if (plan.few) launch_rows<XT, G, Z>(p, plan, grid, s);
   else launch_tiles<XT, G, Z>(p, plan, grid, s);
 }

@@ -73,6 +73,18 @@ def _check_like(x: torch.Tensor, y, name: str, shape=None) -> None:
         raise ValueError(f"{name} must have the rows' dtype and device")
 
 
+def _apart(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether no byte of the rows [rows, columns] of `x` is one of `y`'s."""
+    if not x.numel() or not y.numel():
+        return True
+    (x0, xs, xw), (y0, ys, yw) = ((t.data_ptr(), t.stride(0) * t.element_size(), t.shape[1] * t.element_size())
+                                  for t in (x, y))
+    if x0 + xs * (x.shape[0] - 1) + xw <= y0 or y0 + ys * (y.shape[0] - 1) + yw <= x0:
+        return True
+    # column ranges of one buffer
+    return xs == ys > 0 and xw <= (y0 - x0) % xs <= xs - yw
+
+
 # ------------------------------------------------------------- rows in 8 bits
 class Int8Rows:
     """Rows in 8 bits: ``codes`` ``[..., columns]`` int8, ``scales``
@@ -373,8 +385,11 @@ def quantize_int4_weight(weight: torch.Tensor, *, group_size: int = 128, symmetr
     else:
         low = w.amin(-1).clamp(max=0)
         span = (w.amax(-1).clamp(min=0) - low) / 15
-    # at least the dtype's smallest normal number: a zero group divides by it
-    scales = span.to(weight.dtype).clamp(min=torch.finfo(weight.dtype).tiny)
+    # A zero group divides by its step too. A step below fp16's normal numbers may
+    # have been rounded down by more than the codes' range has to spare.
+    least = torch.finfo(weight.dtype).smallest_normal if weight.dtype != torch.float16 else 2.0 ** -24
+    scales = span.to(weight.dtype).clamp(min=least)
+    scales = torch.where(scales.float() * (1 + 2.0 ** -6) < span, scales * 2, scales)
     step = scales.float()
     zeros = None if low is None else (-low / step).round_().clamp_(0, 15)
     codes = (w / step[..., None] + (8.0 if zeros is None else zeros[..., None])).round_().clamp_(0, 15)
@@ -394,7 +409,7 @@ class PreparedInt4Linear(_Prepared):
         lib = _require_backend()
         if not isinstance(weight, Int4Weight):
             raise ValueError("weight must be an Int4Weight")
-        a = _lib.Int4LinearArgs()
+        a, scales = _lib.Int4LinearArgs(), None
         if isinstance(x, Int8Rows):
             if x.group_size != weight.group_size:
                 raise ValueError("rows and weight must have the same group_size")
@@ -402,25 +417,28 @@ class PreparedInt4Linear(_Prepared):
             if flat.device.type != "cuda":
                 raise ValueError("rows must be on a GPU (torch 'cuda' device)")
             a.x_scales = x.scales.data_ptr()
-            rows = flat.numel() // flat.shape[-1]
+            flat, scales = flat.view(-1, flat.shape[-1]), x.scales.view(-1, x.scales.shape[-1])
         else:
             if x.dtype not in (torch.float16, torch.bfloat16):
                 raise ValueError("rows must be float16, bfloat16 or Int8Rows")
             flat = _rows_of(x, "rows")
             a.x_stride = flat.stride(0)
-            rows = flat.shape[0]
         if x.shape[-1] != weight.in_features:
             raise ValueError(f"rows have {x.shape[-1]} columns, the weight takes {weight.in_features}")
         if weight.device != x.device:
             raise ValueError("weight must be on the rows' device")
-        shape = (*x.shape[:-1], weight.out_features)
+        shape, given = (*x.shape[:-1], weight.out_features), out is not None
         if out is None:
             out = torch.empty(shape, dtype=x.dtype, device=x.device)
         elif out.shape != shape or out.dtype != x.dtype or out.device != x.device:
             raise ValueError(f"out must have shape {shape} and the rows' dtype and device")
+        if out.ndim != 2 and not out.is_contiguous():
+            raise ValueError("out of more than two dimensions must be contiguous")
         y = out if out.ndim == 2 else out.view(-1, weight.out_features)
         if y.shape[1] > 1 and y.stride(1) != 1:
             raise ValueError("out must be contiguous in its rows")
+        if given and not (_apart(flat, y) and (scales is None or _apart(scales, y))):
+            raise ValueError("out must not share memory with the rows")
         a.x, a.y, a.y_stride = flat.data_ptr(), y.data_ptr(), y.stride(0)
         keep = [flat, None, weight, x]
         if residual is not None:
@@ -431,10 +449,13 @@ class PreparedInt4Linear(_Prepared):
             keep[1] = r = residual if residual.ndim == 2 else residual.reshape(y.shape)
             if r.shape[1] > 1 and r.stride(1) != 1:
                 keep[1] = r = r.contiguous()
+            same = r.data_ptr() == y.data_ptr() and r.stride(0) == y.stride(0)
+            if given and not same and not _apart(r, y):
+                raise ValueError("out must be the residual or share no memory with it")
             a.residual, a.residual_stride = r.data_ptr(), r.stride(0)
         a.codes, a.scales = weight.codes.data_ptr(), weight.scales.data_ptr()
         a.zeros = None if weight.zeros is None else weight.zeros.data_ptr()
-        a.rows, a.cols, a.out_cols = rows, weight.in_features, weight.out_features
+        a.rows, a.cols, a.out_cols = flat.shape[0], weight.in_features, weight.out_features
         a.group, a.gated, a.dtype = weight.group_size, weight.gated, _DTYPES[x.dtype]
         size = lib.ikl_int4_linear_workspace_size(ctypes.byref(a))
         if size:

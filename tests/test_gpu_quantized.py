@@ -133,6 +133,60 @@ def test_linear_of_8_bit_rows(dtype, group, cols, zeros):
                 _assert_close(int4_linear_hip(x, packed, residual=res), want, bound)
 
 
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("rows,outs,cols,group", [
+    (16, 20000, 256, 64), (30, 9000, 384, 32), (130, 2070, 384, 128), (300, 2064, 640, 64), (100, 9000, 416, 32),
+    (140, 4112, 3456, 128), (520, 2064, 3456, 64), (2050, 1040, 3456, 128), (520, 9000, 1408, 128),
+    (700, 9000, 1376, 32), (6200, 5000, 320, 64), (6200, 4998, 384, 128)])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_larger_products(rows, outs, cols, group, zeros, eight):
+    """Every form of a launch: blocks of 16 to 128 rows and 16 to 256 columns,
+    contractions in one part and in several."""
+    from inferkernellab_amd import int4_linear_hip, quantize_rows_int8_hip
+
+    gen = _gen(rows + outs)
+    gated = zeros and not eight
+    packed, w, mag = _weight(gen, outs, cols, group, zeros=zeros, gated=gated)
+    x = torch.randn(rows, cols, generator=gen, device="cuda").to(BF16)
+    res = None if gated else torch.randn(rows, outs, generator=gen, device="cuda").to(BF16)
+    if eight:
+        x = quantize_rows_int8_hip(x, group_size=group)
+        xd = (x.codes.double().view(rows, -1, group) * x.scales.double()[..., None]).view(rows, cols)
+        sums = _sums8(x.codes, x.scales, w, group)
+    else:
+        xd = x.double()
+        sums = _sums16(xd, mag, group)
+    want, bound = _expected(xd, w, sums, res, gated, BF16)
+    y = int4_linear_hip(x, packed, residual=res)
+    _assert_close(y, want, bound)
+    assert torch.equal(int4_linear_hip(x, packed, residual=res), y)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("rows,cols", [(70000, 8192), (2200000, 32)])
+def test_more_rows_than_a_grids_second_dimension_holds(rows, cols, eight):
+    from inferkernellab_amd import int4_linear_hip, quantize_rows_int8_hip
+
+    gen = _gen(11)
+    packed, w, mag = _weight(gen, 16, cols, 32, zeros=False)
+    x = torch.randn(rows, cols, generator=gen, device="cuda", dtype=BF16)
+    given = quantize_rows_int8_hip(x, group_size=32) if eight else x
+    y = int4_linear_hip(given, packed)
+    part = slice(rows - 999, rows)  # and the rows before by themselves
+    few = quantize_rows_int8_hip(x[part], group_size=32) if eight else x[part]
+    xd = few.dequantize(FP32).double() if eight else few.double()
+    # dequantised to fp32: half a step of each product more
+    sums = _sums16(xd, mag, 32)
+    want, bound = _expected(xd, w, sums, None, False, BF16)
+    _assert_close(y[part], want, bound)
+    for start in range(0, rows - 64, rows // 7):
+        some = x[start:start + 64]
+        if eight:
+            some = quantize_rows_int8_hip(some, group_size=32).dequantize(FP32)
+        want, bound = _expected(some.double(), w, _sums16(some.double(), mag, 32), None, False, BF16)
+        _assert_close(y[start:start + 64], want, bound)
+
+
 @pytest.mark.parametrize("rows", [3, 40, 200])
 @pytest.mark.parametrize("eight", [False, True])
 def test_nothing_outside_the_result_is_written(rows, eight):
@@ -340,6 +394,58 @@ def _launches(gen, rows):
         (ikl.PreparedSiluMulInt8(x, delta, group_size=32), lambda: ikl.silu_mul_int8_hip(x, delta, group_size=32)),
         (ikl.PreparedAddRMSNormInt8(x, delta, norm), lambda: ikl.add_rms_norm_int8_hip(x, delta, norm)),
     ]
+
+
+@pytest.mark.parametrize("rows", [40, 600])
+def test_captured_eager_calls_hold_their_workspaces(rows):
+    """Calls that split the contraction, in two graphs, replayed in turn with
+    eager calls between."""
+    import inferkernellab_amd as ikl
+
+    gen = _gen(rows)
+    packed, _, _ = _weight(gen, 2064, 3456, 64, zeros=True)
+    x = torch.randn(rows, 3456, generator=gen, device="cuda").to(BF16)
+    graphs = []
+    ikl.int4_linear_hip(ikl.quantize_rows_int8_hip(x, group_size=64), packed)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            q = ikl.quantize_rows_int8_hip(x, group_size=64)
+            out = ikl.int4_linear_hip(x, packed), ikl.int4_linear_hip(q, packed)
+        graphs.append((g, out))
+    for _ in range(3):
+        x.copy_(torch.randn(rows, 3456, generator=gen, device="cuda"))
+        for g, out in graphs:
+            g.replay()
+            want = ikl.int4_linear_hip(x, packed), ikl.int4_linear_hip(ikl.quantize_rows_int8_hip(x, group_size=64),
+                                                                       packed)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_results_that_share_memory_are_refused():
+    from inferkernellab_amd import Int8Rows, int4_linear_hip
+
+    packed, _, _ = _weight(_gen(1), 128, 128, 64, zeros=False)
+    wide = torch.randn(5, 256, device="cuda").to(BF16)
+    x = wide[:, :128]
+    apart = int4_linear_hip(x, packed, out=wide[:, 128:])  # columns beside the rows
+    assert torch.equal(apart, int4_linear_hip(x, packed))
+    for out in (x, wide[:, 64:192]):
+        with pytest.raises(ValueError, match="share"):
+            int4_linear_hip(x, packed, out=out)
+    other = torch.randn(5, 128, device="cuda").to(BF16)
+    with pytest.raises(ValueError, match="residual"):
+        int4_linear_hip(other, packed, residual=wide[:, :128], out=wide[:, 8:136])
+    flat = torch.zeros(20 * 128, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        int4_linear_hip(other, packed, out=flat.as_strided((5, 128), (64, 1)))
+    codes = torch.zeros(5, 128, dtype=torch.int8, device="cuda")
+    rows = Int8Rows(codes, torch.ones(5, 2, device="cuda"), 64, dtype=BF16)
+    half, _, _ = _weight(_gen(1), 64, 128, 64, zeros=False)
+    with pytest.raises(ValueError, match="share"):
+        int4_linear_hip(rows, half, out=codes.view(BF16))
 
 
 def _parts(result):
