@@ -412,12 +412,22 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
       }
       const char *xrow = mem + b * (BM * RB) + hl * RB;
       if constexpr (!I8) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          v4u32 xv[DPG];
+        // The next tile's rows are read ahead where the registers hold them.
+        constexpr bool AHEAD = MT <= 4;
+        v4u32 ahead[DPG];
+        auto read = [&](int m) {
 #pragma unroll
           for (int i = 0; i < DPG; ++i)
-            xv[i] = *reinterpret_cast<const v4u32 *>(xrow + 16 * m * RB + 16 * ((dword_k<G>(g * DPG + i, q) / 8) ^ (hl & 7)));
+            ahead[i] = *reinterpret_cast<const v4u32 *>(xrow + 16 * m * RB + 16 * ((dword_k<G>(g * DPG + i, q) / 8) ^ (hl & 7)));
+        };
+        if (AHEAD) read(0);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if (!AHEAD) read(m);
+          v4u32 xv[DPG];
+#pragma unroll
+          for (int i = 0; i < DPG; ++i) xv[i] = ahead[i];
+          if (AHEAD && m + 1 < MT) read(m + 1);
           f32x4_t X = {0.f, 0.f, 0.f, 0.f};
           if constexpr (!LESS) {
             const v4u32 ones = {mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2};
@@ -509,10 +519,12 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
     for (int n = 0; n < WT; ++n)
       *reinterpret_cast<f32x4_t *>(mine + hl * 16 * WT + 4 * ((4 * n + q) ^ (hl % CHUNKS))) = acc[n][m];
     wave_lds_sync();
-    const int units = (p.gated && !p.part) ? WT / 2 : WT;  // results of 16 columns
-#pragma unroll 1
-    for (int i = lane; i < 16 * 4 * units; i += 64) {
-      const int r = i / (4 * units), c = i % (4 * units), n = c / 4 * (WT / units);
+    const bool paired = p.gated && !p.part;
+    const int units = paired ? WT / 2 : WT, shift = (WT == 4 ? 4 : 3) - paired;  // results of 16 columns; 4 units = 1 << shift
+#pragma unroll
+    for (int k = 0; k < WT; ++k) {  // 64 lanes: 4 WT / 4 of the tile's quads of columns
+      if (k >= units) break;
+      const int i = lane + 64 * k, r = i >> shift, c = i & ((1 << shift) - 1), n = (c >> 2) * (WT / units);
       const int64_t row = row0 + 16 * m + r;
       if (row >= p.rows || n >= tiles) continue;
       const float *at = mine + r * 16 * WT;
@@ -523,7 +535,8 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
         continue;
       }
       const int col = tile_col(p, tile0 + n, c & 3);
-      if (col < p.outs) finish(p, row, col, p.gated ? gate_up(v, *reinterpret_cast<const f32x4_t *>(at + 4 * ((4 * n + 4 + (c & 3)) ^ (r % CHUNKS)))) : v);
+      if (col < p.outs)
+        finish(p, row, col, p.gated ? gate_up(v, *reinterpret_cast<const f32x4_t *>(at + 4 * ((4 * n + 4 + (c & 3)) ^ (r % CHUNKS)))) : v);
     }
     wave_lds_sync();
   }
