@@ -14,7 +14,7 @@
 namespace ikl {
 namespace {
 
-constexpr uint32_t LEAST_AMAX = 0x0d800000u;  // 2^-100: 127 / amax stays finite
+constexpr float LEAST_AMAX = 0x1p-100f;  // 127 / amax stays finite
 
 // The 16-byte piece of a row that a lane holds, widened.
 template <typename Tag>
@@ -66,21 +66,26 @@ __device__ inline uint32_t group_max(uint32_t v) {
   return v;
 }
 
-// Codes and scale of the N values that this lane holds of its group. Adding
-// 1.5 * 2^23 rounds to the nearest whole number, ties to even, and leaves it
-// in the low bits. 16-bit values meet ties often (a value and the largest one
-// have few bits, so 127 v / amax is a half exactly): EXACT takes the quotient
-// to its correct rounding, by its remainder, where one multiplication would
-// put them on either side.
-template <int N, int LANES, bool EXACT>
-__device__ inline float quantize(const float *v, uint32_t *codes) {
-  uint32_t amax = LEAST_AMAX;
+// Largest magnitude of the group that this lane holds N values of.
+template <int N, int LANES>
+__device__ inline float group_amax(const float *v) {
+  uint32_t amax = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
     amax = amax > b ? amax : b;
   }
-  const float most = __uint_as_float(group_max<LANES>(amax));
+  return __uint_as_float(group_max<LANES>(amax));
+}
+
+// Codes of this lane's N values, whose group's largest magnitude is `most`.
+// Adding 1.5 * 2^23 rounds to the nearest whole number, ties to even, and
+// leaves it in the low bits. 16-bit values meet ties often (a value and the
+// largest one have few bits, so 127 v / amax is a half exactly): EXACT takes
+// the quotient to its correct rounding, by its remainder, where one
+// multiplication would put them on either side.
+template <int N, bool EXACT>
+__device__ inline void codes_of(const float *v, float most, uint32_t *codes) {
   const float part = most * 0x1p-7f, inv = EXACT ? 1.f / part : 127.f / most;
 #pragma unroll
   for (int j = 0; j < N / 4; ++j) {
@@ -97,8 +102,10 @@ __device__ inline float quantize(const float *v, uint32_t *codes) {
     const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
     codes[j] = lo | hi;
   }
-  return most / 127.f;
 }
+
+// max(most, 2^-100), a NaN kept.
+__device__ inline float at_least(float most) { return most < LEAST_AMAX ? LEAST_AMAX : most; }
 
 template <int N>
 __device__ inline void store_codes(char *p, const uint32_t *codes) {
@@ -133,9 +140,10 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const RowsParams p) 
     for (int e = 0; e < N; ++e) v[e] = silu_fast(v[e]) * u[e];
   }
   uint32_t codes[N / 4];
-  const float scale = quantize<N, LANES, !SILU>(v, codes);
+  const float most = at_least(group_amax<N, LANES>(v));
+  codes_of<N, !SILU>(v, most, codes);
   store_codes<N>(p.codes + (int64_t)N * i, codes);
-  if (i % LANES == 0) p.scales[i / LANES] = scale;
+  if (i % LANES == 0) p.scales[i / LANES] = most / 127.f;
 }
 
 struct NormParams {
@@ -192,9 +200,20 @@ __global__ __launch_bounds__(256) void norm_int8_kernel(const NormParams p) {
     piece<Tag>::get(v[u], a);
     piece<Tag>::get(load16v_global(p.weight + 16 * (int64_t)c), w);
 #pragma unroll
-    for (int e = 0; e < N; ++e) a[e] = a[e] * r * w[e];
+    for (int e = 0; e < N; ++e) a[e] *= w[e];
+    // The codes do not depend on r: they are those of x * weight, exact where
+    // both have 16 bits. Magnitudes near the least take r first.
+    const float product = group_amax<N, LANES>(a);
+    const bool first = !(product >= LEAST_AMAX && product * r >= LEAST_AMAX);
+    float most = product;
+    if (first) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) a[e] *= r;
+      most = at_least(product * r);
+    }
     uint32_t codes[N / 4];
-    const float scale = quantize<N, LANES, false>(a, codes);
+    codes_of<N, true>(a, most, codes);
+    const float scale = (first ? most : most * r) / 127.f;
     const int64_t at = row * p.pieces + c;
     store_codes<N>(p.codes + N * at, codes);
     if (c % LANES == 0) p.scales[at / LANES] = scale;

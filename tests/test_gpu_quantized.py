@@ -304,6 +304,44 @@ def test_norm_in_8_bits(dtype, group, add):
         _check_codes(got, v, (128 + 10) / 2 * 2.0**-24 + U + 2 * 2.0**-24, dtype)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_codes_of_normalised_16_bit_rows_are_the_nearest(dtype):
+    """They depend on x times weight alone, exact in fp32; fp16's quotient by
+    127 / amax is rounded once, 2^-16 of a step."""
+    from inferkernellab_amd import add_rms_norm_int8_hip
+
+    gen = _gen(6)
+    x = torch.randn(513, 2048, generator=gen, device="cuda").to(dtype)
+    w = (1 + 0.1 * torch.randn(2048, generator=gen, device="cuda")).to(dtype)
+    _, got = add_rms_norm_int8_hip(x, None, w, group_size=32)
+    g = (x.double() * w.double()).view(513, -1, 32)
+    share = g * 127 / g.abs().amax(-1, keepdim=True)
+    off = (got.codes.view_as(share).double() - share).abs()
+    assert float(off.max()) <= 0.5 + (0 if dtype == BF16 else 2.0**-16)
+
+
+def test_norms_of_rows_near_the_ends_of_fp32():
+    """Groups far below their row, rows whose squares overflow (their norm is 0
+    in fp32 arithmetic) and rows of zeros."""
+    from inferkernellab_amd import add_rms_norm_int8_hip
+
+    x = torch.zeros(5, 256, device="cuda")
+    x[0, :128] = torch.linspace(-1e15, 1e15, 128, device="cuda")
+    x[0, 128:] = torch.linspace(-1e-20, 1e-20, 128, device="cuda")
+    x[1] = 1e30
+    x[2] = torch.linspace(-1e-30, 1e-30, 256, device="cuda")
+    x[3, 7] = float("nan")
+    w = torch.ones(256, device="cuda")
+    _, got = add_rms_norm_int8_hip(x, None, w, eps=1e-6)
+    keep = torch.tensor([0, 2, 4], device="cuda")
+    t = x[keep].double()
+    v = t * torch.rsqrt(t.square().mean(-1, keepdim=True) + 1e-6)
+    from inferkernellab_amd import Int8Rows
+    _check_codes(Int8Rows(got.codes[keep], got.scales[keep], 128, dtype=FP32), v, 74 * 2.0**-24 + U, FP32)
+    values = got.dequantize()
+    assert bool((values[1] == 0).all()) and bool(values[3].isnan().all())
+
+
 def test_values_near_the_ends_of_fp32_keep_their_codes():
     from inferkernellab_amd import quantize_rows_int8_hip
 
