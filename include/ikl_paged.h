@@ -9,7 +9,8 @@
  *     log-sum-exp reduce kernel.
  * Around them: the rotary append (with norms of the heads where a model has
  * them), paged prefill attention, a whole decode step, copies of pages, the
- * drawing of tokens and a Llama layer's small kernels.
+ * drawing of tokens, a Llama layer's small kernels, and its quantised ones:
+ * rows in 8 bits and products with 4-bit weights.
  *
  * Conventions
  *   - Every pointer is a device pointer (HBM) except the argument structs

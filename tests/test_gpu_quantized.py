@@ -6,8 +6,10 @@ addition rounded or cut to 24 bits, is off by at most (n - 1) 2^-23 of the
 terms' magnitudes. 16-bit rows: a group's sum of x c and of x z, G terms each,
 scaled and added to the other groups' (two more operations a group, and the
 eight waves' sums): 2^-23 (G + 2 groups + 8) sum |x| s (c + z). 8-bit rows: the
-group's sum is exact, its scales' product and their product with it round, then
-the groups' sum: 2^-23 (groups + 2 + 8) sum over groups |s a P|. Codes: what
+group's sum P is exact, a is cut to 22 bits (3 2^-23 at most), a P rounds (half a
+2^-23), then the multiply-adds with s over the groups and the eight waves' sums
+(half each): 7.5 + groups / 2 of 2^-23, inside 2^-23 (groups + 2 + 8) sum over
+groups |s a P|. Codes: what
 they are rounded from is off by 127 times its relative error, in steps."""
 
 import pytest
