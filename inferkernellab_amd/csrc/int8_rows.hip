@@ -205,14 +205,15 @@ __global__ __launch_bounds__(256) void norm_int8_kernel(const NormParams p) {
 #pragma unroll
     for (int e = 0; e < N; ++e) a[e] *= w[e];
     // The codes do not depend on r: they are those of x * weight, exact where
-    // both have 16 bits. Magnitudes near the least take r first.
-    const float product = group_amax<N, LANES>(a);
-    const bool first = !(product >= LEAST_AMAX && product * r >= LEAST_AMAX);
-    float most = product;
+    // both have 16 bits. Where that, or its largest value by r, is near the
+    // least or past fp32, they are those of x * r * weight.
+    float most = group_amax<N, LANES>(a);
+    const bool first = !(most >= LEAST_AMAX && most * r >= LEAST_AMAX && most < INFINITY && most * r < INFINITY);
     if (first) {
+      piece<Tag>::get(v[u], a);
 #pragma unroll
-      for (int e = 0; e < N; ++e) a[e] *= r;
-      most = at_least(product * r);
+      for (int e = 0; e < N; ++e) a[e] = a[e] * r * w[e];
+      most = at_least(group_amax<N, LANES>(a));
     }
     uint32_t codes[N / 4];
     codes_of<N, true>(a, most, codes);

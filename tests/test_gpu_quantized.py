@@ -344,6 +344,37 @@ def test_norms_of_rows_near_the_ends_of_fp32():
     assert bool((values[1] == 0).all()) and bool(values[3].isnan().all())
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_norms_whose_products_without_the_rows_factor_leave_fp32(dtype):
+    """x times weight past fp32's largest value or below its normal ones, their
+    norms inside."""
+    from inferkernellab_amd import add_rms_norm_int8_hip
+
+    for size, gain in ((2.0**14, 2.0**119), (2.0**-60, 2.0**-80)):
+        gen = _gen(9)
+        x = (torch.randn(7, 256, generator=gen, device="cuda") * size).to(dtype)
+        w = torch.ones(256, device="cuda")
+        w[128:] = gain * (1 + torch.rand(128, generator=gen, device="cuda"))
+        _, got = add_rms_norm_int8_hip(x, None, w.to(dtype), eps=0.0)
+        t = x.double()
+        v = t * torch.rsqrt(t.square().mean(-1, keepdim=True)) * w.to(dtype).double()
+        assert float(v.abs().max()) < torch.finfo(dtype).max
+        # as in test_norm_in_8_bits, of 256 columns: up to 8 squares a thread
+        _check_codes(got, v, (8 + 10) / 2 * 2.0**-24 + U + 2 * 2.0**-24, dtype)
+
+
+def test_norms_past_fp32_stand_for_nan():
+    from inferkernellab_amd import add_rms_norm_int8_hip
+
+    x = torch.ones(1, 256, device="cuda")
+    x[0, 0] = 8.0  # its norm is 7.2 or so
+    w = torch.ones(256, device="cuda")
+    w[:128] = 2.0**126
+    _, got = add_rms_norm_int8_hip(x, None, w, eps=0.0)
+    values = got.dequantize()
+    assert bool(values[0, :128].isnan().all()) and bool(values[0, 128:].isfinite().all())
+
+
 def test_values_near_the_ends_of_fp32_keep_their_codes():
     from inferkernellab_amd import quantize_rows_int8_hip
 
