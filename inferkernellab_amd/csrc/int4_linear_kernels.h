@@ -216,6 +216,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
 // the scales and 64 matrix instructions are 320 of 427 slots. 8192 x 4096 to
 // 14336: 8-bit rows 567-608 us (1.6-1.7 POP/s; a library's int8 product 2.0 at
 // 8192^3), bf16 rows 930 us (1.03 PFLOP/s).
+constexpr int VMCNT_0 = 0x0f70;  // s_waitcnt of vmcnt alone: its bits are 0-3 and 14-15
 typedef const __attribute__((address_space(1))) void *global_ptr;
 typedef __attribute__((address_space(3))) void *lds_ptr;
 
@@ -362,6 +363,8 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
   if constexpr (!I8) codes_ahead(s0, 0);
   fetch(s0);
   put(0);
+  // A barrier waits for LDS, not for loads that write it: their waits are here.
+  __builtin_amdgcn_s_waitcnt(VMCNT_0);
   __syncthreads();
   int b = 0;  // s's buffer of rows and codes
   for (int s = s0; s < s1; ++s) {
@@ -508,15 +511,18 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
     }
     put(sb ^ 1);
     // step s + 1's rows and codes are there when no more is on its way than
-    // what was asked for after them (vmcnt of s_waitcnt: bits 0-3 and 14-15)
+    // what was asked for after them
     constexpr int LATER = (NST - 2) * FLIGHT;
-    __builtin_amdgcn_s_waitcnt(0x0f70 | (LATER & 15) | (LATER >> 4) << 14);
+    __builtin_amdgcn_s_waitcnt(VMCNT_0 | (LATER & 15) | (LATER >> 4) << 14);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
     b = b + 1 == NST ? 0 : b + 1;
   }
-  if constexpr (NST > 2) __syncthreads();  // the last loads write where the tail does
+  if constexpr (NST > 2) {  // the last step's loads write where the tail does
+    __builtin_amdgcn_s_waitcnt(VMCNT_0);
+    __syncthreads();
+  }
   // Through LDS, so that a row's columns leave side by side
   float *mine = reinterpret_cast<float *>(mem) + wave * 16 * 16 * WT;
   constexpr int CHUNKS = 4 * WT;  // of four columns, exchanged by row as the rows' are

@@ -165,6 +165,29 @@ def test_larger_products(rows, outs, cols, group, zeros, eight):
 
 
 @pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("cols", [128, 256, 384, 512])
+@pytest.mark.parametrize("rows", [300, 1900])
+def test_short_contractions_over_many_rows(rows, cols, eight):
+    """A workgroup's results pass through the memory that its last rows came
+    into: each of many launches gives the same."""
+    from inferkernellab_amd import int4_linear_hip, quantize_rows_int8_hip
+
+    gen = _gen(cols + rows)
+    packed, w, mag = _weight(gen, 4000, cols, 128, zeros=eight)
+    x = torch.randn(rows, cols, generator=gen, device="cuda").to(BF16)
+    q = quantize_rows_int8_hip(x)
+    if eight:
+        scales = q.scales.double().repeat_interleave(128, 1)
+        xd, sums = q.codes.double() * scales, _sums8(q.codes, q.scales, w, 128)
+    else:
+        xd, sums = x.double(), _sums16(x.double(), mag, 128)
+    first = int4_linear_hip(q if eight else x, packed)
+    _assert_close(first, *_expected(xd, w, sums, None, False, BF16))
+    for _ in range(20):
+        assert torch.equal(int4_linear_hip(q if eight else x, packed), first)
+
+
+@pytest.mark.parametrize("eight", [False, True])
 @pytest.mark.parametrize("rows,cols", [(70000, 8192), (2200000, 32)])
 def test_more_rows_than_a_grids_second_dimension_holds(rows, cols, eight):
     from inferkernellab_amd import int4_linear_hip, quantize_rows_int8_hip
