@@ -64,13 +64,13 @@ typedef int i32x4_t __attribute__((ext_vector_type(4)));
 // conversion. What turns it into its share of y are two multiply-adds: first
 // times a of its row less MAGIC times a, which is exact because a is held to
 // 22 significant bits (less than 2^-21 of it lost, as in four fp32 operations),
-// then times s of its column. a carries 2^-16 and s 2^16 (without zero points
-// 2^12), so that MAGIC * a stays finite for rows up to 2^127.
+// then times s of its column. a carries 2^-17 and s 2^17 (without zero points
+// 2^13), so that MAGIC * a stays finite up to fp32's largest value over 127.
 constexpr int MAGIC = 0x4b400000;
 template <bool Z>
-constexpr float S_CARRIES = Z ? 65536.f : 4096.f;
+constexpr float S_CARRIES = Z ? 0x1p17f : 0x1p13f;
 __device__ inline f32x2_t row_scale(float a) {
-  a = __uint_as_float(__float_as_uint(a) & ~3u) * 0x1p-16f;
+  a = __uint_as_float(__float_as_uint(a) & ~3u) * 0x1p-17f;
   return f32x2_t{a, a * -12582912.f};
 }
 

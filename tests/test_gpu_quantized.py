@@ -164,6 +164,23 @@ def test_larger_products(rows, outs, cols, group, zeros, eight):
     assert torch.equal(int4_linear_hip(x, packed, residual=res), y)
 
 
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_rows_in_8_bits_up_to_the_largest_values(rows, zeros):
+    """Whose products are finite."""
+    from inferkernellab_amd import int4_linear_hip, quantize_rows_int8_hip
+
+    gen = _gen(rows)
+    packed, w, _ = _weight(gen, 80, 256, 128, zeros=zeros)
+    packed.scales.mul_(2.0**-16)
+    w = w * 2.0**-16
+    x = torch.randn(rows, 256, generator=gen, device="cuda").clamp(-1, 1) * 2.0**127
+    x[:, :2] = torch.finfo(FP32).max
+    q = quantize_rows_int8_hip(x)
+    xd = q.codes.double() * q.scales.double().repeat_interleave(128, 1)
+    _assert_close(int4_linear_hip(q, packed), *_expected(xd, w, _sums8(q.codes, q.scales, w, 128), None, False, FP32))
+
+
 @pytest.mark.parametrize("eight", [False, True])
 @pytest.mark.parametrize("cols", [128, 256, 384, 512])
 @pytest.mark.parametrize("rows", [300, 1900])
