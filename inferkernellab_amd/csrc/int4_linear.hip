@@ -31,27 +31,33 @@ int64_t blocks_of(int64_t rows, int tiles, int mt, int nt) {
 // tile and the fewest column tiles that do, else of two row tiles. us of bf16
 // rows, weights from memory, by 1 / 2 / 4 column tiles: 16 x 4096 x 4096 7.0 /
 // 7.5 / 9.1; 2048 columns from 5632 7.9 / 9.1 / 10.8; 14336 from 4096 21 / 13 /
-// 9.9. Against the many rows' kernel: 64 x 4096 x 4096 9.2 and 13.0; 1024 x 4096
-// x 256 9.3 and 13.1; 128 x 4096 x 4096 by two row tiles 14.8 and 16.3. 8-bit
-// rows of short contractions stay ahead to three rounds of workgroups: 300 x
-// 2048 x 2048 12.1 and 15.4 (16-bit ones 15.5 and 13.7).
+// 9.9. Against the many rows' kernel: 64 x 4096 x 4096 9.9 and 13.4; 128 x 4096 x
+// 4096 by two row tiles 15.1 and 16.6. A CU's eight waves alone keep up with a
+// split contraction to 112 steps (64 x 14336 x 4096 23.7 and 25.9, 64 x 28672 x
+// 4096 46 and 37), two row tiles of 16-bit rows to 56 (100 x 8192 x 4096 24.3 and
+// 22.5; 8-bit ones 19.2 and 21.0, at 28672 55 and 46).
 bool few_rows(int64_t rows, int tiles, int steps, bool gated, bool eight, Int4Plan &plan) {
   auto take = [&](int mt, int nt, int64_t most) {
     const int64_t blocks = blocks_of(rows, tiles, mt, nt);
     plan = {true, mt, nt, 1, blocks};
     return blocks <= most;
   };
-  for (int nt = gated ? 2 : 1; nt <= 4; nt *= 2)
-    if (take(1, nt, 256)) return true;
-  if (rows <= 16 || (eight && steps <= 16 && take(1, 4, 768))) return take(1, 4, INT64_MAX);
+  if (rows <= 16 || steps <= 112)
+    for (int nt = gated ? 2 : 1; nt <= 4; nt *= 2)
+      if (take(1, nt, 256)) return true;
+  if (rows <= 16) return true;
+  if (steps > (eight || rows <= 32 ? 112 : 56)) return false;
   return take(2, 4, rows <= 32 ? INT64_MAX : 256);
 }
 
 // Many rows: the cheapest by an estimate of what bounds a launch. A CU runs
-// `slots` workgroups of a form at once; a step of them takes the longer of one
-// workgroup's own time and of their tiles' work. A split contraction saves
-// steps and pays for a second launch and for the parts' way through memory.
-// Times in us from launches of 8192 and of 1024 rows of 4096, groups of 128.
+// `slots` workgroups of a form at once: a round of them takes `start`, and for
+// each step the longer of one workgroup's own time and of their tiles' work. A
+// split contraction saves steps and pays for a second launch and for the parts'
+// way through memory. Times in us, fitted to launches of 17 to 4096 rows by 512
+// to 28672 and 1024 to 14336 (groups of 128, zero points), of which each form and
+// split was measured: what is taken was 0.6 (16-bit rows) and 0.9 % (8-bit)
+// slower than the fastest in the mean.
 Int4Plan plan_of(int64_t rows, int tiles, int steps, bool gated, bool eight) {
   Int4Plan best{};
   if (few_rows(rows, tiles, steps, gated, eight, best)) return best;
@@ -59,10 +65,11 @@ Int4Plan plan_of(int64_t rows, int tiles, int steps, bool gated, bool eight) {
     int mt, nt, slots;
     double alone[2], tile[2];  // of a step: 16-bit rows, 8-bit rows
   };
-  static const Form forms[] = {{2, 8, 4, {0.8, 0.5}, {0.0255, 0.0172}},
-                               {4, 8, 3, {1.1, 0.75}, {0.0195, 0.0137}},
-                               {4, 16, 2, {1.8, 1.3}, {0.0185, 0.0125}},
-                               {8, 16, 2, {3.3, 2.0}, {0.0166, 0.0101}}};
+  static const Form forms[] = {{2, 8, 4, {0.9, 0.79}, {0.0242, 0.0157}},
+                               {4, 8, 3, {1.4, 0.88}, {0.019, 0.0123}},
+                               {4, 16, 2, {1.6, 1.1}, {0.0186, 0.012}},
+                               {8, 16, 2, {3.3, 1.7}, {0.0181, 0.0099}}};
+  const double start = eight ? 4 : 3.1, join = eight ? 5.1 : 3.3, bytes_a_us = eight ? 15e6 : 8.8e6;
   double least = 1e30;
   for (const Form &f : forms) {
     const int64_t blocks = blocks_of(rows, tiles, f.mt, f.nt);
@@ -72,9 +79,10 @@ Int4Plan plan_of(int64_t rows, int tiles, int steps, bool gated, bool eight) {
     };
     const int most = rows * tiles < 1 << 28 ? 16 : 1;  // the join's launch holds that many
     for (int split = 1; split <= most && (split == 1 || 2 * split <= steps); ++split) {
-      const int64_t per_cu = (blocks * split + 255) / 256;
-      double us = ((per_cu / f.slots) * step(f.slots) + step((int)(per_cu % f.slots))) * ((steps + split - 1) / split);
-      if (split > 1) us += 2.5 + split * (double)rows * tiles * 16 * 8 / 6e6;
+      const int64_t per_cu = (blocks * split + 255) / 256, full = per_cu / f.slots;
+      const int rest = (int)(per_cu % f.slots);
+      double us = (full * step(f.slots) + step(rest)) * ((steps + split - 1) / split) + (full + (rest > 0)) * start;
+      if (split > 1) us += join + split * (double)rows * tiles * 16 * 8 / bytes_a_us;
       if (us < least) least = us, best = {false, f.mt, f.nt, split, blocks};
     }
   }
