@@ -57,7 +57,7 @@ bool few_rows(int64_t rows, int tiles, int steps, bool gated, bool eight, Int4Pl
 // way through memory. Times in us, fitted to launches of 17 to 4096 rows by 512
 // to 28672 and 1024 to 14336 (groups of 128, zero points), of which each form and
 // split was measured: what is taken was 0.6 (16-bit rows) and 0.9 % (8-bit)
-// slower than the fastest in the mean, 38 % at most (40 x 9000 x 1024).
+// slower than the fastest in the mean, 38 % at most (40 x 1024 x 9000).
 Int4Plan plan_of(int64_t rows, int tiles, int steps, bool gated, bool eight) {
   Int4Plan best{};
   if (few_rows(rows, tiles, steps, gated, eight, best)) return best;
