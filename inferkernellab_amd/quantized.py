@@ -358,10 +358,14 @@ def pack_int4_weight(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Ten
     else:  # [tile, row, step, dword / 2, q, dword % 2, half of byte, byte]
         c = c.view(-1, 16, steps, 2, 4, 2, 2, 4).permute(0, 2, 4, 1, 3, 5, 7, 6)
     c = (c[..., 0] | (c[..., 1] << 4)).reshape(parts * tiles, steps, 64, 16).contiguous()
-    s = tiled(scales.to(torch.float32).contiguous(), steps * per_step, 0.0).transpose(1, 2).contiguous()
-    z = None
-    if zeros is not None:
-        z = tiled(zeros.to(torch.uint8).contiguous(), steps * per_step, 8).transpose(1, 2).contiguous()
+
+    def laid_out(t, value):
+        # a clone: of a contraction of one step all that is before it may be the caller's own memory
+        return tiled(t.contiguous(), steps * per_step, value).transpose(1, 2).clone(
+            memory_format=torch.contiguous_format)
+
+    s = laid_out(scales.to(torch.float32), 0.0)
+    z = None if zeros is None else laid_out(zeros.to(torch.uint8), 8)
     dtype = scales.dtype if scales.dtype in _DTYPES else torch.float32
     return Int4Weight(c, s, z, out // parts, cols, group_size, gated, dtype)
 
