@@ -1,0 +1,97 @@
+"""The quantised operators over the whole range of their types: gates far from
+0, 16-bit rows up to their largest values, the mean of 8-bit rows' products.
+Against the definitions in 64 bits."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-23
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+GATES = [-87.0, -87.5, -88.0, -88.5, -90.0, -95.0, -100.0, -103.0, -104.0, -110.0, -1e4, -6e4, -0.0, 0.0, 1e-30, -1e-30,
+         0.5, -0.5, 17.0, -17.0, 87.0, 88.5, 110.0, 6e4]
+
+
+def _silu(x):
+    return x * torch.sigmoid(x)
+
+
+def _silu_bound(x, up):
+    """Of SiLU(x) * up in fp32: e^-|x| to an ulp and what its argument's two
+    products leave (a tenth of one), its sum with 1, the quotient and three
+    products (half an ulp each): 3.6 ulp. Below fp32's normal numbers e^-|x|,
+    its product with the quotient and SiLU are off by half of 2^-149 each, the
+    first two |x| times."""
+    return 3.6 * U * (_silu(x) * up).abs() + (x.abs() + 1) * 2.0**-149 * up.abs()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_silu_in_8_bits_of_gates_far_from_0(dtype):
+    """A group of equal values: its largest magnitude is any one's."""
+    from inferkernellab_amd import silu_mul_int8_hip
+
+    gates = GATES if dtype == FP16 else GATES + [-1e30, -3e38]
+    x = torch.tensor(gates, dtype=torch.float64).to(dtype).cuda().view(-1, 1).expand(-1, 64).contiguous()
+    for size in (1.0, 2.0**15 if dtype == FP16 else 2.0**100):
+        up = torch.full_like(x, size)
+        xd, ud = x.double(), up.double()
+        got = silu_mul_int8_hip(x, up, group_size=32)
+        stands = got.codes.double() * got.scales.double().repeat_interleave(32, 1)
+        want = _silu(xd) * ud
+        # the scale's rounding; values below half a step of the least scale are 0
+        bound = _silu_bound(xd, ud) * (1 + 2.0**-20) + U / 2 * want.abs() + torch.where(
+            want.abs() < 2.0**-100, 2.0**-100 / 254 * 1.01, 0.0)
+        over = (stands - want).abs() - bound
+        assert bool((over <= 0).all()), [(g, float(s[0]), float(w[0])) for g, s, w, o in zip(gates, stands, want, over)
+                                         if float(o.max()) > 0]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_silu_in_8_bits_of_gates_that_are_not_finite(dtype):
+    """SiLU of minus infinity is the product of an infinity and 0."""
+    from inferkernellab_amd import silu_mul_int8_hip
+
+    inf = float("inf")
+    x = torch.ones(4, 64, device="cuda").to(dtype)
+    x[0, 40], x[1, 40], x[2, 40] = inf, -inf, float("nan")
+    values = silu_mul_int8_hip(x, torch.ones_like(x), group_size=32).dequantize()
+    assert bool(values[:3, 32:].isnan().all()) and bool(values[:3, :32].isfinite().all())
+    assert bool(values[3].isfinite().all())
+
+
+@pytest.mark.parametrize("rows", [1, 400, 6200])
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "8 bits to bf16", "8 bits to fp32"])
+def test_gated_products_of_gates_far_from_0(kind, rows):
+    """Each row has a gate and an up value of its own: the weight takes them from
+    two entries of the contraction, in groups apart, times 1."""
+    from inferkernellab_amd import Int8Rows, int4_linear_hip, pack_int4_weight
+
+    outs, cols = (2048 if rows > 1000 else 40), 320
+    codes = torch.full((2 * outs, cols), 8, dtype=torch.uint8)
+    codes[:outs, 3], codes[outs:, 70] = 9, 9
+    packed = pack_int4_weight(codes.cuda(), torch.ones(2 * outs, cols // 64, device="cuda"), group_size=64, gated=True)
+    gates = torch.tensor(GATES if kind == "fp16" else GATES + [-1e30, 1e30], dtype=torch.float64)
+    dtype = {"fp16": FP16, "8 bits to fp32": FP32}.get(kind, BF16)
+    gate = gates[torch.arange(rows) % len(gates)].to(FP16 if kind == "fp16" else BF16).double().cuda()
+    sizes = (1.0, 0.75, 2.0**6) if kind == "fp16" else (1.0, 0.75, 2.0**100)
+    for size in sizes:
+        # (finite results)
+        up = torch.full_like(gate, size)
+        up = torch.where(gate.abs() * up > torch.finfo(dtype).max, 1.0, up)
+        if kind.startswith("8"):
+            q = torch.zeros(rows, cols, dtype=torch.int8, device="cuda")
+            q[:, 3], q[:, 70] = torch.where(gate < 0, -1, 1).to(torch.int8), 1
+            scales = torch.ones(rows, cols // 64, device="cuda")
+            scales[:, 0], scales[:, 1] = gate.abs(), up
+            x = Int8Rows(q, scales, 64, dtype=dtype)
+        else:
+            x = torch.zeros(rows, cols, dtype=dtype, device="cuda")
+            x[:, 3], x[:, 70] = gate.to(dtype), up.to(dtype)
+        y = int4_linear_hip(x, packed).double()
+        want = _silu(gate) * up
+        f = torch.finfo(dtype)
+        bound = _silu_bound(gate, up) * (1 + 2.0**-7) + f.eps / 2 * want.abs() + f.eps * f.tiny / 2
+        over = (y - want[:, None]).abs().amax(1) - bound
+        assert bool((over <= 0).all()), [(float(g), float(v), float(w)) for g, v, w, o in zip(gate, y[:, 0], want, over)
+                                         if float(o) > 0][:8]
