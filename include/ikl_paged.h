@@ -548,8 +548,9 @@ int ikl_add_rms_norm_int8(const ikl_norm_int8_args *args, void *stream);
  * x: F16 or BF16 rows, or rows in 8 bits with x_scales (contiguous as above).
  * Group sums are fp32 (of 8-bit rows exact whole numbers, scaled in fp32) and
  * their sum is fp32, rounded once to y's dtype, after the activation or
- * residual + it (y may be residual). A row of x with a NaN or an infinity
- * gives NaN or infinities. */
+ * residual + it (y may be residual). Group sums of finite 16-bit rows are
+ * finite up to the largest values of their type. A row of x with a NaN or an
+ * infinity gives NaN or infinities. */
 typedef struct ikl_int4_linear_args {
   const void *x;         /* rows 16-byte aligned */
   const float *x_scales; /* NULL: x in `dtype` */

@@ -7,8 +7,11 @@
 // up to 15, exact in every operand type: what is rounded is the fp32 sums.
 // Over 16-bit rows a code reaches its operand through the E4M3 form of its
 // byte: 0 .. 15 read as E4M3 are code * 2^-9 (subnormals, then the first
-// binade, whose step is the same), so one conversion with a scale of 2^9
-// turns two of them into 16-bit numbers. Over 8-bit rows z is taken off the
+// binade, whose step is the same), so one conversion with a scale turns two of
+// them into 16-bit numbers: beside fp16 rows the codes themselves (scale 2^9),
+// beside bf16 ones, which reach fp32's largest values, codes * 2^-11 (scale
+// 2^-2), so that a group's sums, 128 * 15 * 2^-11 of the largest value at most,
+// stay finite. s carries what is missing. Over 8-bit rows z is taken off the
 // bytes themselves.
 #pragma once
 
@@ -75,24 +78,29 @@ __device__ inline f32x2_t row_scale(float a) {
 }
 
 // ------------------------------------------------------------- operands
+// HELD: what a code is held at in an operand; ONES: two 16-bit numbers of it.
 template <typename XT>
 struct codes_as;
 template <>
 struct codes_as<bf16_tag> {
+  static constexpr float HELD = 0x1p-11f;
+  static constexpr uint32_t ONES = 0x3a003a00u;
   __device__ static inline uint32_t two(uint32_t w, bool high) {
-    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.f, true))
-                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.f, false));
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.f * HELD, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.f * HELD, false));
   }
 };
 template <>
 struct codes_as<f16_tag> {
+  static constexpr float HELD = 1.f;
+  static constexpr uint32_t ONES = 0x3c003c00u;
   __device__ static inline uint32_t two(uint32_t w, bool high) {
-    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 512.f, true))
-                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 512.f, false));
+    return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 512.f * HELD, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 512.f * HELD, false));
   }
 };
 
-// The 8 codes of a dword as an operand of 16-bit numbers 0 .. 15.
+// The 8 codes of a dword, times HELD, as an operand.
 template <typename XT>
 __device__ inline v4u32 unpack16(uint32_t w) {
   const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
@@ -113,15 +121,28 @@ __device__ inline u32x2_t unpack8_sixteenfold(uint32_t w) {
   return u32x2_t{((w << 4) & 0xf0f0f0f0u) ^ 0x80808080u, (w & 0xf0f0f0f0u) ^ 0x80808080u};
 }
 
-// The 8 codes less z, times 2^-9, as 16-bit numbers, all exact: z9 = z * 2^-9.
+// The 8 codes less z as 16-bit numbers, all exact, at 2^-11 (bf16) or 2^-9
+// (fp16, which has no normal numbers below 2^-14): zh is z at the same.
 template <typename XT>
-__device__ inline v4u32 unpack16_less(uint32_t w, float z9) {
+constexpr float LESS_HELD = __is_same(XT, bf16_tag) ? 0x1p-11f : 0x1p-9f;
+template <typename XT>
+__device__ inline v4u32 unpack16_less(uint32_t w, float zh) {
   const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
-  const f32x2_t f[4] = {__builtin_amdgcn_cvt_pk_f32_fp8((int)lo, false), __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, true),
-                        __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, false), __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, true)};
+  f32x2_t f[4];
+  if constexpr (__is_same(XT, bf16_tag)) {
+    f[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(lo, 0.25f, false);
+    f[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(lo, 0.25f, true);
+    f[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 0.25f, false);
+    f[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 0.25f, true);
+  } else {
+    f[0] = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, false);
+    f[1] = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, true);
+    f[2] = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, false);
+    f[3] = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, true);
+  }
   v4u32 v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = mfma_ops<XT>::pack(f[i][0] - z9, f[i][1] - z9);
+  for (int i = 0; i < 4; ++i) v[i] = mfma_ops<XT>::pack(f[i][0] - zh, f[i][1] - zh);
   return v;
 }
 

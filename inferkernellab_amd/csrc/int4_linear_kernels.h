@@ -7,6 +7,14 @@
 namespace ikl {
 namespace {
 
+// What the scales of W carry beside their values, 8-bit rows' in the few rows'
+// kernel at the end.
+template <typename XT, bool LESS, bool Z>
+constexpr float scale_carries() {
+  if constexpr (__is_same(XT, i8_tag)) return S_CARRIES<Z>;
+  else return 1.f / (LESS ? LESS_HELD<XT> : codes_as<XT>::HELD);
+}
+
 // --------------------------------------------------------------- few rows
 constexpr int ROW_WAVES = 8;
 
@@ -101,7 +109,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
     for (int g = 0; g < GPS; ++g) {
       if (GPS > 1 && s * GPS + g >= p.groups) continue;  // the contraction ends inside the step
       if constexpr (!I8) {
-        const v4u32 ones = {mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2};
+        const v4u32 ones = {codes_as<XT>::ONES, codes_as<XT>::ONES, codes_as<XT>::ONES, codes_as<XT>::ONES};
         f32x4_t X[MT];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -114,6 +122,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
           v4u32 a[DPG];
 #pragma unroll
           for (int i = 0; i < DPG; ++i) a[i] = unpack16<XT>(t.w[n][g * DPG + i]);
+          const f32x4_t sc = t.sc[n][g] * scale_carries<XT, false, Z>();
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             f32x4_t P = {0.f, 0.f, 0.f, 0.f};
@@ -122,7 +131,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float z = Z ? (float)((t.z[n][g] >> (8 * i)) & 0xffu) : 8.f;
-              acc[n][m][i] = fmaf(t.sc[n][g][i], fmaf(-z, X[m][i], P[i]), acc[n][m][i]);
+              acc[n][m][i] = fmaf(sc[i], fmaf(-z, X[m][i], P[i]), acc[n][m][i]);
             }
           }
         }
@@ -177,7 +186,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int m = 0; m < MT; ++m)
-      *reinterpret_cast<f32x4_t *>(red[wave][n * MT + m][lane]) = I8 ? acc[n][m] * S_CARRIES<Z> : acc[n][m];
+      *reinterpret_cast<f32x4_t *>(red[wave][n * MT + m][lane]) = I8 ? acc[n][m] * scale_carries<XT, false, Z>() : acc[n][m];
   __syncthreads();
   // lane l of an accumulator: columns 4 (l / 16) + i, row l % 16
   const int per = p.gated ? 2 : 1;
@@ -241,7 +250,7 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
   static_assert(LOADS >= 1, "every wave loads");
   // what s carries beside the column's scale
   constexpr bool LESS = !I8 && MT > 4;  // codes less their zero points
-  constexpr float SCALE = I8 ? S_CARRIES<Z> : LESS ? 512.f : 1.f;
+  constexpr float SCALE = scale_carries<XT, LESS, Z>();
   // At most 80 KB, for two workgroups on a CU: the rows' steps (at the end each
   // wave's accumulators of a row tile), a of the rows and less MAGIC times it
   // (groups of 32: a alone), the columns' scales and zero points, the codes.
@@ -389,7 +398,7 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
         uint32_t z = 0;
         if constexpr (Z && (I8 || LESS)) {  // of this lane's row of W
           z = wz[sb][(wave * GPS + g) * 16 * WT + 16 * n + hl];
-          z = I8 ? z * 0x01010101u : __float_as_uint((float)z * 0x1p-9f);
+          z = I8 ? z * 0x01010101u : __float_as_uint((float)z * LESS_HELD<XT>);
         }
 #pragma unroll
         for (int i = 0; i < DPG; ++i) {
@@ -399,7 +408,7 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
             a[n][i / 2][2 * (i & 1)] = v[0];
             a[n][i / 2][2 * (i & 1) + 1] = v[1];
           } else {
-            a[n][i] = LESS ? unpack16_less<XT>(d, Z ? __uint_as_float(z) : 8.f * 0x1p-9f) : unpack16<XT>(d);
+            a[n][i] = LESS ? unpack16_less<XT>(d, Z ? __uint_as_float(z) : 8.f * LESS_HELD<XT>) : unpack16<XT>(d);
           }
         }
       }
@@ -441,7 +450,7 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
           if (AHEAD && m + 1 < MT) read(m + 1);
           f32x4_t X = {0.f, 0.f, 0.f, 0.f};
           if constexpr (!LESS) {
-            const v4u32 ones = {mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2, mfma_ops<XT>::ONE2};
+            const v4u32 ones = {codes_as<XT>::ONES, codes_as<XT>::ONES, codes_as<XT>::ONES, codes_as<XT>::ONES};
 #pragma unroll
             for (int i = 0; i < DPG; ++i) X = mfma_ops<XT>::mma_k32(ones, xv[i], X);
           }

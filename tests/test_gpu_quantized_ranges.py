@@ -95,3 +95,48 @@ def test_gated_products_of_gates_far_from_0(kind, rows):
         over = (y - want[:, None]).abs().amax(1) - bound
         assert bool((over <= 0).all()), [(float(g), float(v), float(w)) for g, v, w, o in zip(gate, y[:, 0], want, over)
                                          if float(o) > 0][:8]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("rows,outs,cols,group", [(3, 80, 256, 128), (16, 20000, 256, 64), (40, 2064, 384, 32),
+                                                  (130, 2070, 384, 128), (300, 2064, 640, 64), (520, 9000, 384, 128),
+                                                  (6200, 5000, 320, 64), (6200, 4998, 384, 128)])
+def test_16_bit_rows_up_to_their_largest_values(rows, outs, cols, group, zeros, dtype):
+    """Whose products are finite: group sums, with or without the zero point, are too."""
+    from inferkernellab_amd import int4_linear_hip
+    from tests.test_gpu_quantized import _assert_close, _expected, _gen, _sums16, _weight
+
+    gen = _gen(rows + outs)
+    packed, w, mag = _weight(gen, outs, cols, group, zeros=zeros, dtype=FP32)
+    packed.scales.mul_(2.0**-16)
+    w, mag = w * 2.0**-16, mag * 2.0**-16
+    most = torch.finfo(dtype).max
+    x = ((torch.rand(rows, cols, generator=gen, device="cuda", dtype=torch.float64) * 2 - 1) * most).to(dtype)
+    x[0], x[1, ::2], x[1, 1::2], x[2] = most, most, -most, -most
+    xd = x.double()
+    want, bound = _expected(xd, w, _sums16(xd, mag, group), None, False, dtype)
+    got = int4_linear_hip(x, packed)
+    assert bool(got.isfinite().all())
+    _assert_close(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,outs", [(3, 80), (130, 2070), (6200, 5000)])
+def test_16_bit_rows_below_the_normal_numbers(rows, outs, dtype):
+    """Products of subnormal values with codes are kept, whatever power of two
+    the codes are held at: of bf16 they are whole numbers of 2^-133 times 2^-11,
+    below 2^24 of them in a group, so that nothing of them is rounded."""
+    from inferkernellab_amd import int4_linear_hip
+    from tests.test_gpu_quantized import _assert_close, _expected, _gen, _sums16, _weight
+
+    f = torch.finfo(dtype)
+    gen = _gen(rows)
+    packed, w, mag = _weight(gen, outs, 320, 64, zeros=True, dtype=FP32)
+    up = 2.0**100 if dtype == BF16 else 2.0**10
+    packed.scales.mul_(up)
+    w, mag = w * up, mag * up
+    x = (torch.randint(-60, 61, (rows, 320), generator=gen, device="cuda").double() * f.tiny * f.eps).to(dtype)
+    xd = x.double()
+    want, bound = _expected(xd, w, _sums16(xd, mag, 64), None, False, dtype)
+    _assert_close(int4_linear_hip(x, packed), want, bound)
