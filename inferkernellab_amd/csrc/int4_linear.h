@@ -65,15 +65,20 @@ typedef int i32x4_t __attribute__((ext_vector_type(4)));
 // below 2^22 (of codes times 16 without zero points: below 2^21) on top of
 // MAGIC, the bits of 1.5 * 2^23 as a float: the number as a float, without a
 // conversion. What turns it into its share of y are two multiply-adds: first
-// times a of its row less MAGIC times a, which is exact because a is held to
-// 22 significant bits (less than 2^-21 of it lost, as in four fp32 operations),
-// then times s of its column. a carries 2^-17 and s 2^17 (without zero points
-// 2^13), so that MAGIC * a stays finite up to fp32's largest value over 127.
+// times a of its row less MAGIC times a, which is exact because a is rounded to
+// 22 significant bits (to the nearest: 2^-22 of it at most, as in two fp32
+// operations), then times s of its column. a carries 2^-17 and s 2^17
+// (without zero points 2^13), so that MAGIC * a stays finite up to fp32's
+// largest value over 127.
 constexpr int MAGIC = 0x4b400000;
 template <bool Z>
 constexpr float S_CARRIES = Z ? 0x1p17f : 0x1p13f;
 __device__ inline f32x2_t row_scale(float a) {
-  a = __uint_as_float(__float_as_uint(a) & ~3u) * 0x1p-17f;
+#pragma clang fp contract(off)
+  a *= 0x1p-17f;
+  // Dekker's split: the sum and difference with 4 times more round a to 24 - 2 bits
+  const float more = a * 5.f, less = a - more;
+  a = more + less;
   return f32x2_t{a, a * -12582912.f};
 }
 
