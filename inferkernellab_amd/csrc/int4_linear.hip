@@ -58,9 +58,11 @@ bool few_rows(int64_t rows, int tiles, int steps, bool gated, bool eight, Int4Pl
 // to 28672 and 1024 to 14336 (groups of 128, zero points), of which each form and
 // split was measured: what is taken was 0.6 (16-bit rows) and 0.9 % (8-bit)
 // slower than the fastest in the mean, 38 % at most (40 x 1024 x 9000).
+// No blocks: no form's fit in a grid.
 Int4Plan plan_of(int64_t rows, int tiles, int steps, bool gated, bool eight) {
   Int4Plan best{};
   if (few_rows(rows, tiles, steps, gated, eight, best)) return best;
+  best = {};
   struct Form {
     int mt, nt, slots;
     double alone[2], tile[2];  // of a step: 16-bit rows, 8-bit rows
@@ -73,6 +75,7 @@ Int4Plan plan_of(int64_t rows, int tiles, int steps, bool gated, bool eight) {
   double least = 1e30;
   for (const Form &f : forms) {
     const int64_t blocks = blocks_of(rows, tiles, f.mt, f.nt);
+    if (blocks > max_grid(256)) continue;
     auto step = [&](int n) {
       const double work = n * f.mt * f.nt * f.tile[eight];
       return n == 0 ? 0. : work > f.alone[eight] ? work : f.alone[eight];
@@ -110,8 +113,14 @@ int check_args(const ikl_int4_linear_args *a) {
   if (a->cols % a->group != 0 || a->cols >= (1 << 24) || a->out_cols >= (1 << 24))
     return fail(IKL_EUNSUPPORTED, "int4 linear: cols must be whole groups; cols and out_cols below 2^24");
   if (a->gated && a->residual) return fail(IKL_EUNSUPPORTED, "int4 linear: a gated weight takes no residual");
-  if (a->rows > max_grid(256) / ((a->out_cols + 15) / 16)) return fail(IKL_EINVAL, "int4 linear: too many rows for a launch");
   return IKL_OK;
+}
+
+// check_args, then the plan of a launch that has rows.
+int plan_args(const ikl_int4_linear_args *a, Int4Plan &plan) {
+  if (const int bad = check_args(a)) return bad;
+  if (a->rows < int64_t(1) << 40) plan = plan_of(a->rows, tiles_of(a), steps_of(a), a->gated != 0, a->x_scales != nullptr);
+  return plan.blocks || !a->rows ? IKL_OK : fail(IKL_EINVAL, "int4 linear: too many rows for a launch");
 }
 
 }  // namespace
@@ -120,12 +129,14 @@ int check_args(const ikl_int4_linear_args *a) {
 using namespace ikl;
 
 extern "C" int64_t ikl_int4_linear_workspace_size(const ikl_int4_linear_args *a) {
-  if (const int bad = check_args(a)) return bad;
-  return part_bytes(a, plan_of(a->rows, tiles_of(a), steps_of(a), a->gated != 0, a->x_scales != nullptr));
+  Int4Plan plan{};
+  if (const int bad = plan_args(a, plan)) return bad;
+  return part_bytes(a, plan);
 }
 
 extern "C" int ikl_int4_linear(const ikl_int4_linear_args *a, void *stream) {
-  if (const int bad = check_args(a)) return bad;
+  Int4Plan plan{};
+  if (const int bad = plan_args(a, plan)) return bad;
   if (a->rows == 0) return IKL_OK;
   const int64_t eb = a->dtype == IKL_F32 ? 4 : 2;
   if (!a->x || !a->codes || !a->scales || !a->y) return fail(IKL_EINVAL, "int4 linear: NULL tensor pointer");
@@ -155,7 +166,6 @@ extern "C" int ikl_int4_linear(const ikl_int4_linear_args *a, void *stream) {
   p.gated = a->gated != 0;
   p.dtype = a->dtype;
   p.wide = (((uintptr_t)p.y | (uintptr_t)p.y_st | (uintptr_t)p.res | (p.res ? (uintptr_t)p.res_st : 0)) & (uintptr_t)(4 * eb - 1)) == 0;
-  const Int4Plan plan = plan_of(a->rows, p.tiles, p.steps, a->gated != 0, a->x_scales != nullptr);
   if (const int64_t need = part_bytes(a, plan)) {
     if (!a->workspace || off16(a->workspace) || a->workspace_bytes < need)
       return fail(IKL_EWORKSPACE, "int4 linear: the workspace is missing, too small or not 16-byte aligned");

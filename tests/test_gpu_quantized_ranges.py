@@ -188,3 +188,30 @@ def test_any_nan_or_infinity_as_the_scale_of_a_row(rows, zeros):
         keep = [r for r in range(rows) if r != 1]
         xd = q[keep].double() * scales[keep].double().repeat_interleave(64, 1)
         _assert_close(y[keep], *_expected(xd, w, _sums8(q[keep], scales[keep], w, 64), None, False, FP32))
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("gated", [False, True])
+def test_a_long_prompt_by_a_wide_layer(gated, eight):
+    """20001 rows by 14336 columns: more 16-column tiles of rows than threads of a
+    grid over 256."""
+    from inferkernellab_amd import int4_linear_hip, quantize_rows_int8_hip
+    from tests.test_gpu_quantized import _assert_close, _expected, _gen, _sums8, _sums16, _weight
+
+    gen, rows = _gen(3), 20001
+    packed, w, mag = _weight(gen, 14336 * (2 if gated else 1), 128, 64, zeros=gated, gated=gated)
+    x = torch.randn(rows, 128, generator=gen, device="cuda").to(BF16)
+    given = quantize_rows_int8_hip(x, group_size=64) if eight else x
+    y = int4_linear_hip(given, packed)
+    assert y.shape == (rows, 14336)
+    for start in (0, 18700, rows - 65):  # around the last row that the count of tiles once held
+        part = slice(start, start + 65)
+        if eight:
+            codes, scales = given.codes[part], given.scales[part]
+            xd = codes.double() * scales.double().repeat_interleave(64, 1)
+            sums = _sums8(codes, scales, w, 64)
+        else:
+            xd = x[part].double()
+            sums = _sums16(xd, mag, 64)
+        want, bound = _expected(xd, w, sums, None, gated, BF16)
+        _assert_close(y[part], want, bound)

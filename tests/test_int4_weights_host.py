@@ -1,9 +1,12 @@
-"""4-bit weights that a caller lays out: their memory is their own. On the CPU."""
+"""4-bit weights on the CPU: a packed weight's memory is its own; the largest
+products that have a plan."""
+
+import ctypes
 
 import pytest
 import torch
 
-from inferkernellab_amd import pack_int4_weight
+from inferkernellab_amd import _lib, pack_int4_weight
 
 ALIGNMENT = {"codes": 16, "scales": 16, "zeros": 4}  # bytes, of ikl_int4_linear
 
@@ -26,3 +29,33 @@ def test_a_packed_weight_shares_no_memory_with_what_it_was_packed_from(group, co
     for t in (codes, scales, zeros):
         t.zero_()
     assert torch.equal(w.dequantize(), want)
+
+
+def _linear(rows, cols, outs, **kw):
+    a = _lib.Int4LinearArgs()
+    a.x = a.codes = a.scales = a.y = 1 << 20  # an aligned address that nothing reads
+    a.rows, a.cols, a.out_cols, a.x_stride, a.y_stride = rows, cols, outs, cols, outs
+    a.group, a.dtype = 128, _lib.IKL_BF16
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("rows,cols,outs,gated", [
+    (18725, 4096, 14336, 0), (32768, 4096, 14336, 1), (4096, 4096, 128256, 0), (131072, 14336, 28672, 0),
+    (1 << 24, 128, 4096, 0), ((1 << 31) - 128, 128, 16, 0)])
+def test_products_of_many_rows_and_columns_have_a_plan(rows, cols, outs, gated, eight):
+    """Long prompts, wide layers, a head's columns: as long as blocks of some form
+    fit in a grid of fewer than 2^32 threads."""
+    a = _linear(rows, cols, outs, gated=gated, x_scales=(1 << 20) if eight else None)
+    assert _lib.load().ikl_int4_linear_workspace_size(ctypes.byref(a)) >= 0, _lib.last_error()
+
+
+@pytest.mark.parametrize("rows,outs", [((1 << 31) + 1, 16), (1 << 40, 16), (1 << 62, 4096), ((1 << 63) - 1, 1)])
+def test_products_that_no_grid_holds_are_refused(rows, outs):
+    lib = _lib.load()
+    a = _linear(rows, 128, outs)
+    assert lib.ikl_int4_linear_workspace_size(ctypes.byref(a)) == _lib.IKL_EINVAL
+    assert lib.ikl_int4_linear(ctypes.byref(a), None) == _lib.IKL_EINVAL
+    assert "too many rows" in _lib.last_error()
