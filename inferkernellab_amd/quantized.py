@@ -388,7 +388,9 @@ def quantize_int4_weight(weight: torch.Tensor, *, group_size: int = 128, symmetr
         low, span = None, w.abs().amax(-1) / 7
     else:
         low = w.amin(-1).clamp(max=0)
-        span = (w.amax(-1).clamp(min=0) - low) / 15
+        high = w.amax(-1).clamp(min=0)
+        span = (high - low) / 15
+        span = torch.where(span.isfinite(), span, high / 15 - low / 15)  # a range past fp32's largest value
     # A zero group divides by its step too. A step below fp16's normal numbers may
     # have been rounded down by more than the codes' range has to spare.
     least = torch.finfo(weight.dtype).smallest_normal if weight.dtype != torch.float16 else 2.0 ** -24

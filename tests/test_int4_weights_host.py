@@ -1,12 +1,12 @@
 """4-bit weights on the CPU: a packed weight's memory is its own; the largest
-products that have a plan."""
+products that have a plan; rounding weights of any finite size."""
 
 import ctypes
 
 import pytest
 import torch
 
-from inferkernellab_amd import _lib, pack_int4_weight
+from inferkernellab_amd import Int4Weight, _lib, pack_int4_weight, quantize_int4_weight
 
 ALIGNMENT = {"codes": 16, "scales": 16, "zeros": 4}  # bytes, of ikl_int4_linear
 
@@ -59,3 +59,27 @@ def test_products_that_no_grid_holds_are_refused(rows, outs):
     assert lib.ikl_int4_linear_workspace_size(ctypes.byref(a)) == _lib.IKL_EINVAL
     assert lib.ikl_int4_linear(ctypes.byref(a), None) == _lib.IKL_EINVAL
     assert "too many rows" in _lib.last_error()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("symmetric", [False, True])
+def test_weights_up_to_the_largest_values_are_rounded_to_finite_ones(dtype, symmetric):
+    """A group's range may be past its type's largest value; its steps are not.
+    Half a step of each weight and half of its zero point, the step rounded to
+    the type, in 64 bits."""
+    most = torch.finfo(dtype).max
+    gen = torch.Generator().manual_seed(4)
+    w = ((torch.rand(6, 64, generator=gen, dtype=torch.float64) * 2 - 1) * most).to(dtype)
+    w[1, 0], w[1, 1], w[2, 0] = most, -most, -most
+    g = w.double().view(6, -1, 32)
+    q = quantize_int4_weight(w, group_size=32, symmetric=symmetric)
+    if symmetric:
+        step = g.abs().amax(-1, keepdim=True) / 7
+    else:
+        step = (g.amax(-1, keepdim=True).clamp(min=0) - g.amin(-1, keepdim=True).clamp(max=0)) / 15
+    bound = step * ((0.5 if symmetric else 1.0) + 15 * torch.finfo(dtype).eps / 2 + 2.0**-20)
+    # what a code stands for may lie half a step past fp32's largest value: codes less zero points, and steps
+    units = Int4Weight(q.codes, torch.ones_like(q.scales), q.zeros, 6, 64, 32, False, torch.float32)
+    steps = q.scales[0, :2, :6].t().double()[..., None]
+    assert bool(steps.isfinite().all())
+    assert bool(((units.dequantize().double().view(6, 2, 32) * steps - g).abs() <= bound).all())
