@@ -411,7 +411,7 @@ int ikl_hbm_read_probe(const void *buffer, int64_t bytes, void *sink, int64_t si
  * here). A caller compares it with IKL_ABI_VERSION of the header it was
  * built against and refuses to run on a mismatch. No counterpart in the
  * reference, whose operators are Python functions. */
-#define IKL_ABI_VERSION 5
+#define IKL_ABI_VERSION 6
 int32_t ikl_abi_version(void);
 
 /* Findings of ikl_check_metadata, a bit each. */
@@ -572,6 +572,12 @@ int ikl_int4_linear(const ikl_int4_linear_args *args, void *stream);
 /* Bytes of workspace that ikl_int4_linear needs with these arguments (0 when
  * it splits no contraction over workgroups). Negative on invalid arguments. */
 int64_t ikl_int4_linear_workspace_size(const ikl_int4_linear_args *args);
+
+/* How ikl_int4_linear runs with these sizes, in a byte each from the lowest:
+ * parts that the contraction is split in over workgroups, 16-column and 16-row
+ * tiles of a workgroup, and 1 for the few rows' kernel. Planning only: tensors
+ * are not looked at. 0 without rows, negative on invalid sizes. */
+int32_t ikl_int4_linear_plan(const ikl_int4_linear_args *args);
 
 /* KV append (in place). Slots outside [0, num_blocks*block_size) are skipped,
  * never written. Replaces append.py:69-106 / cache.py:156-189. */

@@ -27,7 +27,7 @@ IKL_PREFILL_AUTO, IKL_PREFILL_ROWS = -1, 8  # plans of ikl_paged_prefill_plan
 IKL_CHECK_LENGTH_POSITIVE, IKL_CHECK_LENGTH_CAPACITY, IKL_CHECK_BLOCK_ID, IKL_CHECK_LENGTH_MAX = 1, 2, 4, 8
 # IKL_ABI_VERSION of the header these mirrors follow; load() refuses a
 # library that reports another
-IKL_ABI_VERSION = 5
+IKL_ABI_VERSION = 6
 
 EXPORTED_SYMBOLS = (
     "ikl_last_error",
@@ -60,6 +60,7 @@ EXPORTED_SYMBOLS = (
     "ikl_add_rms_norm_int8",
     "ikl_dequantize_rows_int8",
     "ikl_int4_linear",
+    "ikl_int4_linear_plan",
     "ikl_int4_linear_workspace_size",
     "ikl_quantize_rows_int8",
     "ikl_sample_tokens",
@@ -494,6 +495,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ikl_add_rms_norm_int8.argtypes = [ctypes.POINTER(NormInt8Args), _c_ptr]
     lib.ikl_int4_linear.restype = ctypes.c_int
     lib.ikl_int4_linear.argtypes = [ctypes.POINTER(Int4LinearArgs), _c_ptr]
+    lib.ikl_int4_linear_plan.restype = _c_i32
+    lib.ikl_int4_linear_plan.argtypes = [ctypes.POINTER(Int4LinearArgs)]
     lib.ikl_int4_linear_workspace_size.restype = _c_i64
     lib.ikl_int4_linear_workspace_size.argtypes = [ctypes.POINTER(Int4LinearArgs)]
     lib.ikl_qk_norm_rope_append_kv.restype = ctypes.c_int

@@ -134,6 +134,12 @@ extern "C" int64_t ikl_int4_linear_workspace_size(const ikl_int4_linear_args *a)
   return part_bytes(a, plan);
 }
 
+extern "C" int32_t ikl_int4_linear_plan(const ikl_int4_linear_args *a) {
+  Int4Plan plan{};
+  if (const int bad = plan_args(a, plan)) return bad;
+  return a->rows ? plan.split | plan.nt << 8 | plan.mt << 16 | plan.few << 24 : 0;
+}
+
 extern "C" int ikl_int4_linear(const ikl_int4_linear_args *a, void *stream) {
   Int4Plan plan{};
   if (const int bad = plan_args(a, plan)) return bad;
