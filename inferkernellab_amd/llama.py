@@ -457,13 +457,13 @@ class LlamaPagedDecodeRunner:
     def _int4_rows(self, x: torch.Tensor):
         return quantize_rows_int8_hip(x, group_size=self._int4.group_size) if self.int8_rows else x
 
-    def _int4_norm(self, norm, hidden: torch.Tensor, delta: torch.Tensor | None = None):
-        """(hidden + delta, norm of it as the 4-bit linears take it)."""
-        if self.int8_rows and self._norm_restated(norm, hidden, delta):
-            return add_rms_norm_int8_hip(hidden, delta, norm.weight, eps=norm.variance_epsilon,
-                                         group_size=self._int4.group_size)
-        hidden, x = self._add_norm(norm, hidden, delta)
-        return hidden, self._int4_rows(x.to(self.dtype))
+    def _int4_norm(self, norm, hidden: torch.Tensor):
+        """The norm of hidden as the 4-bit linears take it. (The residual's
+        addition is the products'.)"""
+        if self.int8_rows and self._norm_restated(norm, hidden, None):
+            return add_rms_norm_int8_hip(hidden, None, norm.weight, eps=norm.variance_epsilon,
+                                         group_size=self._int4.group_size)[1]
+        return self._int4_rows(self._add_norm(norm, hidden, None)[1].to(self.dtype))
 
     def _int4_qkv(self, w: Int4LlamaLayer, x):
         """q [..., H, D], k and v [..., Hkv, D], column ranges of one product."""
@@ -474,7 +474,7 @@ class LlamaPagedDecodeRunner:
     def _int4_tail(self, layer, w: Int4LlamaLayer, hidden: torch.Tensor, attended: torch.Tensor) -> torch.Tensor:
         """The layer behind its attention."""
         hidden = int4_linear_hip(self._int4_rows(attended), w.o, residual=hidden)
-        _, x = self._int4_norm(layer.post_attention_layernorm, hidden)
+        x = self._int4_norm(layer.post_attention_layernorm, hidden)
         return int4_linear_hip(self._int4_rows(int4_linear_hip(x, w.gate_up)), w.down, residual=hidden)
 
     def _prompt(self, request: InferenceRequest) -> tuple[int, ...]:
@@ -607,7 +607,7 @@ class LlamaPagedDecodeRunner:
             int4 = None if self._int4 is None else self._int4.layers[li]
             kernels = int4 is None and self._decode_linears(layer, hidden, delta)
             if int4 is not None:
-                hidden, x = self._int4_norm(layer.input_layernorm, hidden)
+                x = self._int4_norm(layer.input_layernorm, hidden)
                 q, k, v = self._int4_qkv(int4, x)
             else:
                 hidden, x = self._add_norm(layer.input_layernorm, hidden, delta, packed=kernels)
@@ -710,7 +710,7 @@ class LlamaPagedDecodeRunner:
             att = layer.self_attn
             int4 = None if self._int4 is None else self._int4.layers[li]
             if int4 is not None:
-                hidden, x = self._int4_norm(layer.input_layernorm, hidden)
+                x = self._int4_norm(layer.input_layernorm, hidden)
                 q, k, v = self._int4_qkv(int4, x)
             else:
                 hidden, x = self._add_norm(layer.input_layernorm, hidden, delta)
