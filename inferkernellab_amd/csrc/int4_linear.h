@@ -193,9 +193,12 @@ __device__ inline void finish_as(const Int4Params &p, int64_t row, int col, f32x
   }
 }
 
-// Four columns of y from `col` on, of sums v.
+// Four columns of y from `col` on, of sums v, over rows of XT: y is of 16-bit
+// rows' own type.
+template <typename XT>
 __device__ inline void finish(const Int4Params &p, int64_t row, int col, f32x4_t v) {
-  if (p.dtype == IKL_BF16) finish_as<bf16_tag>(p, row, col, v);
+  if constexpr (!__is_same(XT, i8_tag)) finish_as<XT>(p, row, col, v);
+  else if (p.dtype == IKL_BF16) finish_as<bf16_tag>(p, row, col, v);
   else if (p.dtype == IKL_F16) finish_as<f16_tag>(p, row, col, v);
   else finish_as<f32_tag>(p, row, col, v);
 }

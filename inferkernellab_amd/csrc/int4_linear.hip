@@ -7,7 +7,7 @@ namespace ikl {
 namespace {
 
 // Sums of a split contraction's parts, in their order, and the epilogue: a
-// thread four columns of a row.
+// thread four columns of a row, of any type.
 __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Params p, const int split, const int quads) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / quads;
   if (row >= p.rows) return;
@@ -20,7 +20,7 @@ __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Params p, cons
     if (p.gated) u += *reinterpret_cast<const f32x4_t *>(part + 16);
   }
   const int col = tile_col(p, tile, q);
-  if (col < p.outs) finish(p, row, col, p.gated ? gate_up(v, u) : v);
+  if (col < p.outs) finish<i8_tag>(p, row, col, p.gated ? gate_up(v, u) : v);
 }
 
 int64_t blocks_of(int64_t rows, int tiles, int mt, int nt) {

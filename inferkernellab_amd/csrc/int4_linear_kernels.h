@@ -204,7 +204,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
     const int64_t row = row0 + r;
     if (row >= p.rows || tile0 + n >= p.tiles) continue;
     const int col = tile_col(p, tile0 + n, c & 3);
-    if (col < p.outs) finish(p, row, col, p.gated ? gate_up(v[0], v[1]) : v[0]);
+    if (col < p.outs) finish<XT>(p, row, col, p.gated ? gate_up(v[0], v[1]) : v[0]);
   }
 }
 
@@ -559,7 +559,7 @@ __global__ __launch_bounds__(256, WT > 2 ? 2 : 3) void int4_tiles_kernel(const I
       }
       const int col = tile_col(p, tile0 + n, c & 3);
       if (col < p.outs)
-        finish(p, row, col, p.gated ? gate_up(v, *reinterpret_cast<const f32x4_t *>(at + 4 * ((4 * n + 4 + (c & 3)) ^ (r % CHUNKS)))) : v);
+        finish<XT>(p, row, col, p.gated ? gate_up(v, *reinterpret_cast<const f32x4_t *>(at + 4 * ((4 * n + 4 + (c & 3)) ^ (r % CHUNKS)))) : v);
     }
     wave_lds_sync();
   }
