@@ -18,12 +18,12 @@ def _silu(x):
 
 
 def _silu_bound(x, up):
-    """Of SiLU(x) * up in fp32: e^-|x| to an ulp and what its argument's two
-    products leave (a tenth of one), its sum with 1, the quotient and three
-    products (half an ulp each): 3.6 ulp. Below fp32's normal numbers e^-|x|,
-    its product with the quotient and SiLU are off by half of 2^-149 each, the
-    first two |x| times."""
-    return 3.6 * U * (_silu(x) * up).abs() + (x.abs() + 1) * 2.0**-149 * up.abs()
+    """Of SiLU(x) * up in fp32: e^-x to an ulp of the power of two and what its
+    argument's two products leave (each half a step of 2^-25, times ln 2: 0.17
+    ulp together), its sum with 1 half an ulp, the reciprocal one, two products
+    half an ulp each: 3.67. Below fp32's normal numbers the quotient, |x| times,
+    and SiLU are off by half of 2^-149 each."""
+    return 3.67 * U * (_silu(x) * up).abs() + (x.abs() + 1) * 2.0**-149 * up.abs()
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
