@@ -540,7 +540,8 @@ int ikl_add_rms_norm_int8(const ikl_norm_int8_args *args, void *stream);
  *          128 step + 32 i + 8 (l / 16)), of which code j < 4 is the low half
  *          of byte j, code 4 + j the high half. Codes past the contraction or
  *          the last column may be any.
- *   scales [tiles][S * 128 / group][16] fp32, 16-byte aligned
+ *   scales [tiles][S * 128 / group][16] fp32, 16-byte aligned; from 2^111 in
+ *          magnitude on y may be infinite where it need not be
  *   zeros  the same of uint8, 4-byte aligned
  * gated: even tiles hold a gate's rows and odd ones an up projection's, each
  * padded to whole tiles, and y = silu(x Wgate^T) * (x Wup^T).

@@ -51,7 +51,9 @@ bool few_rows(int64_t rows, int tiles, int steps, bool gated, bool eight, Int4Pl
 }
 
 // Many rows: the cheapest by an estimate of what bounds a launch. A CU runs
-// `slots` workgroups of a form at once: a round of them takes `start`, and for
+// `slots` workgroups of a form at once (as most of its kernels are compiled; {2, 8}
+// is 3 of 16-bit rows in groups of 128 with zero points, and {2, 8} and {4, 8} are 3
+// and 2 of 8-bit rows in groups of 32): a round of them takes `start`, and for
 // each step the longer of one workgroup's own time and of their tiles' work. A
 // split contraction saves steps and pays for a second launch and for the parts'
 // way through memory. Times in us, fitted to launches of 17 to 4096 rows by 512

@@ -33,7 +33,7 @@ struct RowsStep {
 // A workgroup owns NT tiles of 16 columns and MT tiles of 16 rows; its waves
 // split the contraction in steps of 128 and meet in LDS. Bound: the read of W
 // once, and below some 8 MB of it the latency of that read: DEPTH steps are on
-// their way in registers. 1 x 2048 to 2 x 5632 with SiLU * up 5.1 us, 32 x 4096
+// their way in registers. 1 x 2048 to 2 x 5632 with SiLU * up 5.5 us, 32 x 4096
 // to 14336 of 8-bit rows 11.7 (2.7 TB/s).
 //
 // 16-bit rows: z X of a group comes from a matrix product with a row operand
@@ -222,9 +222,9 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void int4_rows_kernel(const Int4Par
 //
 // Bound: the issue of vector instructions (a matrix instruction takes a slot
 // too): of a wave's step of 128 8-bit rows by 64 columns 256 multiply-adds of
-// the scales and 64 matrix instructions are 320 of 427 slots. 8192 x 4096 to
+// the scales and 64 matrix instructions are 320 of 429 slots. 8192 x 4096 to
 // 14336: 8-bit rows 567-608 us (1.6-1.7 POP/s; a library's int8 product 2.0 at
-// 8192^3), bf16 rows 930 us (1.03 PFLOP/s).
+// 8192^3), bf16 rows 930 us (1.03 PFLOP/s; 10 registers spill, with zero points 15).
 constexpr int VMCNT_0 = 0x0f70;  // s_waitcnt of vmcnt alone: its bits are 0-3 and 14-15
 typedef const __attribute__((address_space(1))) void *global_ptr;
 typedef __attribute__((address_space(3))) void *lds_ptr;

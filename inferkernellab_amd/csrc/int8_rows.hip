@@ -83,7 +83,8 @@ __device__ inline float group_amax(const float *v) {
 // leaves it in the low bits. 16-bit values meet ties often (a value and the
 // largest one have few bits, so 127 v / amax is a half exactly): EXACT takes
 // the quotient to its correct rounding, by its remainder, where one
-// multiplication would put them on either side.
+// multiplication would put them on either side. (A norm's products of two fp16
+// numbers have 22 bits, and 127 / 128 of them round: to 2^-16 of a step.)
 template <int N, bool EXACT>
 __device__ inline void codes_of(const float *v, float most, uint32_t *codes) {
   const float part = most * 0x1p-7f, inv = EXACT ? 1.f / part : 127.f / most;
