@@ -89,7 +89,8 @@ def _apart(x: torch.Tensor, y: torch.Tensor) -> bool:
 class Int8Rows:
     """Rows in 8 bits: ``codes`` ``[..., columns]`` int8, ``scales``
     ``[..., columns / group_size]`` float32; ``dtype`` is that of the rows
-    they came from."""
+    they came from. Contiguous ones, the codes 16-byte aligned, are held
+    themselves, others as copies: the attributes are what a product reads."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, group_size: int = 128, *,
                  dtype: torch.dtype = torch.bfloat16) -> None:
